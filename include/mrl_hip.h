@@ -702,6 +702,71 @@ int mrl_critic_loss_bwd_slope(const float* slope, int64_t batch, int64_t padded_
                               const float* upstream, float* g_head, void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * What stands on either side of the lm_head: the final norm of the hidden states, the token table,
+ * and the norm of all gradients.  The reference leaves these to the training framework below it.
+ *
+ * mrl_norm_fwd: y = (x - mu) * rstd * weight + bias per row of `hidden` entries, rstd = (mean (x - mu)^2
+ * + eps)^(-1/2), in fp32, rounded once.  subtract_mean = 1: layer norm (bias nullable); 0: RMS norm
+ * (mu = 0, bias NULL).  x: F32, BF16 or F16 with a row stride in elements, only read; y: the same type,
+ * dense; weight and bias: the rows' type or F32.  mean and rstd [n_rows] fp32, nullable, are what
+ * the backward takes.  A row with an infinity or NaN gives NaN in that row alone; squares of a row have to
+ * stay in fp32.  hidden at most MRL_NORM_MAX_HIDDEN. */
+#define MRL_NORM_MAX_HIDDEN 1048576
+int mrl_norm_fwd(const void* x, int dtype, int64_t n_rows, int64_t hidden, int64_t row_stride,
+                 const void* weight, const void* bias, int weight_dtype, int subtract_mean, float eps,
+                 void* y, float* mean, float* rstd, void* stream);
+
+/* mrl_norm_bwd: dx (dense, the rows' type), dweight and dbias (the weight's type), each nullable:
+ *   g = dy * weight, n = (x - mu) * rstd, dx = rstd * (g - mean g - n * mean(g n))   (RMS: without mean g)
+ *   dweight = sum over rows of dy * n, dbias = sum over rows of dy
+ * mean: the forward's, NULL for RMS norm.  Sums over rows are fp32, in an order that the sizes set: the same
+ * call gives the same bits.  workspace (for dweight or dbias): 16-byte aligned, no clearing needed.  Outputs share
+ * no memory with anything else. */
+int64_t mrl_norm_bwd_workspace_bytes(int64_t n_rows, int64_t hidden);
+int mrl_norm_bwd(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, int dtype,
+                 int64_t n_rows, int64_t hidden, const void* weight, int weight_dtype, const float* mean,
+                 const float* rstd, void* dx, void* dweight, void* dbias, void* workspace,
+                 int64_t workspace_bytes, void* stream);
+
+/* mrl_embedding_fwd: out[t] = scale * table[ids[t] - vocab_start], [n_tokens, hidden]; zeros where
+ * ids[t] - vocab_start is outside [0, vocab) (another rank's share of the table, or no token).  ids: I32 or
+ * I64; table [vocab, hidden] and out: F32, BF16 or F16, dense.  vocab_start >= 0. */
+int mrl_embedding_fwd(const void* ids, int ids_dtype, int64_t n_tokens, int64_t vocab_start,
+                      const void* table, int dtype, int64_t vocab, int64_t hidden, float scale, void* out,
+                      void* stream);
+
+/* mrl_embedding_bwd: dtable[v] = scale * (sum of dy[t] over the tokens with ids[t] - vocab_start == v), in fp32,
+ * rounded once; accumulate != 0: added to what dtable holds, and rows that no token names are not touched.
+ * dy [n_tokens, hidden] dense; dtable [vocab, hidden] of dy's type or F32.  Tokens are sorted by row and summed in
+ * that order: the same call gives the same bits.  workspace: 16-byte aligned, no clearing needed. */
+int64_t mrl_embedding_bwd_workspace_bytes(int64_t n_tokens, int64_t vocab, int64_t hidden);
+int mrl_embedding_bwd(const void* ids, int ids_dtype, int64_t n_tokens, int64_t vocab_start, const void* dy,
+                      int dtype, int64_t vocab, int64_t hidden, float scale, void* dtable, int dtable_dtype,
+                      int accumulate, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* mrl_grad_norm: norm[0] = sqrt(sum of g^2 over all entries of the tensors), squares and sums in fp64.  A list of
+ * at most MRL_GRAD_TENSORS tensors of F32, BF16 or F16, each of n dense entries (`out` and out_dtype are not looked
+ * at; an empty list gives 0).  The list is host memory and may be freed when the call returns: it travels in the
+ * kernels' arguments.  workspace: MRL_GRAD_NORM_PARTIALS doubles, no clearing needed.
+ *
+ * mrl_grad_clip: the same norm, then out = data * min(1, max_norm / (norm + 1e-6)) for every tensor, without a
+ * wait for the device in between.  out == data of the same dtype: in place, and left alone where the factor is 1.
+ * Else `out` has the gradient's type or F32.  What is written may not share memory with anything else in the list.
+ * A norm that is not finite gives the factor 0 or NaN, as the formula does. */
+#define MRL_GRAD_TENSORS 16384
+#define MRL_GRAD_NORM_PARTIALS 2048
+typedef struct mrl_grad {
+    const void* data;
+    void* out;
+    int64_t n;
+    int32_t dtype;
+    int32_t out_dtype;
+} mrl_grad;
+int mrl_grad_norm(const mrl_grad* grads, int64_t n_grads, float* norm, double* workspace, void* stream);
+int mrl_grad_clip(const mrl_grad* grads, int64_t n_grads, float max_norm, float* norm, double* workspace,
+                  void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * Plain device-to-device copy kernel of n_bytes (multiple of 16, 16-byte aligned pointers);
  * used to calibrate the rocprofv3 FETCH_SIZE / WRITE_SIZE counters and as the measured
  * bandwidth ceiling next to the 8 TB/s vendor peak.  No counterpart in the reference. */

@@ -7,11 +7,14 @@ or eager fallback.  Build the library with ``python -m mindspeed_rl_amd._build``
 from . import _lib
 from .advantage import (FixedKLController, compute_group_norm_advantage_return, dynamic_sampling_keep, get_last_reward,
                         dynamic_sampling_keep_mask)
+from .embedding import token_embedding, token_embedding_grad
 from .functional import clip_by_value, is_multimodal, masked_mean, masked_sum
+from .gradients import clip_grad_norm_, global_grad_norm
 from .lmhead import fused_lmhead_policy_loss, lmhead_logprob
 from .loss import (BaseLossFunc, DAPOActorLossFunc, DeferredStats, GradScaleState, GRPOActorLossFunc, LossFuncFactory, LossRegister,
                    MultimodalLogProbComputer, PPOActorLossFunc, ReferenceLossFunc, RewardLossFunc,
                    StandardLogProbComputer, fused_logprob_policy_loss, fused_supported, policy_loss)
+from .norms import layer_norm, rms_norm
 from .packing import (generate_mask, pack_index, postprocess_packed_seqs, preprocess_packed_seqs, response_window,
                       truncate_middle_and_pad, truncate_prompt_and_pad)
 from .seqlen_balancing import (balanced_bin_packing, get_reverse_idx, get_seqlen_balanced_partitions, heapq_partition,

@@ -112,13 +112,22 @@ SIGNATURES = {
     "mrl_critic_loss_fwd_slope_host": [_vp, _i64, _i64, _vp, _int, _vp, _int, _vp, _vp, _i64, _f32, _f32, _vp, _vp, _vp, _vp, _vp, _i64, _vp],
     "mrl_critic_loss_bwd_slope": [_vp, _i64, _i64, _vp, _int, _vp, _int, _i64, _f32, _vp, _vp, _vp, _vp],
     "mrl_value_loss_bwd": [_vp, _vp, _vp, _vp, _int, _vp, _int, _i64, _i64, _f32, _f32, _vp, _vp, _vp, _vp],
+    "mrl_norm_fwd": [_vp, _int, _i64, _i64, _i64, _vp, _vp, _int, _int, _f32, _vp, _vp, _vp, _vp],
+    "mrl_norm_bwd_workspace_bytes": [_i64, _i64],
+    "mrl_norm_bwd": [_vp, _i64, _vp, _i64, _int, _i64, _i64, _vp, _int, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp],
+    "mrl_embedding_fwd": [_vp, _int, _i64, _i64, _vp, _int, _i64, _i64, _f32, _vp, _vp],
+    "mrl_embedding_bwd_workspace_bytes": [_i64, _i64, _i64],
+    "mrl_embedding_bwd": [_vp, _int, _i64, _i64, _vp, _int, _i64, _i64, _f32, _vp, _int, _int, _vp, _i64, _vp],
+    "mrl_grad_norm": [_vp, _i64, _vp, _vp, _vp],
+    "mrl_grad_clip": [_vp, _i64, _f32, _vp, _vp, _vp],
     "mrl_copy_bytes": [_vp, _vp, _i64, _vp],
     "mrl_bandwidth_probe": [_int, _vp, _vp, _i64, _i64, _vp],
 }
 _RESTYPES = {"mrl_last_error": ctypes.c_char_p, "mrl_fused_workspace_bytes": ctypes.c_int64, "mrl_fused_max_vocab": ctypes.c_int64,
              "mrl_lmhead_workspace_bytes": ctypes.c_int64, "mrl_lmhead_static_max_tokens": ctypes.c_int64,
              "mrl_set_wide_spin_limit": ctypes.c_int64, "mrl_gae_whiten_workspace_bytes": ctypes.c_int64,
-             "mrl_value_loss_workspace_bytes": ctypes.c_int64, "mrl_lmhead_bwd_workspace_bytes": ctypes.c_int64}
+             "mrl_value_loss_workspace_bytes": ctypes.c_int64, "mrl_lmhead_bwd_workspace_bytes": ctypes.c_int64,
+             "mrl_norm_bwd_workspace_bytes": ctypes.c_int64, "mrl_embedding_bwd_workspace_bytes": ctypes.c_int64}
 
 _lib = None
 _entry = {}             # name -> bound function, looked up once

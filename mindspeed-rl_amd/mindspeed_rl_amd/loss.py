@@ -18,6 +18,7 @@ import torch
 
 from . import _lib, vocab_ops
 from .functional import is_multimodal
+from .norms import final_norm
 from .packing import (ResponseWindows, generate_mask, postprocess_packed_seqs, response_window,
                       truncate_middle_and_pad, truncate_prompt_and_pad)
 from .vocab_ops import compute_log_probs, vocab_logprob_entropy, vocab_parallel_entropy
@@ -494,6 +495,8 @@ class StandardLogProbComputer(LogProbComputer):
             # `output` holds the hidden states: the rows of the response windows are projected and scored
             # tile by tile on the matrix cores, no logits are written (forward only, no autograd)
             from . import lmhead
+            with torch.no_grad():
+                output = final_norm(output, kwargs)
             if own_cut and self._rows_in_windows is StandardLogProbComputer._rows_in_windows:
                 windows = self._windows(output, batch, kwargs)
                 scores = lmhead.score_windows(output, weight, labels, windows, inv_t, not skip_entropy)
@@ -548,6 +551,7 @@ class MultimodalLogProbComputer(LogProbComputer):
     gradient flows back through the sweep: no ``[B, L, V]`` copy in either direction."""
 
     def compute(self, output, batch, skip_entropy, **kwargs):
+        _refuse_norm_of_logits(kwargs)
         responses = batch["responses"]
         if output.dim() != 3:
             raise ValueError("output must have shape (mbs, seq_len, vocab_size)")
@@ -572,6 +576,11 @@ class MultimodalLogProbComputer(LogProbComputer):
         log_probs = truncate_prompt_and_pad(responses, row_logp, window, pad_value=pad)
         entropy = torch.zeros_like(log_probs) if skip_entropy else vocab_parallel_entropy(output)
         return log_probs, entropy
+
+
+def _refuse_norm_of_logits(kwargs):
+    if kwargs.get("final_norm_weight") is not None:
+        raise ValueError("final_norm_weight= needs lm_head_weight=: logits are not normalised")
 
 
 # ------------------------------------------------------------------------------------ loss objects
@@ -601,18 +610,21 @@ class BaseLossFunc(ABC):
     def _fused(self, output, kwargs):
         """The one-pass sweep scores rows against ``labels``: it stands in for the standard log-prob
         strategy only (a caller that installs another ``logprob_computer`` gets the split path)."""
+        _refuse_norm_of_logits(kwargs)
         return type(self.logprob_computer) is StandardLogProbComputer and _use_fused(output, kwargs)
 
     def _from_hidden(self, output, batch, kwargs, **loss_args):
         """The training step when the caller hands over the hidden states and ``lm_head_weight=``
         instead of logits (keyword arguments ``lm_head_chunk_rows``, ``lm_head_compact_rows``):
         logits exist for one chunk of rows at a time, and ``backward()`` reaches the hidden states
-        and the weight.  Forward-only calls take the same keyword through ``compute_log_probs``."""
+        and the weight.  Forward-only calls take the same keyword through ``compute_log_probs``.  With
+        ``final_norm_weight=`` the hidden states are those in front of the model's last norm
+        (:func:`norms.final_norm`), and ``backward()`` reaches its weight and bias as well."""
         from .lmhead import fused_lmhead_policy_loss
         if type(self.logprob_computer) is not StandardLogProbComputer:
             raise NotImplementedError("lm_head_weight= needs the standard log-prob strategy")
         return fused_lmhead_policy_loss(
-            output, kwargs["lm_head_weight"], batch, packed=kwargs.get("use_remove_padding", False),
+            final_norm(output, kwargs), kwargs["lm_head_weight"], batch, packed=kwargs.get("use_remove_padding", False),
             seqlens=kwargs.get("seqlens_in_batch"), cu_seqlens=kwargs.get("cu_seqlens_padded"),
             inv_temperature=float(kwargs.get("inv_temperature", 1.0)),
             expected_upstream=kwargs.get("expected_grad_scale"), scale_state=self.grad_scale_state(output.device),
@@ -633,6 +645,8 @@ class BaseLossFunc(ABC):
         return truncate_prompt_and_pad(batch["responses"], logprob, window)
 
     def compute_log_probs(self, output, batch: Dict[str, torch.Tensor], skip_entropy=True, **kwargs):
+        if kwargs.get("lm_head_weight") is None:
+            _refuse_norm_of_logits(kwargs)
         return self.logprob_computer.compute(output, batch, skip_entropy, **kwargs)
 
 

@@ -1,0 +1,104 @@
+"""Layer norm and RMS norm of hidden states, forward and backward: what a model's last stage does to the hidden states
+that :func:`lmhead_logprob` and the loss objects with ``lm_head_weight=`` take.
+
+The reference leaves them to the model below it; the loss objects call them with ``final_norm_weight=``.
+"""
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .vocab_ops import _flat_rows
+
+_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+
+
+class _Norm(torch.autograd.Function):
+    """(x[..., H], weight[H], bias[H] or None) -> y[..., H]; mean and rstd of the rows are kept for the backward."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, layer):
+        dev = x.device
+        hidden = x.shape[-1]
+        flat, x_stride = _flat_rows(x)
+        n_rows = flat.shape[0]
+        w, b = weight.contiguous(), None if bias is None else bias.contiguous()
+        y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        p_mean = p_rstd = None
+        if any(ctx.needs_input_grad[:3]):
+            stats = torch.empty((2 if layer else 1, n_rows), dtype=torch.float32, device=dev)
+            p_rstd = stats.data_ptr()
+            p_mean = p_rstd + 4 * n_rows if layer else None
+            ctx.save_for_backward(flat, w, stats)
+            ctx.meta = (x.shape, x_stride, layer, None if bias is None else bias.dtype)
+        _lib.call("mrl_norm_fwd", flat.data_ptr(), _lib.dtype_code(x), n_rows, hidden, x_stride, w.data_ptr(), _lib.ptr(b),
+                  _lib.dtype_code(w), 1 if layer else 0, eps, y.data_ptr(), p_mean, p_rstd, _lib.stream(dev))
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        flat, w, stats = ctx.saved_tensors
+        shape, x_stride, layer, has_bias = ctx.meta
+        dev = flat.device
+        n_rows, hidden = flat.shape
+        dy, dy_stride = _flat_rows(dy)
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        dx = torch.empty(shape, dtype=flat.dtype, device=dev) if need_x else None
+        dw = torch.empty(hidden, dtype=w.dtype, device=dev) if need_w else None
+        db = torch.empty(hidden, dtype=w.dtype, device=dev) if need_b and has_bias is not None else None
+        ws_bytes = _lib.load().mrl_norm_bwd_workspace_bytes(n_rows, hidden) if need_w or need_b else 0
+        workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+        p_rstd = stats.data_ptr()
+        _lib.call("mrl_norm_bwd", dy.data_ptr(), dy_stride, flat.data_ptr(), x_stride, _lib.dtype_code(flat), n_rows, hidden,
+                  w.data_ptr(), _lib.dtype_code(w), p_rstd + 4 * n_rows if layer else None, p_rstd, _lib.ptr(dx), _lib.ptr(dw),
+                  _lib.ptr(db), _lib.ptr(workspace), ws_bytes, _lib.stream(dev))
+        return dx, dw, db, None, None
+
+
+def _norm(x, weight, bias, eps, layer):
+    if x.dtype not in _FLOATS:
+        raise TypeError("x must be float32, bfloat16 or float16, not %s" % x.dtype)
+    if weight.dtype is not x.dtype and weight.dtype is not torch.float32:
+        raise TypeError("weight must have the type of x (%s) or float32, not %s" % (x.dtype, weight.dtype))
+    if x.dim() < 1 or x.shape[-1] < 1 or weight.dim() != 1 or weight.shape[0] != x.shape[-1]:
+        raise ValueError("weight must have the shape of x's last dimension: x %s, weight %s"
+                         % (tuple(x.shape), tuple(weight.shape)))
+    if bias is not None and (bias.shape != weight.shape or bias.dtype is not weight.dtype):
+        raise ValueError("bias must have the shape and type of weight: %s %s and %s %s"
+                         % (tuple(bias.shape), bias.dtype, tuple(weight.shape), weight.dtype))
+    eps = float(eps)
+    if not 0.0 < eps < float("inf"):
+        raise ValueError("eps must be positive and finite, not %r" % eps)
+    _lib.require_device(x, weight, bias)
+    return _Norm.apply(x, weight, bias, eps, layer)
+
+
+def layer_norm(x, weight, bias=None, eps=1e-5):
+    """``(x - mean) * (var + eps)^(-1/2) * weight + bias`` over the last dimension of ``x`` ``[..., H]`` (fp32, bf16
+    or fp16; rows of any stride), in fp32, rounded once to the type of ``x``.  ``weight`` and ``bias`` ``[H]`` have the type of
+    ``x`` or fp32.  Differentiable (once) with respect to all three; sums over rows are taken in an order that the
+    sizes set.  A row's squares have to stay in fp32: entries above 1.8e19 do not."""
+    return _norm(x, weight, bias, eps, True)
+
+
+def rms_norm(x, weight, eps=1e-6):
+    """``x * (mean(x^2) + eps)^(-1/2) * weight`` over the last dimension, otherwise as :func:`layer_norm`."""
+    return _norm(x, weight, None, eps, False)
+
+
+def final_norm(hidden, kwargs):
+    """The hidden states that the lm_head takes: ``hidden`` itself, or normalised if the caller of a loss object says
+    how (``final_norm_weight=``; ``final_norm_type=`` "rms" (default) or "layer", ``final_norm_bias=``, ``final_norm_eps=``)."""
+    weight = kwargs.get("final_norm_weight")
+    kind, bias = kwargs.get("final_norm_type", "rms"), kwargs.get("final_norm_bias")
+    if kind not in ("rms", "layer"):
+        raise ValueError("final_norm_type must be 'rms' or 'layer', not %r" % (kind,))
+    if weight is None:
+        if bias is not None:
+            raise ValueError("final_norm_bias= needs final_norm_weight=")
+        return hidden
+    if kind == "rms":
+        if bias is not None:
+            raise ValueError("final_norm_bias= needs final_norm_type='layer'")
+        return rms_norm(hidden, weight, kwargs.get("final_norm_eps", 1e-6))
+    return layer_norm(hidden, weight, bias, kwargs.get("final_norm_eps", 1e-5))
