@@ -6,7 +6,9 @@
 //   dw_j = sum_rows dy_j n_j,  db_j = sum_rows dy_j
 //
 // Everything is held in fp32 and rounded once, to the output's type.  Both passes are bound by memory.
+#include "lane_ops.h"
 #include "mrl_internal.h"
+#include "vector_access.h"
 #include "vocab_common.h"
 
 namespace {
@@ -127,9 +129,352 @@ __global__ __launch_bounds__(kBlock) void norm_columns_finish_kernel(const float
     if (dbias) Elem<WDT>::store(dbias + j, db);
 }
 
+// ------------------------------------------------------------------------------------ rows in registers
+// A team of 16 lanes or of whole wavefronts holds a row, kVecs vectors of 16 bytes a lane, so that every row is read
+// once.  The last vector of a row that is not whole vectors ends where the row ends and overlaps the one in front of it; lanes
+// behind it hold it again.  Entries that a lane holds twice over are left out of its sums (`skip` of them, from the front)
+// and written twice with the same bits, so that no access hides behind a branch: around a branch the compiler cannot count
+// what is on its way, and every wait would be one for all of it.
+struct Team {
+    int lanes, vecs;                        // 0 lanes: the row is not held
+};
+
+// Of a lane's vectors the last alone may lie behind the row.
+__host__ Team team_that_fits(int64_t nv, int64_t lanes, int vecs) {
+    return nv > (vecs - 1) * lanes && nv <= vecs * lanes ? Team{(int)lanes, vecs} : Team{0, 0};
+}
+
+constexpr int kMaxVecs = 4;
+
+
+int64_t vectors_of(int dtype, int64_t hidden) {
+    const int64_t vec = dtype == MRL_F32 ? 4 : 8;
+    return hidden < vec ? 0 : (hidden + vec - 1) / vec;
+}
+
+Team team_of(int dtype, int64_t hidden) {
+    const int64_t nv = vectors_of(dtype, hidden);
+    if (nv == 0) return {0, 0};
+    if (nv <= 64) return team_that_fits(nv, 16, (int)((nv + 15) / 16));
+    for (int lanes = 64; lanes <= 1024; lanes *= 2)
+        if (nv <= (int64_t)lanes * kMaxVecs) return team_that_fits(nv, lanes, (int)((nv + lanes - 1) / lanes));
+    return {0, 0};
+}
+
+// Where lane `tl` of a team finds its vector q, and how many entries of its last one are others'.
+template <int kVecs, int kVec>
+struct Columns {
+    int first, step, last, skip;
+    __device__ __forceinline__ Columns(int tl, int lanes, int hidden) {
+        const int at = (tl + (kVecs - 1) * lanes) * kVec;
+        first = tl * kVec;
+        step = lanes * kVec;
+        last = at < hidden - kVec ? at : hidden - kVec;
+        skip = at >= hidden ? kVec : at - last;
+    }
+    __device__ __forceinline__ int at(int q) const { return q < kVecs - 1 ? first + q * step : last; }
+    // entry i of vector q is this lane's
+    __device__ __forceinline__ bool own(int q, int i) const { return q < kVecs - 1 || i >= skip; }
+};
+
+// Sums of two values over a team, in all of its lanes.  `lds`: an entry per wavefront, not in use since the last barrier but
+// one.  Every thread of the workgroup calls it.
+__device__ __forceinline__ float2 team_sum2(float a, float b, int lanes, float2* lds) {
+    a = mrl::lanes_sum<4>(a);
+    b = mrl::lanes_sum<4>(b);
+    if (lanes == 16) return make_float2(a, b);
+    a = (mrl::lane_value(a, 0) + mrl::lane_value(a, 16)) + (mrl::lane_value(a, 32) + mrl::lane_value(a, 48));
+    b = (mrl::lane_value(b, 0) + mrl::lane_value(b, 16)) + (mrl::lane_value(b, 32) + mrl::lane_value(b, 48));
+    if (lanes == 64) return make_float2(a, b);
+    lds[threadIdx.x >> 6] = make_float2(a, b);
+    __syncthreads();
+    // the team's wavefronts' sums, one in each of 16 lanes
+    const int waves = lanes >> 6, first = (threadIdx.x >> 6) / waves * waves, w = threadIdx.x & 15;
+    const float2 s = w < waves ? lds[first + w] : make_float2(0.f, 0.f);
+    return make_float2(mrl::lanes_sum<4>(s.x), mrl::lanes_sum<4>(s.y));
+}
+
+template <int DT, int WDT, bool kLayer, int kVecs, bool kStream>
+__global__ __launch_bounds__(1024) void norm_fwd_rows_kernel(const typename Elem<DT>::T* __restrict__ x, int64_t x_stride,
+                                                             int64_t n_rows, int hidden, int lanes,
+                                                             const typename Elem<WDT>::T* __restrict__ weight,
+                                                             const typename Elem<WDT>::T* __restrict__ bias, float eps,
+                                                             typename Elem<DT>::T* __restrict__ y, float* __restrict__ mean,
+                                                             float* __restrict__ rstd) {
+    constexpr int kVec = Elem<DT>::kVec;
+    __shared__ float2 lds[2][16];
+    const int tl = threadIdx.x & (lanes - 1);
+    const int64_t wanted = (int64_t)blockIdx.x * (blockDim.x / lanes) + threadIdx.x / lanes;
+    const bool live = wanted < n_rows;
+    const int64_t row = live ? wanted : n_rows - 1;
+    const typename Elem<DT>::T* xr = x + row * x_stride;
+    typename Elem<DT>::T* yr = y + row * hidden;
+    const Columns<kVecs, kVec> col(tl, lanes, hidden);
+    u32x4 v[kVecs];
+#pragma unroll
+    for (int q = 0; q < kVecs; ++q) v[q] = kStream ? mrl::Vec<DT>::load_nt(xr + col.at(q)) : mrl::Vec<DT>::load(xr + col.at(q));
+    const float inv = 1.f / (float)hidden;
+    float mu = 0.f;
+    if (kLayer) {
+        float s = 0.f;
+#pragma unroll
+        for (int q = 0; q < kVecs; ++q) {
+            float z[kVec];
+            Elem<DT>::unpack(v[q], z);
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) s += col.own(q, i) ? z[i] : 0.f;
+        }
+        mu = team_sum2(s, 0.f, lanes, lds[0]).x * inv;
+    }
+    float ss = 0.f;
+#pragma unroll
+    for (int q = 0; q < kVecs; ++q) {
+        float z[kVec];
+        Elem<DT>::unpack(v[q], z);
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) {
+            const float d = z[i] - mu;
+            ss += col.own(q, i) ? d * d : 0.f;
+        }
+    }
+    const float r = 1.f / sqrtf(team_sum2(ss, 0.f, lanes, lds[1]).x * inv + eps);
+    if (!live) return;
+#pragma unroll
+    for (int q = 0; q < kVecs; ++q) {
+        float z[kVec], w[kVec];
+        Elem<DT>::unpack(v[q], z);
+        mrl::load_floats<WDT>(weight + col.at(q), w);
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) z[i] = (z[i] - mu) * r * w[i];
+        if (kLayer && bias) {
+            mrl::load_floats<WDT>(bias + col.at(q), w);
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) z[i] += w[i];
+        }
+        if (kStream) mrl::Vec<DT>::store_nt(yr + col.at(q), Elem<DT>::pack(z));
+        else mrl::Vec<DT>::store(yr + col.at(q), Elem<DT>::pack(z));
+    }
+    if (tl == 0) {
+        if (mean) mean[row] = mu;
+        if (rstd) rstd[row] = r;
+    }
+}
+
+// The backward in one pass: workgroups stay and take rows in turn, a team a row, and hold the sums over their rows of the
+// lane's columns in registers; the workgroup's sums go to part[group][2][hidden] (dw, db).  The next row's entries are on
+// their way while this one's are summed.  The weight stays in registers: a load of it behind the request for the next
+// row would wait for that as well.
+constexpr int kBwdBlock = 512;              // threads of a workgroup that holds several teams
+constexpr int kBwdGroups = 512;             // most workgroups: two on each of 256 CUs
+
+template <int DT, int WDT, bool kLayer, int kVecs, int kBlockMost, bool kStream>
+__global__ __launch_bounds__(kBlockMost) void norm_bwd_rows_kernel(
+    const typename Elem<DT>::T* __restrict__ dy, int64_t dy_stride, const typename Elem<DT>::T* __restrict__ x, int64_t x_stride,
+    int64_t n_rows, int hidden, int lanes, const typename Elem<WDT>::T* __restrict__ weight, const float* __restrict__ mean,
+    const float* __restrict__ rstd, typename Elem<DT>::T* __restrict__ dx, float* __restrict__ part) {
+    constexpr int kVec = Elem<DT>::kVec, kWVec = Elem<WDT>::kVec;
+    constexpr bool kOne = kBlockMost > kBwdBlock;       // the team is the workgroup
+    extern __shared__ float columns[];                  // [kVecs * kVec][lanes] sums on their way between teams
+    __shared__ float2 lds[2][16];
+    const int teams = kOne ? 1 : blockDim.x / lanes, team = kOne ? 0 : threadIdx.x / lanes;
+    const int tl = threadIdx.x - team * lanes;
+    const Columns<kVecs, kVec> col(tl, lanes, hidden);
+    const float inv = 1.f / (float)hidden;
+    float dw[kVecs][kVec] = {}, db[kVecs][kVec] = {};
+    u32x4 wv[kVecs][kVec / kWVec];
+#pragma unroll
+    for (int q = 0; q < kVecs; ++q)
+#pragma unroll
+        for (int p = 0; p < kVec / kWVec; ++p) wv[q][p] = mrl::Vec<WDT>::load(weight + col.at(q) + p * kWVec);
+    const auto unpack_weight = [&](int q, float (&w)[kVec]) {
+#pragma unroll
+        for (int p = 0; p < kVec / kWVec; ++p) {
+            float t[kWVec];
+            Elem<WDT>::unpack(wv[q][p], t);
+#pragma unroll
+            for (int i = 0; i < kWVec; ++i) w[p * kWVec + i] = t[i];
+        }
+    };
+    const int64_t step = (int64_t)gridDim.x * teams;
+    u32x4 xn[kVecs], gn[kVecs];
+    float mun, rn;
+    const auto request = [&](int64_t wanted) {
+        const int64_t row = wanted < n_rows ? wanted : n_rows - 1;
+        const typename Elem<DT>::T *xr = x + row * x_stride, *dyr = dy + row * dy_stride;
+        mun = kLayer ? mean[row] : 0.f;
+        rn = rstd[row];
+#pragma unroll
+        for (int q = 0; q < kVecs; ++q) {
+            xn[q] = kStream ? mrl::Vec<DT>::load_nt(xr + col.at(q)) : mrl::Vec<DT>::load(xr + col.at(q));
+            gn[q] = kStream ? mrl::Vec<DT>::load_nt(dyr + col.at(q)) : mrl::Vec<DT>::load(dyr + col.at(q));
+        }
+    };
+    request((int64_t)blockIdx.x * teams + team);
+    int turn = 0;
+    for (int64_t base = (int64_t)blockIdx.x * teams; base < n_rows; base += step, turn ^= 1) {
+        // teams behind the last row do that row again, without its share of the columns' sums
+        const bool counts = kOne || base + team < n_rows;
+        const int64_t row = counts ? base + team : n_rows - 1;
+        u32x4 xv[kVecs], gv[kVecs];
+#pragma unroll
+        for (int q = 0; q < kVecs; ++q) {
+            xv[q] = xn[q];
+            gv[q] = gn[q];
+        }
+        const float mu = mun, r = rn;
+        request(base + team + step);
+        float sg = 0.f, sgn = 0.f;
+#pragma unroll
+        for (int q = 0; q < kVecs; ++q) {
+            float z[kVec], g[kVec], w[kVec];
+            Elem<DT>::unpack(xv[q], z);
+            Elem<DT>::unpack(gv[q], g);
+            unpack_weight(q, w);
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) {
+                const float own = col.own(q, i) ? g[i] : 0.f, n = (z[i] - mu) * r;
+                const float add = counts ? own : 0.f;
+                dw[q][i] += add * n;
+                if (kLayer) db[q][i] += add;
+                sg += own * w[i];
+                sgn += own * w[i] * n;
+            }
+        }
+        const float2 sums = team_sum2(sg, sgn, lanes, lds[turn]);
+        const float c = kLayer ? sums.x * inv : 0.f, cn = sums.y * inv;
+        typename Elem<DT>::T* dxr = dx + row * hidden;
+#pragma unroll
+        for (int q = 0; q < kVecs; ++q) {
+            float z[kVec], g[kVec], w[kVec];
+            Elem<DT>::unpack(xv[q], z);
+            Elem<DT>::unpack(gv[q], g);
+            unpack_weight(q, w);
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) z[i] = r * (g[i] * w[i] - c - (z[i] - mu) * r * cn);
+            if (kStream) mrl::Vec<DT>::store_nt(dxr + col.at(q), Elem<DT>::pack(z));
+            else mrl::Vec<DT>::store(dxr + col.at(q), Elem<DT>::pack(z));
+        }
+    }
+    if (!part) return;
+    // the workgroup's sums: teams of a wavefront by lane exchange, then one after the other through LDS
+    const bool paired = !kOne && lanes < 64;
+    const int turns = paired ? blockDim.x >> 6 : teams, mine = paired ? threadIdx.x >> 6 : team;
+    const bool holds = !paired || (threadIdx.x & 63) < 16;
+#pragma unroll
+    for (int b = 0; b < (kLayer ? 2 : 1); ++b) {
+        if (paired) {
+#pragma unroll
+            for (int q = 0; q < kVecs; ++q)
+#pragma unroll
+                for (int i = 0; i < kVec; ++i) {
+                    float& s = b ? db[q][i] : dw[q][i];
+                    s += __shfl_xor(s, 16, 64);
+                    s += __shfl_xor(s, 32, 64);
+                }
+        }
+        float* out = part + ((int64_t)blockIdx.x * 2 + b) * hidden;
+        for (int t = 0; t < turns; ++t) {
+            if (t == mine && holds) {
+#pragma unroll
+                for (int q = 0; q < kVecs; ++q) {
+                    float s[kVec];
+#pragma unroll
+                    for (int i = 0; i < kVec; ++i) {
+                        float* at = columns + (q * kVec + i) * lanes + tl;      // a lane's place is the same for every team
+                        s[i] = (b ? db[q][i] : dw[q][i]) + (!kOne && t > 0 ? *at : 0.f);
+                        if (t < turns - 1) *at = s[i];
+                    }
+                    if (t < turns - 1) continue;
+                    if (q < kVecs - 1 || col.skip == 0) {
+#pragma unroll
+                        for (int p = 0; p < kVec; p += 4)
+                            mrl::Vec<MRL_F32>::store(out + col.at(q) + p, mrl::make_u32x4(__float_as_uint(s[p]),
+                                                     __float_as_uint(s[p + 1]), __float_as_uint(s[p + 2]), __float_as_uint(s[p + 3])));
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < kVec; ++i)
+                            if (i >= col.skip) out[col.last + i] = s[i];
+                    }
+                }
+            }
+            if (!kOne) __syncthreads();
+        }
+    }
+}
+
+// Sums of the groups' sums: 32 columns a workgroup, 32 lanes a column that each take every 32nd group.
+template <int WDT>
+__global__ __launch_bounds__(1024) void norm_part_sum_kernel(const float* __restrict__ part, int n_parts, int64_t hidden,
+                                                             typename Elem<WDT>::T* __restrict__ dweight,
+                                                             typename Elem<WDT>::T* __restrict__ dbias) {
+    __shared__ float lds[32][33];
+    typename Elem<WDT>::T* out = blockIdx.y == 0 ? dweight : dbias;
+    if (!out) return;
+    const int c = threadIdx.x & 31, slice = threadIdx.x >> 5;
+    const int64_t j = (int64_t)blockIdx.x * 32 + c;
+    const float* p = part + blockIdx.y * hidden + (j < hidden ? j : hidden - 1);
+    float s = 0.f;
+    for (int g = slice; g < n_parts; g += 16 * 32) {    // sixteen on their way at a time
+        float v[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int k = g + i * 32;
+            v[i] = p[(int64_t)(k < n_parts ? k : slice) * 2 * hidden];
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s += g + i * 32 < n_parts ? v[i] : 0.f;
+    }
+    lds[slice][c] = s;
+    __syncthreads();
+    // a wavefront joins the slices of two columns
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    s = mrl::lanes_sum<4>(lds[lane & 31][2 * wave + (lane >> 5)]);
+    s += __shfl_xor(s, 16, 64);
+    const int64_t column = (int64_t)blockIdx.x * 32 + 2 * wave + (lane >> 5);
+    if ((lane & 31) == 0 && column < hidden) Elem<WDT>::store(out + column, s);
+}
+
 int64_t slab_rows_of(int64_t n_rows) {
     const int64_t rows = (n_rows + kColumnSlabs - 1) / kColumnSlabs;
     return rows < 16 ? 16 : rows;
+}
+
+// The backward's teams are larger, with one or two vectors a lane (four in rows of more than 2 048 vectors): it holds twice
+// the entries, and the sums of the columns besides.
+Team bwd_team_of(int dtype, int64_t hidden) {
+    const int64_t nv = vectors_of(dtype, hidden);
+    if (nv == 0) return {0, 0};
+    if (nv <= 32) return team_that_fits(nv, 16, (int)((nv + 15) / 16));
+    for (int vecs = 1; vecs <= 4; vecs *= 2) {
+        const int64_t waves = (nv + 64 * vecs - 1) / (64 * vecs);
+        if (waves <= 16) return team_that_fits(nv, waves * 64, vecs);
+    }
+    return {0, 0};
+}
+
+// Threads and number of the backward's workgroups.
+int bwd_block(const Team& team) { return team.lanes > kBwdBlock ? team.lanes : kBwdBlock / team.lanes * team.lanes; }
+
+int bwd_groups(const Team& team, int64_t n_rows) {
+    const int teams = bwd_block(team) / team.lanes;
+    const int64_t turns = (n_rows + teams - 1) / teams, fit = team.lanes > kBwdBlock ? kBwdGroups / 2 : kBwdGroups;
+    const int64_t each = (turns + fit - 1) / fit;       // and no more workgroups than take as long
+    return (int)((turns + each - 1) / each);
+}
+
+template <int N>
+struct Int {
+    static constexpr int value = N;
+};
+
+template <typename F>
+void with_vecs(int vecs, F launch) {
+    switch (vecs) {
+        case 1: return launch(Int<1>());
+        case 2: return launch(Int<2>());
+        case 3: return launch(Int<3>());
+        default: return launch(Int<4>());
+    }
 }
 
 struct FwdArgs {
@@ -145,6 +490,19 @@ template <int DT, int WDT, bool kLayer>
 void launch_fwd(const FwdArgs& a) {
     using T = typename Elem<DT>::T;
     using W = typename Elem<WDT>::T;
+    const Team team = team_of(DT, a.hidden);
+    if (team.lanes > 0) {
+        const int block = team.lanes > 256 ? team.lanes : 256, teams = block / team.lanes;
+        const dim3 grid((unsigned)((a.n_rows + teams - 1) / teams));
+        const auto launch = [&](auto vecs, auto stream) {
+            hipLaunchKernelGGL((norm_fwd_rows_kernel<DT, WDT, kLayer, decltype(vecs)::value, decltype(stream)::value != 0>), grid,
+                               dim3(block), 0, a.stream, (const T*)a.x, a.x_stride, a.n_rows, (int)a.hidden, team.lanes,
+                               (const W*)a.weight, (const W*)a.bias, a.eps, (T*)a.y, a.mean, a.rstd);
+        };
+        if (team.lanes >= 64 && a.hidden * (int64_t)sizeof(T) % 128 == 0) with_vecs(team.vecs, [&](auto v) { launch(v, Int<1>()); });
+        else with_vecs(team.vecs, [&](auto v) { launch(v, Int<0>()); });
+        return;
+    }
     hipLaunchKernelGGL((norm_fwd_kernel<DT, WDT, kLayer>), dim3((unsigned)a.n_rows), dim3(kBlock), 0, a.stream, (const T*)a.x,
                        a.x_stride, a.hidden, (const W*)a.weight, (const W*)a.bias, a.eps, (T*)a.y, a.mean, a.rstd);
 }
@@ -162,6 +520,32 @@ template <int DT, int WDT, bool kLayer>
 void launch_bwd(const BwdArgs& a) {
     using T = typename Elem<DT>::T;
     using W = typename Elem<WDT>::T;
+    const Team team = bwd_team_of(DT, a.hidden);
+    if (team.lanes > 0 && a.n_rows > 0 && a.dx) {
+        const bool sums = a.dweight || a.dbias;
+        const int groups = bwd_groups(team, a.n_rows);
+        const auto launch = [&](auto vecs, auto most, auto stream) {
+            const int block = bwd_block(team);
+            hipLaunchKernelGGL((norm_bwd_rows_kernel<DT, WDT, kLayer, decltype(vecs)::value, decltype(most)::value,
+                                                     decltype(stream)::value != 0>),
+                               dim3((unsigned)groups), dim3(block), sums && block > team.lanes ? (size_t)team.lanes * team.vecs * Elem<DT>::kVec * 4 : 0, a.stream,
+                               (const T*)a.dy, a.dy_stride, (const T*)a.x, a.x_stride, a.n_rows, (int)a.hidden, team.lanes,
+                               (const W*)a.weight, a.mean, a.rstd, (T*)a.dx, sums ? a.part : nullptr);
+        };
+        const auto launch_block = [&](auto stream) {
+            if (team.vecs == 4) launch(Int<4>(), Int<1024>(), stream);
+            else if (team.vecs == 2 && team.lanes > kBwdBlock) launch(Int<2>(), Int<1024>(), stream);
+            else if (team.vecs == 2) launch(Int<2>(), Int<kBwdBlock>(), stream);
+            else if (team.lanes > kBwdBlock) launch(Int<1>(), Int<1024>(), stream);
+            else launch(Int<1>(), Int<kBwdBlock>(), stream);
+        };
+        if (team.lanes >= 64 && a.hidden * (int64_t)sizeof(T) % 128 == 0) launch_block(Int<1>());
+        else launch_block(Int<0>());
+        if (sums)
+            hipLaunchKernelGGL((norm_part_sum_kernel<WDT>), dim3((unsigned)((a.hidden + 31) / 32), a.dbias ? 2 : 1), dim3(1024), 0,
+                               a.stream, a.part, groups, a.hidden, (W*)a.dweight, (W*)a.dbias);
+        return;
+    }
     if (a.dx && a.n_rows > 0)
         hipLaunchKernelGGL((norm_dx_kernel<DT, WDT, kLayer>), dim3((unsigned)a.n_rows), dim3(kBlock), 0, a.stream, (const T*)a.dy,
                            a.dy_stride, (const T*)a.x, a.x_stride, a.hidden, (const W*)a.weight, a.mean, a.rstd, (T*)a.dx);
@@ -234,8 +618,8 @@ extern "C" int mrl_norm_fwd(const void* x, int dtype, int64_t n_rows, int64_t hi
 
 extern "C" int64_t mrl_norm_bwd_workspace_bytes(int64_t n_rows, int64_t hidden) {
     if (n_rows <= 0 || hidden <= 0 || n_rows > 0x7fffffffLL || hidden > MRL_NORM_MAX_HIDDEN) return 0;
-    const int64_t slab = slab_rows_of(n_rows);
-    return (n_rows + slab - 1) / slab * 2 * hidden * 4;
+    const int64_t slab = slab_rows_of(n_rows), slabs = (n_rows + slab - 1) / slab;
+    return (slabs > kBwdGroups ? slabs : kBwdGroups) * 2 * hidden * 4;
 }
 
 extern "C" int mrl_norm_bwd(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, int dtype, int64_t n_rows,
