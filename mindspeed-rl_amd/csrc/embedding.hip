@@ -7,7 +7,9 @@
 // sorted list, in its order, in fp32, by workgroups of equal shares of it, and what crosses a share is joined afterwards:
 // the same tokens give the same bits, a row that many tokens name is summed by many workgroups, and every row is rounded
 // once.  Bound by memory, and by the sort's few launches where tokens are few.
+#include "lane_ops.h"
 #include "mrl_internal.h"
+#include "vector_access.h"
 #include "vocab_common.h"
 
 namespace {
@@ -20,8 +22,9 @@ constexpr int kSortWaves = kSortBlock / 64;
 constexpr int kDigits = 512;
 constexpr int kDigitBits = 9;
 constexpr int kSortGroups = 128;            // most workgroups of a sort pass
-constexpr int kShares = 2048;               // most shares of the sorted list
-constexpr int kMinShare = 32;
+constexpr int kShares = 1024;               // most shares of the sorted list
+constexpr int kMinShare = 8;
+constexpr int kFewTokens = 2048;            // that one workgroup sorts in its LDS
 
 // the row that a token names, `vocab` where it is outside
 __device__ __forceinline__ int32_t row_of(const void* ids, int dtype, int64_t t, int64_t start, int64_t vocab) {
@@ -30,14 +33,49 @@ __device__ __forceinline__ int32_t row_of(const void* ids, int dtype, int64_t t,
     return id >= start && id - start < vocab ? (int32_t)(id - start) : (int32_t)vocab;
 }
 
+// Rows shorter than a vector: a thread an entry.
 template <int DT>
-__global__ __launch_bounds__(kBlock) void lookup_kernel(const void* __restrict__ ids, int ids_dtype, int64_t start,
+__global__ __launch_bounds__(kBlock) void lookup_narrow_kernel(const void* __restrict__ ids, int ids_dtype, int64_t n_tokens,
+                                                               int64_t start, const typename Elem<DT>::T* __restrict__ table,
+                                                               int64_t vocab, int hidden, float scale,
+                                                               typename Elem<DT>::T* __restrict__ out) {
+    const int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+    if (i >= n_tokens * hidden) return;
+    const int64_t t = i / hidden, row = row_of(ids, ids_dtype, t, start, vocab);
+    Elem<DT>::store(out + i, row < vocab ? Elem<DT>::load(table + row * hidden + (i - t * hidden)) * scale : 0.f);
+}
+
+// A wavefront a token and kVecs vectors a lane, all on their way together; a row that is not whole vectors ends with one that
+// overlaps the one in front of it, and lanes behind the row write that again: the same bits.  Table rows are read through
+// the caches (tokens repeat), what is written goes past them.
+template <int DT, int kVecs>
+__global__ __launch_bounds__(kBlock) void lookup_kernel(const void* __restrict__ ids, int ids_dtype, int64_t n_tokens, int64_t start,
                                                         const typename Elem<DT>::T* __restrict__ table, int64_t vocab,
-                                                        int64_t hidden, float scale, typename Elem<DT>::T* __restrict__ out) {
-    const int64_t t = blockIdx.x;
-    const int32_t row = row_of(ids, ids_dtype, t, start, vocab);
-    for (int64_t j = threadIdx.x; j < hidden; j += kBlock)
-        Elem<DT>::store(out + t * hidden + j, row < vocab ? Elem<DT>::load(table + row * hidden + j) * scale : 0.f);
+                                                        int hidden, float scale, typename Elem<DT>::T* __restrict__ out) {
+    constexpr int kVec = Elem<DT>::kVec;
+    const int lane = threadIdx.x & 63;
+    const int64_t t = (int64_t)blockIdx.x * (kBlock / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (t >= n_tokens) return;
+    const int64_t row = row_of(ids, ids_dtype, t, start, vocab);
+    const bool inside = row < vocab;
+    const typename Elem<DT>::T* from = table + (inside ? row : 0) * hidden;
+    typename Elem<DT>::T* to = out + t * hidden;
+    const int first = ((int)blockIdx.y * kVecs * 64 + lane) * kVec, most = hidden - kVec;
+    u32x4 v[kVecs];
+#pragma unroll
+    for (int q = 0; q < kVecs; ++q) {
+        const int j = first + q * 64 * kVec;
+        v[q] = mrl::Vec<DT>::load(from + (j < most ? j : most));
+    }
+#pragma unroll
+    for (int q = 0; q < kVecs; ++q) {
+        const int j = first + q * 64 * kVec;
+        float z[kVec];
+        Elem<DT>::unpack(v[q], z);
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) z[i] = inside ? z[i] * scale : 0.f;
+        mrl::Vec<DT>::store_nt(to + (j < most ? j : most), Elem<DT>::pack(z));
+    }
 }
 
 // ------------------------------------------------------------------------------------ sort
@@ -58,11 +96,34 @@ __host__ SortPlan sort_plan(int64_t n_tokens, int64_t vocab) {
     return p;
 }
 
+// Zeros for the gradient's rows that no token names: workgroups behind the sort's, which is bound by latency and leaves the
+// memory to them.  Rows that are named are written later.
+struct Fill {
+    char* at;                               // 2-byte aligned at least
+    int64_t bytes;                          // this launch's part
+};
+
+constexpr int kFillVecs = 1;                // vectors a thread
+constexpr int64_t kFillBytes = (int64_t)kSortBlock * kFillVecs * 16;
+
+__device__ __forceinline__ void fill_part(const Fill& f, int64_t block) {
+    const u32x4 zero = mrl::make_u32x4(0u, 0u, 0u, 0u);
+    const int64_t lo = block * kFillBytes;
+#pragma unroll
+    for (int q = 0; q < kFillVecs; ++q) {
+        const int64_t at = lo + ((int64_t)q * kSortBlock + threadIdx.x) * 16;
+        if (at + 16 <= f.bytes) *(mrl::u32x4_anywhere*)(f.at + at) = zero;
+        else
+            for (int64_t i = at; i < f.bytes; i += 2) *(uint16_t*)(f.at + i) = 0;
+    }
+}
+
 // counts[group][digit] of the first digit, and zeros in those of the later passes.
 __global__ __launch_bounds__(kSortBlock) void sort_count_kernel(const void* __restrict__ ids, int ids_dtype, int64_t n_tokens,
                                                                 int64_t start, int64_t vocab, SortPlan p,
-                                                                int32_t* __restrict__ counts) {
+                                                                int32_t* __restrict__ counts, Fill fill) {
     __shared__ int32_t hist[kDigits];
+    if ((int)blockIdx.x >= p.groups) return fill_part(fill, blockIdx.x - p.groups);
     hist[threadIdx.x] = 0;
     __syncthreads();
     const int64_t lo = blockIdx.x * p.per_group, hi = lo + p.per_group < n_tokens ? lo + p.per_group : n_tokens;
@@ -75,8 +136,75 @@ __global__ __launch_bounds__(kSortBlock) void sort_count_kernel(const void* __re
     for (int q = 1; q < p.passes; ++q) counts[q * matrix + at] = 0;
 }
 
-// One stable pass: a workgroup's tokens, in order, behind those of the workgroups in front of it.  Each wavefront takes a
-// contiguous part of them; lanes of equal digit find each other by ballots.  Counts the next digit where the tokens land.
+// The steps of a stable pass by a workgroup over its tokens [lo, hi), of which each wavefront takes `per_wave` in a row.
+// `place[wave][digit]` counts at first and then says where the next token of the digit goes.
+struct Placing {
+    int32_t (*place)[kDigits];
+    int64_t w_lo, w_hi;
+    int bits, shift;
+
+    __device__ __forceinline__ void clear() const {
+#pragma unroll
+        for (int w = 0; w < kSortWaves; ++w) place[w][threadIdx.x] = 0;
+    }
+    template <typename Key>
+    __device__ __forceinline__ void count(Key key_at) const {
+        for (int64_t t = w_lo + (threadIdx.x & 63); t < w_hi; t += 64)
+            atomicAdd(&place[threadIdx.x >> 6][(key_at(t) >> shift) & ((1 << bits) - 1)], 1);
+    }
+    // thread d: where the workgroup's first token of digit d goes
+    __device__ __forceinline__ void start(int32_t base) const {
+#pragma unroll
+        for (int w = 0; w < kSortWaves; ++w) {
+            const int32_t c = place[w][threadIdx.x];
+            place[w][threadIdx.x] = base;
+            base += c;
+        }
+    }
+    // put(t, key, at) for every token, in order within the wavefront: lanes of equal digit find each other by ballots.
+    template <typename Key, typename Put>
+    __device__ __forceinline__ void run(Key key_at, Put put) const {
+        const int lane = threadIdx.x & 63;
+        volatile int32_t* mine = place[threadIdx.x >> 6];
+        for (int64_t t0 = w_lo; t0 < w_hi; t0 += 64) {
+            const int64_t t = t0 + lane;
+            const bool active = t < w_hi;
+            const int32_t key = active ? key_at(t) : 0;
+            const int32_t digit = (key >> shift) & ((1 << bits) - 1);
+            uint64_t same = __ballot(active);
+            for (int b = 0; b < bits; ++b) {
+                const uint64_t set = __ballot((digit >> b) & 1);
+                same &= ((digit >> b) & 1) ? set : ~set;
+            }
+            const int32_t at = mine[digit] + __popcll(same & ((1ull << lane) - 1));
+            __builtin_amdgcn_wave_barrier();
+            if (active) {
+                if ((same >> lane) == 1ull) mine[digit] = at + 1;   // the last lane of this digit
+                put(t, key, at);
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+    }
+};
+
+// Sum of the values of the threads in front of this one.  `lds`: an entry per wavefront; a barrier inside.
+__device__ __forceinline__ int32_t sum_in_front(int32_t x, int32_t* lds) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int32_t incl = x;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const int32_t o = __shfl_up(incl, off, 64);
+        if (lane >= off) incl += o;
+    }
+    if (lane == 63) lds[wave] = incl;
+    __syncthreads();
+    int32_t before = incl - x;
+    for (int w = 0; w < wave; ++w) before += lds[w];
+    return before;
+}
+
+// One stable pass: a workgroup's tokens, in order, behind those of the workgroups in front of it.  Counts the next digit
+// where the tokens land.
 template <bool kFirst>
 __global__ __launch_bounds__(kSortBlock) void sort_pass_kernel(const void* __restrict__ ids, int ids_dtype, int64_t n_tokens,
                                                                int64_t start, int64_t vocab, SortPlan p, int pass,
@@ -84,127 +212,288 @@ __global__ __launch_bounds__(kSortBlock) void sort_pass_kernel(const void* __res
                                                                const int32_t* __restrict__ tokens_in,
                                                                int32_t* __restrict__ keys_out, int32_t* __restrict__ tokens_out,
                                                                const int32_t* __restrict__ counts,
-                                                               int32_t* __restrict__ next_counts) {
+                                                               int32_t* __restrict__ next_counts, Fill fill) {
+    if ((int)blockIdx.x >= p.groups) return fill_part(fill, blockIdx.x - p.groups);
     __shared__ int32_t place[kSortWaves][kDigits];
     __shared__ int32_t wave_sum[kSortWaves];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int32_t mask = (1 << p.bits) - 1;
-    const int shift = pass * p.bits;
-#pragma unroll
-    for (int w = 0; w < kSortWaves; ++w) place[w][tid] = 0;
-    // this digit's tokens altogether, and in the workgroups in front of this one
-    int32_t total = 0, before = 0;
-    for (int g = 0; g < p.groups; ++g) {
-        const int32_t c = counts[g * kDigits + tid];
-        total += c;
-        if (g < (int)blockIdx.x) before += c;
-    }
-    int32_t incl = total;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const int32_t o = __shfl_up(incl, off, 64);
-        if (lane >= off) incl += o;
-    }
-    if (lane == 63) wave_sum[wave] = incl;
-    __syncthreads();
-    int32_t base = incl - total + before;
-    for (int w = 0; w < wave; ++w) base += wave_sum[w];
-
+    const int tid = threadIdx.x;
     const int64_t lo = blockIdx.x * p.per_group, hi = lo + p.per_group < n_tokens ? lo + p.per_group : n_tokens;
     const int64_t per_wave = p.per_group / kSortWaves;             // whole wavefronts: per_group is whole workgroups
-    const int64_t w_lo = lo + wave * per_wave, w_hi = w_lo + per_wave < hi ? w_lo + per_wave : hi;
+    const int64_t w_lo = lo + (tid >> 6) * per_wave;
+    const Placing step = {place, w_lo, w_lo + per_wave < hi ? w_lo + per_wave : hi, p.bits, pass * p.bits};
     const auto key_at = [&](int64_t t) { return kFirst ? row_of(ids, ids_dtype, t, start, vocab) : keys_in[t]; };
-    for (int64_t t = w_lo + lane; t < w_hi; t += 64) atomicAdd(&place[wave][(key_at(t) >> shift) & mask], 1);
-    __syncthreads();
+    step.clear();
+    // this digit's tokens altogether, and in the workgroups in front of this one
+    int32_t total = 0, before = 0;
+    for (int g0 = 0; g0 < p.groups; g0 += 16) {         // sixteen on their way at a time
+        int32_t c[16];
 #pragma unroll
-    for (int w = 0; w < kSortWaves; ++w) {
-        const int32_t c = place[w][tid];
-        place[w][tid] = base;
-        base += c;
+        for (int i = 0; i < 16; ++i) c[i] = counts[(g0 + i < p.groups ? g0 + i : 0) * kDigits + tid];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            total += g0 + i < p.groups ? c[i] : 0;
+            before += g0 + i < (int)blockIdx.x ? c[i] : 0;
+        }
     }
+    const int32_t base = sum_in_front(total, wave_sum) + before;   // its barrier: `place` is cleared
+    step.count(key_at);
     __syncthreads();
-    volatile int32_t* mine = place[wave];
-    for (int64_t t0 = w_lo; t0 < w_hi; t0 += 64) {
-        const int64_t t = t0 + lane;
-        const bool active = t < w_hi;
-        const int32_t key = active ? key_at(t) : 0;
-        const int32_t digit = (key >> shift) & mask;
-        uint64_t same = __ballot(active);
-        for (int b = 0; b < p.bits; ++b) {
-            const uint64_t set = __ballot((digit >> b) & 1);
-            same &= ((digit >> b) & 1) ? set : ~set;
-        }
-        const int rank = __popcll(same & ((1ull << lane) - 1));
-        const int32_t at = mine[digit] + rank;
-        __builtin_amdgcn_wave_barrier();
-        if (active) {
-            if ((same >> lane) == 1ull) mine[digit] = at + 1;      // the last lane of this digit
-            keys_out[at] = key;
-            tokens_out[at] = kFirst ? (int32_t)t : tokens_in[t];
-            if (next_counts) atomicAdd(&next_counts[(int64_t)(at / p.per_group) * kDigits + ((key >> (shift + p.bits)) & mask)], 1);
-        }
-        __builtin_amdgcn_wave_barrier();
+    step.start(base);
+    __syncthreads();
+    const uint32_t per_group = (uint32_t)p.per_group;
+    step.run(key_at, [&](int64_t t, int32_t key, int32_t at) {
+        keys_out[at] = key;
+        tokens_out[at] = kFirst ? (int32_t)t : tokens_in[t];
+        if (next_counts)
+            atomicAdd(&next_counts[(uint32_t)at / per_group * kDigits + ((key >> (step.shift + p.bits)) & ((1 << p.bits) - 1))], 1);
+    });
+}
+
+// All passes in one launch, for as many tokens as a workgroup holds.
+__global__ __launch_bounds__(kSortBlock) void sort_few_kernel(const void* __restrict__ ids, int ids_dtype, int n_tokens, int64_t start,
+                                                              int64_t vocab, SortPlan p, int32_t* __restrict__ keys_out,
+                                                              int32_t* __restrict__ tokens_out, Fill fill) {
+    if (blockIdx.x >= 1) return fill_part(fill, blockIdx.x - 1);
+    __shared__ int32_t place[kSortWaves][kDigits];
+    __shared__ int32_t wave_sum[kSortWaves];
+    __shared__ int32_t keys[2][kFewTokens];
+    __shared__ uint16_t tokens[2][kFewTokens];
+    const int tid = threadIdx.x;
+    for (int t = tid; t < n_tokens; t += kSortBlock) {
+        keys[0][t] = row_of(ids, ids_dtype, t, start, vocab);
+        tokens[0][t] = (uint16_t)t;
+    }
+    const int per_wave = ((n_tokens + kSortBlock - 1) / kSortBlock) * 64, w_lo = (tid >> 6) * per_wave;
+    for (int pass = 0; pass < p.passes; ++pass) {
+        const int from = pass & 1, to = from ^ 1;
+        const bool last = pass == p.passes - 1;
+        const Placing step = {place, w_lo, w_lo + per_wave < n_tokens ? w_lo + per_wave : n_tokens, p.bits, pass * p.bits};
+        const auto key_at = [&](int64_t t) { return keys[from][t]; };
+        step.clear();
+        __syncthreads();                                // the tokens of the step in front are in their places, too
+        step.count(key_at);
+        __syncthreads();
+        int32_t total = 0;
+#pragma unroll
+        for (int w = 0; w < kSortWaves; ++w) total += place[w][tid];
+        step.start(sum_in_front(total, wave_sum));
+        __syncthreads();
+        step.run(key_at, [&](int64_t t, int32_t key, int32_t at) {
+            if (last) {
+                keys_out[at] = key;
+                tokens_out[at] = tokens[from][t];
+            } else {
+                keys[to][at] = key;
+                tokens[to][at] = tokens[from][t];
+            }
+        });
+        __syncthreads();
     }
 }
 
 // ------------------------------------------------------------------------------------ sums
+// The sorted list in equal shares, a workgroup each; part[share][2][hidden] holds the sum of a run that the share in front
+// began, and that of one which goes on behind this share.
 struct Sums {
-    const int32_t *keys, *tokens;           // sorted
-    float* part;                            // [share][2][hidden]: of a run from the share in front, of one that goes on behind
+    float* part;
     int64_t n_tokens, hidden, share;
     int32_t vocab;
     float scale;
 };
 
-template <int GT, bool kAdd>
-__device__ __forceinline__ void put(typename Elem<GT>::T* at, float sum, float scale) {
-    Elem<GT>::store(at, kAdd ? Elem<GT>::load(at) + sum * scale : sum * scale);
-}
-
-// A share of the sorted list, a thread for a column.
+// Rows shorter than a vector: a thread a column.
 template <int DT, int GT, bool kAdd>
-__global__ __launch_bounds__(kBlock) void sum_kernel(Sums s, const typename Elem<DT>::T* __restrict__ dy,
-                                                     typename Elem<GT>::T* __restrict__ dtable) {
-    const int64_t j = (int64_t)blockIdx.y * kBlock + threadIdx.x;
+__global__ __launch_bounds__(64) void sum_narrow_kernel(Sums s, const int32_t* __restrict__ keys, const int32_t* __restrict__ tokens,
+                                                        const typename Elem<DT>::T* __restrict__ dy,
+                                                        typename Elem<GT>::T* __restrict__ dtable) {
+    const int64_t j = threadIdx.x;
     if (j >= s.hidden) return;
     const int64_t begin = blockIdx.x * s.share, end = begin + s.share < s.n_tokens ? begin + s.share : s.n_tokens;
-    const int32_t prev = begin > 0 ? s.keys[begin - 1] : -1, next = end < s.n_tokens ? s.keys[end] : -1;
+    const int32_t prev = begin > 0 ? keys[begin - 1] : -1, next = end < s.n_tokens ? keys[end] : -1;
     for (int64_t p = begin; p < end;) {
         const int64_t first = p;
-        const int32_t key = s.keys[p];
+        const int32_t key = keys[p];
         if (key >= s.vocab) break;                                  // so are all behind it
         float acc = 0.f;
-        do acc += Elem<DT>::load(dy + (int64_t)s.tokens[p] * s.hidden + j);
-        while (++p < end && s.keys[p] == key);
+        do acc += Elem<DT>::load(dy + (int64_t)tokens[p] * s.hidden + j);
+        while (++p < end && keys[p] == key);
+        typename Elem<GT>::T* at = dtable + key * s.hidden + j;
         if (first == begin && prev == key) s.part[(blockIdx.x * 2ll) * s.hidden + j] = acc;
         else if (p == end && next == key) s.part[(blockIdx.x * 2ll + 1) * s.hidden + j] = acc;
-        else put<GT, kAdd>(dtable + key * s.hidden + j, acc, s.scale);
+        else Elem<GT>::store(at, kAdd ? Elem<GT>::load(at) + acc * s.scale : acc * s.scale);
     }
 }
 
-// The runs that cross shares: the share that one begins in adds up its parts.
+// kVec columns of a row: written, or added to what is there.  Entries in front of `skip` are another lane's.
+template <int GT, int kVec, bool kAdd>
+__device__ __forceinline__ void put_columns(typename Elem<GT>::T* at, const float (&acc)[kVec], float scale, int skip) {
+    constexpr int kGVec = Elem<GT>::kVec;
+    if (skip != 0) {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i)
+            if (i >= skip) Elem<GT>::store(at + i, kAdd ? Elem<GT>::load(at + i) + acc[i] * scale : acc[i] * scale);
+        return;
+    }
+#pragma unroll
+    for (int p = 0; p < kVec / kGVec; ++p) {
+        float z[kGVec] = {};
+        if (kAdd) Elem<GT>::unpack(mrl::Vec<GT>::load(at + p * kGVec), z);
+#pragma unroll
+        for (int i = 0; i < kGVec; ++i) z[i] = kAdd ? z[i] + acc[p * kGVec + i] * scale : acc[p * kGVec + i] * scale;
+        mrl::Vec<GT>::store(at + p * kGVec, Elem<GT>::pack(z));
+    }
+}
+
+constexpr int kSumBlock = 512;              // most lanes of a share
+constexpr int kSumRows = 4;                 // rows of a batch, of which one is summed and one on its way
+
+// A lane a vector of columns; the tokens of the share one after the other.
+template <int DT, int GT, bool kAdd>
+__global__ __launch_bounds__(kSumBlock) void sum_kernel(Sums s, const int32_t* __restrict__ keys, const int32_t* __restrict__ tokens,
+                                                        const typename Elem<DT>::T* __restrict__ dy,
+                                                        typename Elem<GT>::T* __restrict__ dtable) {
+    constexpr int kVec = Elem<DT>::kVec;
+    const int64_t begin = blockIdx.x * s.share, end = begin + s.share < s.n_tokens ? begin + s.share : s.n_tokens;
+    int32_t key = keys[begin];
+    if (key >= s.vocab) return;                                     // so are all behind it
+    const int64_t want = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * kVec;
+    const int64_t col = want < s.hidden - kVec ? want : s.hidden - kVec;
+    const int skip = want >= s.hidden ? kVec : (int)(want - col);
+    const int32_t next = end < s.n_tokens ? keys[end] : -1;
+    bool from_front = begin > 0 && keys[begin - 1] == key;
+    float acc[kVec] = {};
+    const auto finish = [&](bool goes_on) {
+        if (from_front || goes_on) {
+            float* to = s.part + (blockIdx.x * 2ll + (from_front ? 0 : 1)) * s.hidden + col;
+#pragma unroll
+            for (int p = 0; p < kVec; p += 4)                       // overlapping entries are the same bits
+                mrl::Vec<MRL_F32>::store(to + p, mrl::make_u32x4(__float_as_uint(acc[p]), __float_as_uint(acc[p + 1]),
+                                                                 __float_as_uint(acc[p + 2]), __float_as_uint(acc[p + 3])));
+        } else {
+            put_columns<GT, kVec, kAdd>(dtable + key * s.hidden + col, acc, s.scale, skip);
+        }
+    };
+    int32_t kn[kSumRows];
+    u32x4 vn[kSumRows];
+    const auto request = [&](int64_t p) {
+#pragma unroll
+        for (int i = 0; i < kSumRows; ++i) {
+            const int64_t at = p + i < end ? p + i : end - 1;
+            kn[i] = keys[at];
+            vn[i] = mrl::Vec<DT>::load_nt(dy + (int64_t)tokens[at] * s.hidden + col);
+        }
+    };
+    request(begin);
+    for (int64_t p = begin; p < end; p += kSumRows) {
+        int32_t k[kSumRows];
+        u32x4 v[kSumRows];
+#pragma unroll
+        for (int i = 0; i < kSumRows; ++i) {
+            k[i] = kn[i];
+            v[i] = vn[i];
+        }
+        request(p + kSumRows);
+#pragma unroll
+        for (int i = 0; i < kSumRows; ++i) {
+            if (p + i >= end) break;
+            if (k[i] != key) {
+                finish(false);
+                key = k[i];
+                if (key >= s.vocab) return;
+                from_front = false;
+#pragma unroll
+                for (int c = 0; c < kVec; ++c) acc[c] = 0.f;
+            }
+            float z[kVec];
+            Elem<DT>::unpack(v[i], z);
+#pragma unroll
+            for (int c = 0; c < kVec; ++c) acc[c] += z[c];
+        }
+    }
+    finish(next == key);
+}
+
+constexpr int kJoinWaves = 8, kJoinColumns = 64, kJoinGroups = 64, kJoinShort = 16;
+constexpr int kMaxShares = kJoinGroups * 64;
+
+// The runs that cross shares.  A workgroup takes a tile of columns and every kJoinGroups-th share, a lane for each at first:
+// does such a run begin there, and in how many shares does it go on.  Short runs are joined by a wavefront each, long ones by
+// all of them, each taking every kJoinWaves-th part.
 template <int GT, bool kAdd>
-__global__ __launch_bounds__(kBlock) void join_kernel(Sums s, typename Elem<GT>::T* __restrict__ dtable) {
-    const int64_t j = (int64_t)blockIdx.y * kBlock + threadIdx.x;
-    const int64_t begin = blockIdx.x * s.share, end = begin + s.share;
-    if (end >= s.n_tokens) return;
-    const int32_t key = s.keys[end - 1];
-    if (key >= s.vocab || s.keys[end] != key) return;
-    if (begin > 0 && s.keys[begin - 1] == key) return;              // begun further in front
-    int64_t lo = end, hi = s.n_tokens;                              // the run's last token is in [lo, hi)
-    while (hi - lo > 1) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (s.keys[mid] == key) lo = mid; else hi = mid;
+__global__ __launch_bounds__(kJoinWaves* kJoinColumns) void join_kernel(Sums s, const int32_t* __restrict__ keys,
+                                                                        typename Elem<GT>::T* __restrict__ dtable) {
+    __shared__ float lds[kJoinWaves][kJoinColumns];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t j = (int64_t)blockIdx.x * kJoinColumns + lane;
+    const int64_t jc = j < s.hidden ? j : s.hidden - 1;
+    // whether the run of `key` goes on in share g
+    const auto goes_on = [&](int64_t g, int32_t key) {
+        const int64_t first = g * s.share;
+        return first < s.n_tokens && keys[first < s.n_tokens ? first : 0] == key;
+    };
+    const int64_t mine = blockIdx.y + (int64_t)lane * kJoinGroups, mine_end = (mine + 1) * s.share;
+    int32_t my_key = s.vocab;
+    int more = 0;                                                   // shares behind this one, kJoinShort: as many or more
+    if (mine_end < s.n_tokens) {
+        my_key = keys[mine_end - 1];
+        if (my_key < s.vocab && (mine == 0 || keys[mine * s.share - 1] != my_key)) {
+            bool in = true;
+#pragma unroll
+            for (int i = 0; i < kJoinShort; ++i) {
+                in = in && goes_on(mine + 1 + i, my_key);
+                more += in ? 1 : 0;
+            }
+        }
     }
-    if (j >= s.hidden) return;
-    float acc = s.part[(blockIdx.x * 2ll + 1) * s.hidden + j];
-    for (int64_t g = blockIdx.x + 1ll; g <= lo / s.share; ++g) acc += s.part[g * 2 * s.hidden + j];
-    put<GT, kAdd>(dtable + key * s.hidden + j, acc, s.scale);
-}
-
-template <int GT>
-__global__ __launch_bounds__(kBlock) void zero_kernel(typename Elem<GT>::T* __restrict__ p, int64_t n) {
-    for (int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x; i < n; i += (int64_t)gridDim.x * kBlock) p[i] = 0;
+    const auto put = [&](int32_t key, float sum) {
+        if (j >= s.hidden) return;
+        typename Elem<GT>::T* at = dtable + key * s.hidden + j;
+        Elem<GT>::store(at, kAdd ? Elem<GT>::load(at) + sum * s.scale : sum * s.scale);
+    };
+    int nth = 0;
+    for (uint64_t todo = __ballot(more > 0 && more < kJoinShort); todo != 0; todo &= todo - 1, ++nth) {
+        if (nth % kJoinWaves != wave) continue;
+        const int from = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)todo) - 1);
+        const int64_t share = blockIdx.y + (int64_t)from * kJoinGroups;
+        const int n = __shfl(more, from, 64);
+        float v[kJoinShort];
+        v[0] = s.part[(share * 2 + 1) * s.hidden + jc];
+#pragma unroll
+        for (int i = 1; i < kJoinShort; ++i) v[i] = s.part[(share + (i <= n ? i : n)) * 2 * s.hidden + jc];
+        float sum = v[0];
+#pragma unroll
+        for (int i = 1; i < kJoinShort; ++i) sum += i <= n ? v[i] : 0.f;
+        put(__shfl(my_key, from, 64), sum);
+    }
+    for (uint64_t todo = __ballot(more == kJoinShort); todo != 0; todo &= todo - 1) {       // the same in every wavefront
+        const int from = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)todo) - 1);
+        const int64_t share = blockIdx.y + (int64_t)from * kJoinGroups;
+        const int32_t key = __shfl(my_key, from, 64);
+        int64_t last = share + kJoinShort;
+        for (uint64_t in = ~0ull; in == ~0ull;) {
+            in = __ballot(goes_on(last + 1 + lane, key));           // shares in a row from the front
+            last += in == ~0ull ? 64 : __ffsll((unsigned long long)~in) - 1;
+        }
+        float sum = 0.f;
+        for (int64_t g = share + wave; g <= last; g += kJoinWaves * 8) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int64_t part = g + i * kJoinWaves <= last ? g + i * kJoinWaves : last;
+                v[i] = s.part[(part * 2 + (part == share ? 1 : 0)) * s.hidden + jc];
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum += g + i * kJoinWaves <= last ? v[i] : 0.f;
+        }
+        lds[wave][lane] = sum;
+        __syncthreads();
+        if (wave == 0) {
+#pragma unroll
+            for (int w = 1; w < kJoinWaves; ++w) sum += lds[w][lane];
+            put(key, sum);
+        }
+        __syncthreads();
+    }
 }
 
 // ------------------------------------------------------------------------------------ host
@@ -214,6 +503,11 @@ int64_t share_of(int64_t n_tokens) {
     const int64_t s = (n_tokens + kShares - 1) / kShares;
     return s < kMinShare ? kMinShare : s;
 }
+
+template <int N>
+struct Int {
+    static constexpr int value = N;
+};
 
 struct Workspace {
     int64_t keys[2], tokens[2], counts, part, bytes;
@@ -254,20 +548,67 @@ int check_sizes(const char* fn, const void* ids, int ids_dtype, int64_t n_tokens
     return MRL_OK;
 }
 
+static_assert(kShares <= kMaxShares, "a lane of the join for every share");
+
 template <int DT, int GT, bool kAdd>
-void launch_sums(const Sums& s, const void* dy, void* dtable, hipStream_t stream) {
+void launch_sums(const Sums& s, const int32_t* keys, const int32_t* tokens, const void* dy, void* dtable, hipStream_t stream) {
+    using T = typename Elem<DT>::T;
     using G = typename Elem<GT>::T;
-    const unsigned columns = (unsigned)((s.hidden + kBlock - 1) / kBlock);
-    const unsigned shares = (unsigned)((s.n_tokens + s.share - 1) / s.share);
-    hipLaunchKernelGGL((sum_kernel<DT, GT, kAdd>), dim3(shares, columns), dim3(kBlock), 0, stream, s,
-                       (const typename Elem<DT>::T*)dy, (G*)dtable);
-    hipLaunchKernelGGL((join_kernel<GT, kAdd>), dim3(shares, columns), dim3(kBlock), 0, stream, s, (G*)dtable);
+    const int64_t shares = (s.n_tokens + s.share - 1) / s.share, nv = (s.hidden + Elem<DT>::kVec - 1) / Elem<DT>::kVec;
+    if (s.hidden < Elem<DT>::kVec) {
+        hipLaunchKernelGGL((sum_narrow_kernel<DT, GT, kAdd>), dim3((unsigned)shares), dim3(64), 0, stream, s, keys, tokens,
+                           (const T*)dy, (G*)dtable);
+    } else {
+        const int64_t block = nv < kSumBlock ? (nv + 63) / 64 * 64 : kSumBlock;
+        hipLaunchKernelGGL((sum_kernel<DT, GT, kAdd>), dim3((unsigned)shares, (unsigned)((nv + block - 1) / block)),
+                           dim3((unsigned)block), 0, stream, s, keys, tokens, (const T*)dy, (G*)dtable);
+    }
+    if (shares > 1)
+        hipLaunchKernelGGL((join_kernel<GT, kAdd>),
+                           dim3((unsigned)((s.hidden + kJoinColumns - 1) / kJoinColumns),
+                                (unsigned)(shares < kJoinGroups ? shares : kJoinGroups)),
+                           dim3(kJoinWaves * kJoinColumns), 0, stream, s, keys, (G*)dtable);
 }
 
 template <int DT, int GT>
-void launch_sums(bool add, const Sums& s, const void* dy, void* dtable, hipStream_t stream) {
-    if (add) launch_sums<DT, GT, true>(s, dy, dtable, stream);
-    else launch_sums<DT, GT, false>(s, dy, dtable, stream);
+void launch_sums(bool add, const Sums& s, const int32_t* keys, const int32_t* tokens, const void* dy, void* dtable,
+                 hipStream_t stream) {
+    if (add) launch_sums<DT, GT, true>(s, keys, tokens, dy, dtable, stream);
+    else launch_sums<DT, GT, false>(s, keys, tokens, dy, dtable, stream);
+}
+
+// The part of a fill that launch `k` of `n` takes, in whole workgroups.
+Fill fill_share(void* dtable, int64_t bytes, int k, int n) {
+    const int64_t blocks = (bytes + kFillBytes - 1) / kFillBytes;
+    const int64_t lo = blocks * k / n * kFillBytes, hi = k == n - 1 ? bytes : blocks * (k + 1) / n * kFillBytes;
+    return {(char*)dtable + lo, hi - lo};
+}
+
+unsigned fill_blocks(const Fill& f) { return (unsigned)((f.bytes + kFillBytes - 1) / kFillBytes); }
+
+template <int DT>
+void launch_lookup(const void* ids, int ids_dtype, int64_t n_tokens, int64_t start, const void* table, int64_t vocab,
+                   int64_t hidden, float scale, void* out, hipStream_t stream) {
+    using T = typename Elem<DT>::T;
+    if (hidden < Elem<DT>::kVec) {
+        hipLaunchKernelGGL((lookup_narrow_kernel<DT>), dim3((unsigned)((n_tokens * hidden + kBlock - 1) / kBlock)), dim3(kBlock), 0,
+                           stream, ids, ids_dtype, n_tokens, start, (const T*)table, vocab, (int)hidden, scale, (T*)out);
+        return;
+    }
+    const int64_t waves = (hidden + Elem<DT>::kVec * 64 - 1) / (Elem<DT>::kVec * 64);       // of a row, a vector a lane
+    const auto launch = [&](auto vecs) {
+        constexpr int kVecs = decltype(vecs)::value;
+        const dim3 grid((unsigned)((n_tokens + kBlock / 64 - 1) / (kBlock / 64)), (unsigned)((waves + kVecs - 1) / kVecs));
+        hipLaunchKernelGGL((lookup_kernel<DT, kVecs>), grid, dim3(kBlock), 0, stream, ids, ids_dtype, n_tokens, start,
+                           (const T*)table, vocab, (int)hidden, scale, (T*)out);
+    };
+    if (n_tokens * waves <= 4096 || waves == 1) launch(Int<1>());     // few tokens: spread over the chip
+    else if (waves % 7 == 0) launch(Int<7>());
+    else if (waves % 5 == 0) launch(Int<5>());
+    else if (waves % 3 == 0) launch(Int<3>());
+    else if (waves % 4 == 0) launch(Int<4>());
+    else if (waves % 2 == 0) launch(Int<2>());
+    else launch(Int<4>());
 }
 
 }  // namespace
@@ -280,17 +621,10 @@ extern "C" int mrl_embedding_fwd(const void* ids, int ids_dtype, int64_t n_token
     MRL_REQUIRE(table && out, MRL_ERR_INVALID_ARG, "%s: NULL pointer", fn);
     const size_t es = mrl::float_dtype_bytes(dtype);
     MRL_REQUIRE(mrl::aligned(table, es) && mrl::aligned(out, es), MRL_ERR_MISALIGNED, "%s: misaligned buffer", fn);
-    const dim3 grid((unsigned)n_tokens), block(kBlock);
     hipStream_t s = mrl::as_stream(stream);
-    if (dtype == MRL_F32)
-        hipLaunchKernelGGL((lookup_kernel<MRL_F32>), grid, block, 0, s, ids, ids_dtype, vocab_start, (const float*)table, vocab,
-                           hidden, scale, (float*)out);
-    else if (dtype == MRL_BF16)
-        hipLaunchKernelGGL((lookup_kernel<MRL_BF16>), grid, block, 0, s, ids, ids_dtype, vocab_start, (const uint16_t*)table, vocab,
-                           hidden, scale, (uint16_t*)out);
-    else
-        hipLaunchKernelGGL((lookup_kernel<MRL_F16>), grid, block, 0, s, ids, ids_dtype, vocab_start, (const uint16_t*)table, vocab,
-                           hidden, scale, (uint16_t*)out);
+    if (dtype == MRL_F32) launch_lookup<MRL_F32>(ids, ids_dtype, n_tokens, vocab_start, table, vocab, hidden, scale, out, s);
+    else if (dtype == MRL_BF16) launch_lookup<MRL_BF16>(ids, ids_dtype, n_tokens, vocab_start, table, vocab, hidden, scale, out, s);
+    else launch_lookup<MRL_F16>(ids, ids_dtype, n_tokens, vocab_start, table, vocab, hidden, scale, out, s);
     return mrl::check_launch(fn);
 }
 
@@ -317,14 +651,14 @@ extern "C" int mrl_embedding_bwd(const void* ids, int ids_dtype, int64_t n_token
                     mrl::aligned(workspace, 16),
                 MRL_ERR_MISALIGNED, "%s: misaligned buffer", fn);
     hipStream_t s = mrl::as_stream(stream);
-    if (!accumulate) {
-        const int64_t n = vocab * hidden;
-        const int64_t blocks = (n + kBlock * 16 - 1) / (kBlock * 16);
-        const dim3 grid((unsigned)(blocks < 65536 ? blocks : 65536)), block(kBlock);
-        if (dtable_dtype == MRL_F32) hipLaunchKernelGGL((zero_kernel<MRL_F32>), grid, block, 0, s, (float*)dtable, n);
-        else hipLaunchKernelGGL((zero_kernel<MRL_BF16>), grid, block, 0, s, (uint16_t*)dtable, n);
+    const int64_t fill_bytes = accumulate ? 0 : vocab * hidden * (int64_t)mrl::float_dtype_bytes(dtable_dtype);
+    if (n_tokens == 0) {
+        if (fill_bytes == 0) return MRL_OK;
+        const Fill f = {(char*)dtable, fill_bytes};
+        hipLaunchKernelGGL(sort_count_kernel, dim3(fill_blocks(f)), dim3(kSortBlock), 0, s, (const void*)nullptr, ids_dtype, 0, 0, 1,
+                           SortPlan{1, 1, 0, kSortBlock}, (int32_t*)nullptr, f);
+        return mrl::check_launch(fn);
     }
-    if (n_tokens == 0) return mrl::check_launch(fn);
     const Workspace w = workspace_of(n_tokens, vocab, hidden);
     const SortPlan p = sort_plan(n_tokens, vocab);
     char* base = (char*)workspace;
@@ -334,27 +668,38 @@ extern "C" int mrl_embedding_bwd(const void* ids, int ids_dtype, int64_t n_token
         tokens[q] = (int32_t*)(base + w.tokens[q]);
     }
     int32_t* counts = (int32_t*)(base + w.counts);
-    const dim3 grid((unsigned)p.groups), block(kSortBlock);
-    hipLaunchKernelGGL(sort_count_kernel, grid, block, 0, s, ids, ids_dtype, n_tokens, vocab_start, vocab, p, counts);
-    for (int q = 0; q < p.passes; ++q) {
+    const dim3 block(kSortBlock);
+    if (n_tokens <= kFewTokens) {
+        const Fill f = {(char*)dtable, fill_bytes};
+        const int to = (p.passes - 1) & 1;
+        hipLaunchKernelGGL(sort_few_kernel, dim3(1 + fill_blocks(f)), block, 0, s, ids, ids_dtype, (int)n_tokens, vocab_start, vocab, p,
+                           keys[to], tokens[to], f);
+    }
+    const Fill f0 = fill_share(dtable, fill_bytes, 0, p.passes + 1);
+    if (n_tokens > kFewTokens)
+    hipLaunchKernelGGL(sort_count_kernel, dim3(p.groups + fill_blocks(f0)), block, 0, s, ids, ids_dtype, n_tokens, vocab_start,
+                       vocab, p, counts, f0);
+    for (int q = 0; n_tokens > kFewTokens && q < p.passes; ++q) {
         const int to = q & 1, from = to ^ 1;
         int32_t* here = counts + (int64_t)q * kSortGroups * kDigits;
         int32_t* next = q + 1 < p.passes ? here + (int64_t)kSortGroups * kDigits : nullptr;
+        const Fill f = fill_share(dtable, fill_bytes, q + 1, p.passes + 1);
+        const dim3 grid(p.groups + fill_blocks(f));
         if (q == 0)
             hipLaunchKernelGGL((sort_pass_kernel<true>), grid, block, 0, s, ids, ids_dtype, n_tokens, vocab_start, vocab, p, q,
-                               (const int32_t*)nullptr, (const int32_t*)nullptr, keys[to], tokens[to], here, next);
+                               (const int32_t*)nullptr, (const int32_t*)nullptr, keys[to], tokens[to], here, next, f);
         else
             hipLaunchKernelGGL((sort_pass_kernel<false>), grid, block, 0, s, ids, ids_dtype, n_tokens, vocab_start, vocab, p, q,
-                               keys[from], tokens[from], keys[to], tokens[to], here, next);
+                               keys[from], tokens[from], keys[to], tokens[to], here, next, f);
     }
     const int sorted = (p.passes - 1) & 1;
-    const Sums sums = {keys[sorted], tokens[sorted], (float*)(base + w.part), n_tokens, hidden, share_of(n_tokens),
-                       (int32_t)vocab, scale};
+    const Sums sums = {(float*)(base + w.part), n_tokens, hidden, share_of(n_tokens), (int32_t)vocab, scale};
+    const int32_t *sk = keys[sorted], *st = tokens[sorted];
     const bool add = accumulate != 0;
-    if (dtype == MRL_F32) launch_sums<MRL_F32, MRL_F32>(add, sums, dy, dtable, s);
-    else if (dtype == MRL_BF16 && dtable_dtype == MRL_F32) launch_sums<MRL_BF16, MRL_F32>(add, sums, dy, dtable, s);
-    else if (dtype == MRL_BF16) launch_sums<MRL_BF16, MRL_BF16>(add, sums, dy, dtable, s);
-    else if (dtable_dtype == MRL_F32) launch_sums<MRL_F16, MRL_F32>(add, sums, dy, dtable, s);
-    else launch_sums<MRL_F16, MRL_F16>(add, sums, dy, dtable, s);
+    if (dtype == MRL_F32) launch_sums<MRL_F32, MRL_F32>(add, sums, sk, st, dy, dtable, s);
+    else if (dtype == MRL_BF16 && dtable_dtype == MRL_F32) launch_sums<MRL_BF16, MRL_F32>(add, sums, sk, st, dy, dtable, s);
+    else if (dtype == MRL_BF16) launch_sums<MRL_BF16, MRL_BF16>(add, sums, sk, st, dy, dtable, s);
+    else if (dtable_dtype == MRL_F32) launch_sums<MRL_F16, MRL_F32>(add, sums, sk, st, dy, dtable, s);
+    else launch_sums<MRL_F16, MRL_F16>(add, sums, sk, st, dy, dtable, s);
     return mrl::check_launch(fn);
 }

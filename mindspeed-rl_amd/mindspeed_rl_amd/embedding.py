@@ -10,6 +10,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
+from .vocab_ops import _transformed
 
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 
@@ -38,29 +39,41 @@ def _add_up(ids, dy, scale, vocab_start, out, accumulate):
     return out
 
 
+def _look_up(ids, weight, scale, vocab_start):
+    """The rows, and the ids as the kernels take them."""
+    dev = weight.device
+    table, flat = weight.contiguous(), _lib.index_column(ids, dev)
+    vocab, hidden = table.shape
+    out = torch.empty((*ids.shape, hidden), dtype=table.dtype, device=dev)
+    _lib.call("mrl_embedding_fwd", flat.data_ptr(), _lib.dtype_code(flat), flat.numel(), vocab_start, table.data_ptr(),
+              _lib.dtype_code(table), vocab, hidden, scale, out.data_ptr(), _lib.stream(dev))
+    return out, flat
+
+
+def _backward(ctx, dy):
+    (flat,) = ctx.saved_tensors
+    shape, dtype, scale, vocab_start = ctx.meta
+    out = torch.empty(shape, dtype=dtype, device=dy.device)
+    return None, _add_up(flat, dy.contiguous(), scale, vocab_start, out, False), None, None
+
+
+_backward_once = once_differentiable(_backward)
+
+
 class _TokenEmbedding(torch.autograd.Function):
     """(ids[...], weight[V, H]) -> [..., H]; the backward gives the dense gradient of the table."""
 
     @staticmethod
     def forward(ctx, ids, weight, scale, vocab_start):
-        dev = weight.device
-        table, flat = weight.contiguous(), _lib.index_column(ids, dev)
-        vocab, hidden = table.shape
-        out = torch.empty((*ids.shape, hidden), dtype=table.dtype, device=dev)
-        _lib.call("mrl_embedding_fwd", flat.data_ptr(), _lib.dtype_code(flat), flat.numel(), vocab_start, table.data_ptr(),
-                  _lib.dtype_code(table), vocab, hidden, scale, out.data_ptr(), _lib.stream(dev))
-        if ctx.needs_input_grad[1]:
-            ctx.save_for_backward(flat)
-            ctx.meta = (vocab, hidden, weight.dtype, scale, vocab_start)
+        out, flat = _look_up(ids, weight, scale, vocab_start)
+        ctx.save_for_backward(flat)
+        ctx.meta = (weight.shape, weight.dtype, scale, vocab_start)
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        (flat,) = ctx.saved_tensors
-        vocab, hidden, dtype, scale, vocab_start = ctx.meta
-        out = torch.empty((vocab, hidden), dtype=dtype, device=dy.device)
-        return None, _add_up(flat, dy.contiguous(), scale, vocab_start, out, False), None, None
+        # the wrapper that refuses a second differentiation costs as much as a launch: only where there may be one
+        return _backward_once(ctx, dy) if torch.is_grad_enabled() else _backward(ctx, dy)
 
 
 def token_embedding(ids, weight, scale=1.0, vocab_start=0):
@@ -74,6 +87,8 @@ def token_embedding(ids, weight, scale=1.0, vocab_start=0):
         raise ValueError("weight must have shape (vocab, hidden_dim), not %s" % (tuple(weight.shape),))
     scale, vocab_start = _check(ids, scale, vocab_start)
     _lib.require_device(ids, weight)
+    if not (torch.is_grad_enabled() and weight.requires_grad) and not _transformed():
+        return _look_up(ids, weight, scale, vocab_start)[0]         # nothing for autograd to see
     return _TokenEmbedding.apply(ids, weight, scale, vocab_start)
 
 

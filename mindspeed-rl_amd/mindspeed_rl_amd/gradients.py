@@ -14,14 +14,14 @@ _PARTIALS = 2048            # MRL_GRAD_NORM_PARTIALS
 _CODES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 
 
-def _listed(grads):
-    grads = [grads] if isinstance(grads, torch.Tensor) else [g for g in grads if g is not None]
-    for g in grads:
-        if not isinstance(g, torch.Tensor):
-            raise TypeError("gradients must be tensors, not %s" % type(g).__name__)
-        if g.layout is not torch.strided or g.dtype not in _CODES:
-            raise TypeError("gradients must be dense float32, bfloat16 or float16 tensors, not %s of %s" % (g.layout, g.dtype))
-    return grads
+def _code(g):
+    """The dtype code of a gradient that can be taken."""
+    if not isinstance(g, torch.Tensor):
+        raise TypeError("gradients must be tensors, not %s" % type(g).__name__)
+    code = _CODES.get(g.dtype)
+    if code is None or g.layout is not torch.strided:
+        raise TypeError("gradients must be dense float32, bfloat16 or float16 tensors, not %s of %s" % (g.layout, g.dtype))
+    return code
 
 
 def _steps(t):
@@ -41,16 +41,17 @@ def _fills(t):
     return True
 
 
-def _table(pairs):
-    """The list as mrl_grad structures: ``pairs`` of (gradient, output or None), dense."""
-    words = array.array("q")
-    for g, o in pairs:
-        code = _CODES[g.dtype]
-        if o is None:
-            words.extend((g.data_ptr(), 0, g.numel(), code | code << 32))
-        else:
-            words.extend((g.data_ptr(), o.data_ptr(), g.numel(), code | _CODES[o.dtype] << 32))
-    return words
+def _device(tensors):
+    """Their one device, as :func:`_lib.require_device` would have it."""
+    if not tensors:
+        raise ValueError("no gradients")
+    index = tensors[0].get_device()
+    for t in tensors:
+        if t.get_device() != index:
+            index = -1
+    if index < 0:
+        _lib.require_device(*tensors)       # raises
+    return _lib.require_device(tensors[0])
 
 
 def _result(dev):
@@ -62,15 +63,32 @@ def global_grad_norm(grads):
     """The 2-norm over all entries of ``grads`` (a tensor, or an iterable of them; None is skipped) as an fp32 scalar on their
     device: squares and sums in fp64, in an order that the sizes set.  A tensor that is listed twice counts twice.  Not
     differentiable."""
-    grads = _listed(grads)
-    if not grads:
-        raise ValueError("no gradients")
-    dev = _lib.require_device(*grads)
-    pairs = [(g if _fills(g) else g.detach().contiguous(), None) for g in grads]
-    words = _table(pairs)
+    grads = [grads] if isinstance(grads, torch.Tensor) else [g for g in grads if g is not None]
+    words, kept = [], []
+    for g in grads:
+        code = _code(g)
+        if not _fills(g):
+            g = g.detach().contiguous()
+            kept.append(g)
+        words += (g.data_ptr(), 0, g.numel(), code | code << 32)
+    dev = _device(grads)
+    table = array.array("q", words)
     norm, partial = _result(dev)
-    _lib.call("mrl_grad_norm", words.buffer_info()[0], len(pairs), norm.data_ptr(), partial.data_ptr(), _lib.stream(dev))
+    _lib.call("mrl_grad_norm", table.buffer_info()[0], len(grads), norm.data_ptr(), partial.data_ptr(), _lib.stream(dev))
     return norm
+
+
+def _spaced(g, o, in_place):
+    """(gradient, output) as dense tensors of one order, by copies where they are not."""
+    source = g.detach().contiguous()
+    if o.is_contiguous():
+        return source, o
+    extent = 1
+    for st, n in _steps(o):
+        if st < extent:
+            raise ValueError("an output's entries share memory")
+        extent += (n - 1) * st
+    return source, source if in_place else torch.empty(o.shape, dtype=o.dtype, device=o.device)
 
 
 def clip_grad_norm_(grads, max_norm, out=None):
@@ -81,46 +99,46 @@ def clip_grad_norm_(grads, max_norm, out=None):
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError("max_norm must not be negative: %r" % max_norm)
+    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    words, back, tensors = [], [], []
     if out is None:
-        grads = _listed(grads)
-        outs = grads
+        for g in grads:
+            if g is None:
+                continue
+            code = _code(g)
+            tensors.append(g)
+            p = q = g.data_ptr()
+            if not _fills(g):
+                source, target = _spaced(g, g, True)
+                back.append((g, target))
+                p, q = source.data_ptr(), target.data_ptr()
+            words += (p, q, g.numel(), code | code << 32)
     else:
-        grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
         outs = [out] if isinstance(out, torch.Tensor) else list(out)
         if len(grads) != len(outs):
             raise ValueError("%d gradients and %d outputs" % (len(grads), len(outs)))
-        both = [(g, o) for g, o in zip(grads, outs) if g is not None]
-        grads, outs = _listed([g for g, _ in both]), _listed([o for _, o in both])
-        if len(grads) != len(outs):
-            raise ValueError("a gradient without an output")
         for g, o in zip(grads, outs):
-            if g.shape != o.shape or (o.dtype is not g.dtype and o.dtype is not torch.float32):
+            if g is None:
+                continue
+            if o is None:
+                raise ValueError("a gradient without an output")
+            code, to = _code(g), _code(o)
+            if g.shape != o.shape or (to != code and to != _lib.F32):
                 raise ValueError("an output must have the shape of its gradient, and its type or float32: %s %s and %s %s"
                                  % (tuple(g.shape), g.dtype, tuple(o.shape), o.dtype))
-    if not grads:
-        raise ValueError("no gradients")
-    dev = _lib.require_device(*grads, *([] if out is None else outs))
-    pairs, back = [], []
-    for g, o in zip(grads, outs):
-        g, o = g.detach(), o.detach()
-        if o.data_ptr() == g.data_ptr() and o.dtype is g.dtype and o.stride() == g.stride() and _fills(g):
-            pairs.append((g, g))
-            continue
-        # entries lie in another order than their outputs, or apart: by way of dense tensors
-        source, target = g.contiguous(), o
-        if not o.is_contiguous():
-            extent = 1
-            for st, n in _steps(o):
-                if st < extent:
-                    raise ValueError("an output's entries share memory")
-                extent += (n - 1) * st
-            target = source if out is None else torch.empty(o.shape, dtype=o.dtype, device=dev)
-            back.append((o, target))
-        pairs.append((source, target))
-    words = _table(pairs)
+            tensors += (g, o)
+            p, q = g.data_ptr(), o.data_ptr()
+            if not (g.is_contiguous() and o.is_contiguous()) and not (p == q and g.stride() == o.stride() and _fills(g)):
+                source, target = _spaced(g, o, False)
+                back.append((o, target, source))
+                p, q = source.data_ptr(), target.data_ptr()
+            words += (p, q, g.numel(), code | to << 32)
+    dev = _device(tensors)
+    table = array.array("q", words)
     norm, partial = _result(dev)
-    _lib.call("mrl_grad_clip", words.buffer_info()[0], len(pairs), max_norm, norm.data_ptr(), partial.data_ptr(),
+    _lib.call("mrl_grad_clip", table.buffer_info()[0], len(words) // 4, max_norm, norm.data_ptr(), partial.data_ptr(),
               _lib.stream(dev))
-    for o, target in back:
-        o.copy_(target)
+    for o, target, *_ in back:
+        if target is not o:
+            o.detach().copy_(target)
     return norm

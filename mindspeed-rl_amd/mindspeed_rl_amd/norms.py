@@ -7,9 +7,56 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .vocab_ops import _flat_rows
+from .vocab_ops import _flat_rows, _transformed
 
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def _forward(x, weight, bias, eps, layer, keep):
+    """y, and what the backward takes if `keep`: the rows, their stride, the weight, [mean and] rstd of the rows."""
+    dev, hidden = x.device, x.shape[-1]
+    if x.is_contiguous():
+        flat, n_rows, x_stride, y = x, x.numel() // hidden, hidden, torch.empty_like(x)
+    else:
+        flat, x_stride = _flat_rows(x)
+        n_rows, y = flat.shape[0], torch.empty(x.shape, dtype=x.dtype, device=dev)
+    w, b = weight.contiguous(), None if bias is None else bias.contiguous()
+    stats = p_mean = p_rstd = None
+    if keep:
+        stats = torch.empty((2 if layer else 1, n_rows), dtype=torch.float32, device=dev)
+        p_rstd = stats.data_ptr()
+        p_mean = p_rstd + 4 * n_rows if layer else None
+    _lib.call("mrl_norm_fwd", flat.data_ptr(), _lib.dtype_code(x), n_rows, hidden, x_stride, w.data_ptr(), _lib.ptr(b),
+              _lib.dtype_code(w), 1 if layer else 0, eps, y.data_ptr(), p_mean, p_rstd, _lib.stream(dev))
+    return y, flat, x_stride, w, stats
+
+
+def _backward(ctx, dy):
+    flat, w, stats = ctx.saved_tensors
+    shape, n_rows, hidden, x_stride, layer = ctx.meta
+    dev = flat.device
+    if dy.is_contiguous():
+        dy_stride = hidden
+    else:
+        dy, dy_stride = _flat_rows(dy)
+    need_x, need_w, need_b = ctx.needs_input_grad[:3]
+    dx = dw = db = workspace = None
+    if need_x:
+        dx = torch.empty_like(flat) if flat.is_contiguous() and flat.shape == shape else torch.empty(shape, dtype=flat.dtype, device=dev)
+    ws_bytes = 0
+    if need_w or need_b:
+        dw = torch.empty_like(w) if need_w else None
+        db = torch.empty_like(w) if need_b else None
+        ws_bytes = _lib.load().mrl_norm_bwd_workspace_bytes(n_rows, hidden)
+        workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    p_rstd = stats.data_ptr()
+    _lib.call("mrl_norm_bwd", dy.data_ptr(), dy_stride, flat.data_ptr(), x_stride, _lib.dtype_code(flat), n_rows, hidden,
+              w.data_ptr(), _lib.dtype_code(w), p_rstd + 4 * n_rows if layer else None, p_rstd, _lib.ptr(dx), _lib.ptr(dw),
+              _lib.ptr(db), _lib.ptr(workspace), ws_bytes, _lib.stream(dev))
+    return dx, dw, db, None, None
+
+
+_backward_once = once_differentiable(_backward)
 
 
 class _Norm(torch.autograd.Function):
@@ -17,42 +64,15 @@ class _Norm(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, eps, layer):
-        dev = x.device
-        hidden = x.shape[-1]
-        flat, x_stride = _flat_rows(x)
-        n_rows = flat.shape[0]
-        w, b = weight.contiguous(), None if bias is None else bias.contiguous()
-        y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        p_mean = p_rstd = None
-        if any(ctx.needs_input_grad[:3]):
-            stats = torch.empty((2 if layer else 1, n_rows), dtype=torch.float32, device=dev)
-            p_rstd = stats.data_ptr()
-            p_mean = p_rstd + 4 * n_rows if layer else None
-            ctx.save_for_backward(flat, w, stats)
-            ctx.meta = (x.shape, x_stride, layer, None if bias is None else bias.dtype)
-        _lib.call("mrl_norm_fwd", flat.data_ptr(), _lib.dtype_code(x), n_rows, hidden, x_stride, w.data_ptr(), _lib.ptr(b),
-                  _lib.dtype_code(w), 1 if layer else 0, eps, y.data_ptr(), p_mean, p_rstd, _lib.stream(dev))
+        y, flat, x_stride, w, stats = _forward(x, weight, bias, eps, layer, True)
+        ctx.save_for_backward(flat, w, stats)
+        ctx.meta = (x.shape, stats.shape[1], x.shape[-1], x_stride, layer)
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        flat, w, stats = ctx.saved_tensors
-        shape, x_stride, layer, has_bias = ctx.meta
-        dev = flat.device
-        n_rows, hidden = flat.shape
-        dy, dy_stride = _flat_rows(dy)
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        dx = torch.empty(shape, dtype=flat.dtype, device=dev) if need_x else None
-        dw = torch.empty(hidden, dtype=w.dtype, device=dev) if need_w else None
-        db = torch.empty(hidden, dtype=w.dtype, device=dev) if need_b and has_bias is not None else None
-        ws_bytes = _lib.load().mrl_norm_bwd_workspace_bytes(n_rows, hidden) if need_w or need_b else 0
-        workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
-        p_rstd = stats.data_ptr()
-        _lib.call("mrl_norm_bwd", dy.data_ptr(), dy_stride, flat.data_ptr(), x_stride, _lib.dtype_code(flat), n_rows, hidden,
-                  w.data_ptr(), _lib.dtype_code(w), p_rstd + 4 * n_rows if layer else None, p_rstd, _lib.ptr(dx), _lib.ptr(dw),
-                  _lib.ptr(db), _lib.ptr(workspace), ws_bytes, _lib.stream(dev))
-        return dx, dw, db, None, None
+        # the wrapper that refuses a second differentiation costs as much as a launch: only where there may be one
+        return _backward_once(ctx, dy) if torch.is_grad_enabled() else _backward(ctx, dy)
 
 
 def _norm(x, weight, bias, eps, layer):
@@ -70,6 +90,9 @@ def _norm(x, weight, bias, eps, layer):
     if not 0.0 < eps < float("inf"):
         raise ValueError("eps must be positive and finite, not %r" % eps)
     _lib.require_device(x, weight, bias)
+    if not _transformed() and not (torch.is_grad_enabled() and (
+            x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad))):
+        return _forward(x, weight, bias, eps, layer, False)[0]      # nothing for autograd to see
     return _Norm.apply(x, weight, bias, eps, layer)
 
 
