@@ -754,7 +754,7 @@ int mrl_embedding_bwd(const void* ids, int ids_dtype, int64_t n_tokens, int64_t 
  * Else `out` has the gradient's type or F32.  What is written may not share memory with anything else in the list.
  * A norm that is not finite gives the factor 0 or NaN, as the formula does. */
 #define MRL_GRAD_TENSORS 16384
-#define MRL_GRAD_NORM_PARTIALS 2048
+#define MRL_GRAD_NORM_PARTIALS 2304
 typedef struct mrl_grad {
     const void* data;
     void* out;

@@ -7,7 +7,9 @@
 // holds it, and nothing is copied to the device.
 #include <algorithm>
 
+#include "lane_ops.h"
 #include "mrl_internal.h"
+#include "vector_access.h"
 #include "vocab_common.h"
 
 namespace {
@@ -16,37 +18,91 @@ using mrl_vocab::Elem;
 
 constexpr int kBlock = 256;
 constexpr int kTable = 112;                 // tensors of a launch: 4 KB of arguments
-constexpr int64_t kChunk = 8192;            // entries that a workgroup takes at a time
+constexpr int kSumVecs = 4;                 // vectors of 16 bytes that a thread has on its way where squares are summed
+constexpr int kScaleVecs = 1;               // ... and where gradients are scaled
+constexpr int64_t kCached = 256 << 20;      // bytes that the memory-side cache holds
+
+constexpr int chunk_bytes(int vecs) { return kBlock * vecs * 16; }  // of a tensor that a workgroup takes at a time
 constexpr int kMaxPartials = MRL_GRAD_NORM_PARTIALS;
+constexpr int kGroups = 2048;               // workgroups of a list: eight on each of 256 CUs
 
 struct Part {
     const void* data;
     void* out;
     int64_t n;
-    int32_t last_chunk;                     // chunks of this tensor and the ones in front of it
-    int16_t dtype, out_dtype;
+    int64_t end_chunk;                      // chunks of this tensor and the ones in front of it
 };
 
+// Tensors of one type, and of one type of their outputs.
 struct Table {
     Part part[kTable];
     int32_t n_parts, n_chunks;
+    int32_t in_place;                       // all of them
 };
 
-__device__ __forceinline__ float load_as(const void* p, int dtype, int64_t i) {
-    if (dtype == MRL_F32) return Elem<MRL_F32>::load((const float*)p + i);
-    if (dtype == MRL_BF16) return Elem<MRL_BF16>::load((const uint16_t*)p + i);
-    return Elem<MRL_F16>::load((const uint16_t*)p + i);
+// A chunk of the table: its tensor, its first byte there and how many it has.
+struct Place {
+    int part, bytes;
+    int64_t first;
+};
+
+__device__ __forceinline__ int part_of(const int32_t* ends, int chunk) {       // as many tensors end at or in front of it
+    const int lane = threadIdx.x & 63;
+    return __builtin_amdgcn_readfirstlane(__popcll(__ballot(ends[lane] <= chunk)) + __popcll(__ballot(ends[64 + lane] <= chunk)));
 }
 
-__device__ __forceinline__ void store_as(void* p, int dtype, int64_t i, float v) {
-    if (dtype == MRL_F32) Elem<MRL_F32>::store((float*)p + i, v);
-    else if (dtype == MRL_BF16) Elem<MRL_BF16>::store((uint16_t*)p + i, v);
-    else Elem<MRL_F16>::store((uint16_t*)p + i, v);
+template <int DT, int kVecs>
+__device__ __forceinline__ Place place_of(const Table& t, const int32_t* ends, int chunk) {
+    constexpr int kChunk = chunk_bytes(kVecs);
+    Place c;
+    c.part = part_of(ends, chunk);
+    c.first = (chunk - (c.part == 0 ? 0 : t.part[c.part - 1].end_chunk)) * kChunk;
+    const int64_t left = t.part[c.part].n * (int64_t)sizeof(typename Elem<DT>::T) - c.first;
+    c.bytes = left < kChunk ? (int)left : kChunk;
+    return c;
 }
 
-__device__ __forceinline__ double block_sum(double x, double* lds) {
+template <bool kStream>
+__device__ __forceinline__ u32x4 load_16(const char* p) {
+    const mrl::u32x4_anywhere* v = (const mrl::u32x4_anywhere*)p;
+    return kStream ? __builtin_nontemporal_load(v) : *v;
+}
+
+// Its bytes as raw vectors.  Vectors behind the tensor's end are zeros, of one that the end cuts the entries behind it.
+template <int kVecs, bool kStream>
+__device__ __forceinline__ void load_chunk(const Table& t, const Place& c, u32x4 (&v)[kVecs]) {
+    const char* from = (const char*)t.part[c.part].data + c.first;
+    if (c.bytes == chunk_bytes(kVecs)) {
 #pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) x += __shfl_xor(x, off, 64);
+        for (int q = 0; q < kVecs; ++q) v[q] = load_16<kStream>(from + (q * kBlock + threadIdx.x) * 16);
+        return;
+    }
+#pragma unroll
+    for (int q = 0; q < kVecs; ++q) {
+        const int at = (q * kBlock + threadIdx.x) * 16;
+        v[q] = mrl::make_u32x4(0u, 0u, 0u, 0u);
+        if (at + 16 <= c.bytes) {
+            v[q] = load_16<kStream>(from + at);
+        } else if (at < c.bytes) {
+            uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (at + 2 * i < c.bytes) w[i >> 1] |= (uint32_t)*(const uint16_t*)(from + at + 2 * i) << (16 * (i & 1));
+            v[q] = mrl::make_u32x4(w[0], w[1], w[2], w[3]);
+        }
+    }
+}
+
+// Where the tensors of the table end, in LDS; 128 entries.
+__device__ __forceinline__ void load_ends(const Table& t, int32_t* ends) {
+    if (threadIdx.x < 128) ends[threadIdx.x] = (int)threadIdx.x < t.n_parts ? (int32_t)t.part[threadIdx.x].end_chunk : 0x7fffffff;
+    __syncthreads();
+}
+
+// Sum over the workgroup, the same in every thread.
+__device__ __forceinline__ double block_sum(double x, double* lds) {
+    x = mrl::lanes_sum<4>(x);
+    x = (mrl::lane_value(x, 0) + mrl::lane_value(x, 16)) + (mrl::lane_value(x, 32) + mrl::lane_value(x, 48));
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
     __syncthreads();
     double s = lds[0];
@@ -55,80 +111,158 @@ __device__ __forceinline__ double block_sum(double x, double* lds) {
     return s;
 }
 
-__global__ __launch_bounds__(kBlock) void grad_squares_kernel(Table t, double* __restrict__ partial) {
+// The sum of squares of a workgroup's chunks, one of which is on its way while the one in front is summed.
+template <int DT, bool kStream>
+__global__ __launch_bounds__(kBlock, 8) void grad_squares_kernel(Table t, double* __restrict__ partial) {
     __shared__ double lds[kBlock / 64];
+    __shared__ int32_t ends[128];
+    load_ends(t, ends);
     double acc = 0.0;
-    int k = 0;
+    u32x4 next[kSumVecs];
+    load_chunk<kSumVecs, kStream>(t, place_of<DT, kSumVecs>(t, ends, blockIdx.x), next);
     for (int c = blockIdx.x; c < t.n_chunks; c += gridDim.x) {
-        while (c >= t.part[k].last_chunk) ++k;
-        const int first = k == 0 ? 0 : t.part[k - 1].last_chunk;
-        const int64_t lo = (int64_t)(c - first) * kChunk;
-        const int64_t hi = lo + kChunk < t.part[k].n ? lo + kChunk : t.part[k].n;
-        for (int64_t i = lo + threadIdx.x; i < hi; i += kBlock) {
-            const double g = (double)load_as(t.part[k].data, t.part[k].dtype, i);
-            acc += g * g;
+        u32x4 v[kSumVecs];
+#pragma unroll
+        for (int q = 0; q < kSumVecs; ++q) v[q] = next[q];
+        if (c + (int)gridDim.x < t.n_chunks) load_chunk<kSumVecs, kStream>(t, place_of<DT, kSumVecs>(t, ends, c + gridDim.x), next);
+#pragma unroll
+        for (int q = 0; q < kSumVecs; ++q) {
+            float z[Elem<DT>::kVec];
+            Elem<DT>::unpack(v[q], z);
+#pragma unroll
+            for (int i = 0; i < Elem<DT>::kVec; ++i) acc = __builtin_fma((double)z[i], (double)z[i], acc);
         }
     }
     const double s = block_sum(acc, lds);
     if (threadIdx.x == 0) partial[blockIdx.x] = s;
 }
 
+// The norm from the workgroups' sums, in every thread.
+__device__ __forceinline__ float norm_of(const double* partial, int n, double* lds) {
+    double acc = 0.0;
+    for (int i0 = threadIdx.x; i0 < n; i0 += kBlock * 8) {
+        double v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = partial[i0 + i * kBlock < n ? i0 + i * kBlock : 0];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc += i0 + i * kBlock < n ? v[i] : 0.0;
+    }
+    return (float)sqrt(block_sum(acc, lds));
+}
+
 __global__ __launch_bounds__(kBlock) void grad_norm_kernel(const double* __restrict__ partial, int n, float* __restrict__ norm) {
     __shared__ double lds[kBlock / 64];
-    double acc = 0.0;
-    for (int i = threadIdx.x; i < n; i += kBlock) acc += partial[i];
-    const double s = block_sum(acc, lds);
-    if (threadIdx.x == 0) *norm = (float)sqrt(s);
+    const float v = norm_of(partial, n, lds);
+    if (threadIdx.x == 0) *norm = v;
 }
 
-// fp32 as a caller would form it from the norm that is handed out; NaN (a norm that is none) stays NaN
-__device__ __forceinline__ float clip_factor(float norm, float max_norm) {
-    const float f = max_norm / (norm + 1e-6f);
-    return f > 1.f ? 1.f : f;
-}
-
-__global__ __launch_bounds__(kBlock) void grad_scale_kernel(Table t, const float* __restrict__ norm, float max_norm) {
-    const float f = clip_factor(*norm, max_norm);
-    int k = 0;
-    for (int c = blockIdx.x; c < t.n_chunks; c += gridDim.x) {
-        while (c >= t.part[k].last_chunk) ++k;
-        const Part& p = t.part[k];
-        if (f == 1.f && p.out == p.data) continue;
-        const int64_t lo = (int64_t)(c - (k == 0 ? 0 : t.part[k - 1].last_chunk)) * kChunk;
-        const int64_t hi = lo + kChunk < p.n ? lo + kChunk : p.n;
-        for (int64_t i = lo + threadIdx.x; i < hi; i += kBlock)
-            store_as(p.out, p.out_dtype, i, load_as(p.data, p.dtype, i) * f);
+template <int DT>
+__device__ __forceinline__ void scale_chunk(const Table& t, const Place& c, float f) {
+    constexpr int kVec = Elem<DT>::kVec, kVecs = kScaleVecs;
+    u32x4 v[kVecs];
+    load_chunk<kVecs, true>(t, c, v);
+    typename Elem<DT>::T* to = (typename Elem<DT>::T*)((char*)t.part[c.part].out + c.first);
+    const int n = c.bytes / (16 / kVec);
+#pragma unroll
+    for (int q = 0; q < kVecs; ++q) {
+        const int at = (q * kBlock + threadIdx.x) * kVec;
+        float z[kVec];
+        Elem<DT>::unpack(v[q], z);
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) z[i] *= f;
+        if (at + kVec <= n) {
+            mrl::Vec<DT>::store_nt(to + at, Elem<DT>::pack(z));
+        } else {
+#pragma unroll
+            for (int i = 0; i < kVec; ++i)
+                if (at + i < n) Elem<DT>::store(to + at + i, z[i]);
+        }
     }
 }
 
-int64_t chunks_of(int64_t n) { return (n + kChunk - 1) / kChunk; }
+// To fp32: a lane reads 8 bytes and writes 16, so that what a wavefront writes at a time lies together.
+template <int DT>
+__device__ __forceinline__ void widen_chunk(const Table& t, const Place& c, float f) {
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    typedef u32x2 u32x2_anywhere __attribute__((aligned(2)));
+    constexpr int kUnits = 2 * kScaleVecs;
+    const char* from = (const char*)t.part[c.part].data + c.first;
+    float* to = (float*)t.part[c.part].out + c.first / 2;
+    u32x2 v[kUnits] = {};
+    if (c.bytes >= 8) {
+#pragma unroll
+        for (int q = 0; q < kUnits; ++q) {
+            const int at = (q * kBlock + threadIdx.x) * 8;
+            v[q] = __builtin_nontemporal_load((const u32x2_anywhere*)(from + (at + 8 <= c.bytes ? at : 0)));
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < kUnits; ++q) {
+        const int at = (q * kBlock + threadIdx.x) * 8;
+        if (at + 8 <= c.bytes) {
+            float z[8];
+            Elem<DT>::unpack(mrl::make_u32x4(v[q].x, v[q].y, 0u, 0u), z);
+            mrl::Vec<MRL_F32>::store_nt(to + at / 2, mrl::make_u32x4(__float_as_uint(z[0] * f), __float_as_uint(z[1] * f),
+                                                                     __float_as_uint(z[2] * f), __float_as_uint(z[3] * f)));
+        } else {
+            for (int i = at; i < c.bytes; i += 2) to[i / 2] = Elem<DT>::load((const uint16_t*)(from + i)) * f;
+        }
+    }
+}
 
-// The launches of a list: tables of at most kTable tensors that are not empty and 2^30 chunks; `launch(table)` for each.
+// The norm comes from the partial sums, formed by every workgroup for itself, or from where a launch in front left it
+// (n_partial == 0); the factor in fp32, as a caller would form it from the norm that is handed out (NaN, of a norm that
+// is none, stays NaN).  Chunks are taken from the last to the first: of a list larger than the memory-side cache the last
+// ones are still there.
+template <int DT, int OT>
+__global__ __launch_bounds__(kBlock, 8) void grad_scale_kernel(Table t, const double* __restrict__ partial, int n_partial,
+                                                               float* norm, float max_norm, int write_norm) {
+    __shared__ double lds[kBlock / 64];
+    __shared__ int32_t ends[128];
+    const float total = n_partial > 0 ? norm_of(partial, n_partial, lds) : *norm;
+    if (write_norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = total;
+    const float quotient = max_norm / (total + 1e-6f), f = quotient > 1.f ? 1.f : quotient;
+    if (f == 1.f && t.in_place) return;
+    load_ends(t, ends);
+    for (int c = t.n_chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {
+        const Place at = place_of<DT, kScaleVecs>(t, ends, c);
+        if constexpr (DT == OT) scale_chunk<DT>(t, at, f);
+        else widen_chunk<DT>(t, at, f);
+    }
+}
+
+int64_t bytes_of(const mrl_grad& g) { return g.n * mrl::float_dtype_bytes(g.dtype); }
+
+int64_t chunks_of(const mrl_grad& g, int vecs) { return (bytes_of(g) + chunk_bytes(vecs) - 1) / chunk_bytes(vecs); }
+
+// The launches of a list for the tensors of a kind - type, type of the output (-1: any), whether in place (-1: either) - that
+// are not empty: launch(table) for each at most kTable of them.
 template <typename F>
-void for_tables(const mrl_grad* grads, int64_t n, F launch) {
+void for_tables(const mrl_grad* grads, int64_t n, int vecs, int dtype, int out_dtype, int in_place, F launch) {
     Table t;
     t.n_parts = 0;
+    t.in_place = in_place;
     int64_t chunks = 0;
     for (int64_t i = 0; i < n; ++i) {
-        if (grads[i].n == 0) continue;
-        chunks += chunks_of(grads[i].n);
-        t.part[t.n_parts++] = {grads[i].data, grads[i].out, grads[i].n, (int32_t)chunks, (int16_t)grads[i].dtype,
-                               (int16_t)grads[i].out_dtype};
+        const mrl_grad& g = grads[i];
+        if (g.n == 0 || g.dtype != dtype || (out_dtype >= 0 && g.out_dtype != out_dtype) ||
+            (in_place >= 0 && (g.out == g.data) != (in_place != 0)))
+            continue;
+        chunks += chunks_of(g, vecs);
+        t.part[t.n_parts++] = {g.data, g.out, g.n, chunks};
+        t.n_chunks = (int32_t)chunks;
         if (t.n_parts == kTable) {
-            t.n_chunks = (int32_t)chunks;
             launch(t);
             t.n_parts = 0;
             chunks = 0;
         }
     }
-    if (t.n_parts > 0) {
-        t.n_chunks = (int32_t)chunks;
-        launch(t);
-    }
+    if (t.n_parts > 0) launch(t);
 }
 
 int check_grads(const char* fn, const mrl_grad* grads, int64_t n, bool with_out) {
     MRL_REQUIRE(n >= 0 && (n == 0 || grads), MRL_ERR_INVALID_ARG, "%s: n_grads=%lld", fn, (long long)n);
+    static_assert(kGroups + MRL_GRAD_TENSORS / kTable + 3 <= kMaxPartials, "a partial sum for every workgroup");
     MRL_REQUIRE(n <= MRL_GRAD_TENSORS, MRL_ERR_UNSUPPORTED, "%s: %lld tensors (at most %d)", fn, (long long)n, MRL_GRAD_TENSORS);
     for (int64_t i = 0; i < n; ++i) {
         const mrl_grad& g = grads[i];
@@ -177,18 +311,32 @@ int check_overlap(const char* fn, const mrl_grad* grads, int64_t n) {
     return MRL_OK;
 }
 
-// Squares of all tables into the workspace; the number of partial sums.  A launch has as many workgroups as its share of
-// the entries, so that there are at most kMaxPartials of them (and one for each launch).
-int launch_squares(const mrl_grad* grads, int64_t n, double* partial, hipStream_t s) {
+// Chunks that each workgroup takes: as many as make kGroups of them for the list (and one more at most for each launch).
+int64_t chunks_each(const mrl_grad* grads, int64_t n, int vecs) {
     int64_t total = 0;
-    for (int64_t i = 0; i < n; ++i) total += chunks_of(grads[i].n);
-    const int64_t per = (total + kMaxPartials / 2 - 1) / (kMaxPartials / 2);
+    for (int64_t i = 0; i < n; ++i) total += chunks_of(grads[i], vecs);
+    return (total + kGroups - 1) / kGroups;
+}
+
+// Squares of all tensors into the workspace; the number of partial sums.  A list that is read again and that the
+// memory-side cache holds is left there, anything else goes past it.
+int launch_squares(const mrl_grad* grads, int64_t n, bool read_again, double* partial, hipStream_t s) {
+    const int64_t each = chunks_each(grads, n, kSumVecs);
+    int64_t bytes = 0;
+    for (int64_t i = 0; i < n; ++i) bytes += bytes_of(grads[i]);
+    const bool stream = !read_again || bytes > kCached;
     int used = 0;
-    for_tables(grads, n, [&](const Table& t) {
-        const int groups = (int)((t.n_chunks + per - 1) / per);
-        hipLaunchKernelGGL(grad_squares_kernel, dim3((unsigned)groups), dim3(kBlock), 0, s, t, partial + used);
+    const auto launch = [&](const Table& t, auto through, auto past) {
+        const int groups = (int)((t.n_chunks + each - 1) / each);
+        hipLaunchKernelGGL(stream ? past : through, dim3((unsigned)groups), dim3(kBlock), 0, s, t, partial + used);
         used += groups;
-    });
+    };
+    for_tables(grads, n, kSumVecs, MRL_BF16, -1, -1,
+               [&](const Table& t) { launch(t, grad_squares_kernel<MRL_BF16, false>, grad_squares_kernel<MRL_BF16, true>); });
+    for_tables(grads, n, kSumVecs, MRL_F16, -1, -1,
+               [&](const Table& t) { launch(t, grad_squares_kernel<MRL_F16, false>, grad_squares_kernel<MRL_F16, true>); });
+    for_tables(grads, n, kSumVecs, MRL_F32, -1, -1,
+               [&](const Table& t) { launch(t, grad_squares_kernel<MRL_F32, false>, grad_squares_kernel<MRL_F32, true>); });
     return used;
 }
 
@@ -201,7 +349,7 @@ extern "C" int mrl_grad_norm(const mrl_grad* grads, int64_t n_grads, float* norm
     MRL_REQUIRE(norm && workspace, MRL_ERR_INVALID_ARG, "%s: NULL pointer", fn);
     MRL_REQUIRE(mrl::aligned(norm, 4) && mrl::aligned(workspace, 8), MRL_ERR_MISALIGNED, "%s: misaligned buffer", fn);
     hipStream_t s = mrl::as_stream(stream);
-    const int used = launch_squares(grads, n_grads, workspace, s);
+    const int used = launch_squares(grads, n_grads, false, workspace, s);
     hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(kBlock), 0, s, workspace, used, norm);
     return mrl::check_launch(fn);
 }
@@ -217,11 +365,25 @@ extern "C" int mrl_grad_clip(const mrl_grad* grads, int64_t n_grads, float max_n
     rc = check_overlap(fn, grads, n_grads);
     if (rc != MRL_OK) return rc;
     hipStream_t s = mrl::as_stream(stream);
-    const int used = launch_squares(grads, n_grads, workspace, s);
-    hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(kBlock), 0, s, workspace, used, norm);
-    for_tables(grads, n_grads, [&](const Table& t) {
-        const int groups = t.n_chunks < 4096 ? t.n_chunks : 4096;
-        hipLaunchKernelGGL(grad_scale_kernel, dim3((unsigned)groups), dim3(kBlock), 0, s, t, norm, max_norm);
-    });
+    const int used = launch_squares(grads, n_grads, true, workspace, s);
+    const int64_t each = chunks_each(grads, n_grads, kScaleVecs);
+    // Lists of more chunks than workgroups fit: those that go elsewhere take a workgroup a chunk, which the memory serves
+    // best, and a launch in front forms the norm for them; in place the workgroups stay, for there may be nothing to do.
+    const bool alone = used == 0 || each > 1;
+    if (alone) hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(kBlock), 0, s, workspace, used, norm);
+    int write_norm = alone ? 0 : 1;
+    const auto launch = [&](const Table& t, auto kernel) {
+        const int64_t groups = t.in_place ? (t.n_chunks + each - 1) / each : t.n_chunks;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(kBlock), 0, s, t, workspace, alone ? 0 : used, norm, max_norm,
+                           write_norm);
+        write_norm = 0;
+    };
+    for (int in_place = 0; in_place < 2; ++in_place) {
+        for_tables(grads, n_grads, kScaleVecs, MRL_BF16, MRL_BF16, in_place, [&](const Table& t) { launch(t, grad_scale_kernel<MRL_BF16, MRL_BF16>); });
+        for_tables(grads, n_grads, kScaleVecs, MRL_F16, MRL_F16, in_place, [&](const Table& t) { launch(t, grad_scale_kernel<MRL_F16, MRL_F16>); });
+        for_tables(grads, n_grads, kScaleVecs, MRL_F32, MRL_F32, in_place, [&](const Table& t) { launch(t, grad_scale_kernel<MRL_F32, MRL_F32>); });
+    }
+    for_tables(grads, n_grads, kScaleVecs, MRL_BF16, MRL_F32, 0, [&](const Table& t) { launch(t, grad_scale_kernel<MRL_BF16, MRL_F32>); });
+    for_tables(grads, n_grads, kScaleVecs, MRL_F16, MRL_F32, 0, [&](const Table& t) { launch(t, grad_scale_kernel<MRL_F16, MRL_F32>); });
     return mrl::check_launch(fn);
 }

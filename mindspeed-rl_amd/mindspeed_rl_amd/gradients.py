@@ -10,7 +10,7 @@ import torch
 
 from . import _lib
 
-_PARTIALS = 2048            # MRL_GRAD_NORM_PARTIALS
+_PARTIALS = 2304            # MRL_GRAD_NORM_PARTIALS
 _CODES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 
 
