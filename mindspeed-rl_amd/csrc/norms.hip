@@ -266,12 +266,14 @@ __global__ __launch_bounds__(1024) void norm_fwd_rows_kernel(const typename Elem
 // row would wait for that as well.
 constexpr int kBwdBlock = 512;              // threads of a workgroup that holds several teams
 constexpr int kBwdGroups = 512;             // most workgroups: two on each of 256 CUs
+constexpr int kBwdFewTurns = 4;             // that one workgroup takes alone: the second launch costs more
 
 template <int DT, int WDT, bool kLayer, int kVecs, int kBlockMost, bool kStream>
 __global__ __launch_bounds__(kBlockMost) void norm_bwd_rows_kernel(
     const typename Elem<DT>::T* __restrict__ dy, int64_t dy_stride, const typename Elem<DT>::T* __restrict__ x, int64_t x_stride,
     int64_t n_rows, int hidden, int lanes, const typename Elem<WDT>::T* __restrict__ weight, const float* __restrict__ mean,
-    const float* __restrict__ rstd, typename Elem<DT>::T* __restrict__ dx, float* __restrict__ part) {
+    const float* __restrict__ rstd, typename Elem<DT>::T* __restrict__ dx, float* __restrict__ part,
+    typename Elem<WDT>::T* __restrict__ dweight, typename Elem<WDT>::T* __restrict__ dbias) {
     constexpr int kVec = Elem<DT>::kVec, kWVec = Elem<WDT>::kVec;
     constexpr bool kOne = kBlockMost > kBwdBlock;       // the team is the workgroup
     extern __shared__ float columns[];                  // [kVecs * kVec][lanes] sums on their way between teams
@@ -355,7 +357,7 @@ __global__ __launch_bounds__(kBlockMost) void norm_bwd_rows_kernel(
             else mrl::Vec<DT>::store(dxr + col.at(q), Elem<DT>::pack(z));
         }
     }
-    if (!part) return;
+    if (!part && !dweight && !dbias) return;
     // the workgroup's sums: teams of a wavefront by lane exchange, then one after the other through LDS
     const bool paired = !kOne && lanes < 64;
     const int turns = paired ? blockDim.x >> 6 : teams, mine = paired ? threadIdx.x >> 6 : team;
@@ -372,7 +374,8 @@ __global__ __launch_bounds__(kBlockMost) void norm_bwd_rows_kernel(
                     s += __shfl_xor(s, 32, 64);
                 }
         }
-        float* out = part + ((int64_t)blockIdx.x * 2 + b) * hidden;
+        float* out = part ? part + ((int64_t)blockIdx.x * 2 + b) * hidden : nullptr;
+        typename Elem<WDT>::T* vec = b ? dbias : dweight;       // the sums themselves, of the only workgroup
         for (int t = 0; t < turns; ++t) {
             if (t == mine && holds) {
 #pragma unroll
@@ -385,7 +388,11 @@ __global__ __launch_bounds__(kBlockMost) void norm_bwd_rows_kernel(
                         if (t < turns - 1) *at = s[i];
                     }
                     if (t < turns - 1) continue;
-                    if (q < kVecs - 1 || col.skip == 0) {
+                    if (!out) {
+#pragma unroll
+                        for (int i = 0; i < kVec; ++i)
+                            if (vec && col.own(q, i)) Elem<WDT>::store(vec + col.at(q) + i, s[i]);
+                    } else if (q < kVecs - 1 || col.skip == 0) {
 #pragma unroll
                         for (int p = 0; p < kVec; p += 4)
                             mrl::Vec<MRL_F32>::store(out + col.at(q) + p, mrl::make_u32x4(__float_as_uint(s[p]),
@@ -458,6 +465,7 @@ int bwd_block(const Team& team) { return team.lanes > kBwdBlock ? team.lanes : k
 int bwd_groups(const Team& team, int64_t n_rows) {
     const int teams = bwd_block(team) / team.lanes;
     const int64_t turns = (n_rows + teams - 1) / teams, fit = team.lanes > kBwdBlock ? kBwdGroups / 2 : kBwdGroups;
+    if (turns <= kBwdFewTurns) return 1;
     const int64_t each = (turns + fit - 1) / fit;       // and no more workgroups than take as long
     return (int)((turns + each - 1) / each);
 }
@@ -530,7 +538,8 @@ void launch_bwd(const BwdArgs& a) {
                                                      decltype(stream)::value != 0>),
                                dim3((unsigned)groups), dim3(block), sums && block > team.lanes ? (size_t)team.lanes * team.vecs * Elem<DT>::kVec * 4 : 0, a.stream,
                                (const T*)a.dy, a.dy_stride, (const T*)a.x, a.x_stride, a.n_rows, (int)a.hidden, team.lanes,
-                               (const W*)a.weight, a.mean, a.rstd, (T*)a.dx, sums ? a.part : nullptr);
+                               (const W*)a.weight, a.mean, a.rstd, (T*)a.dx, sums && groups > 1 ? a.part : nullptr,
+                               groups > 1 ? (W*)nullptr : (W*)a.dweight, groups > 1 ? (W*)nullptr : (W*)a.dbias);
         };
         const auto launch_block = [&](auto stream) {
             if (team.vecs == 4) launch(Int<4>(), Int<1024>(), stream);
@@ -541,7 +550,7 @@ void launch_bwd(const BwdArgs& a) {
         };
         if (team.lanes >= 64 && a.hidden * (int64_t)sizeof(T) % 128 == 0) launch_block(Int<1>());
         else launch_block(Int<0>());
-        if (sums)
+        if (sums && groups > 1)
             hipLaunchKernelGGL((norm_part_sum_kernel<WDT>), dim3((unsigned)((a.hidden + 31) / 32), a.dbias ? 2 : 1), dim3(1024), 0,
                                a.stream, a.part, groups, a.hidden, (W*)a.dweight, (W*)a.dbias);
         return;

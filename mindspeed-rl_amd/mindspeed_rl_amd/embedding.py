@@ -4,6 +4,7 @@
 A table that both ends share has two gradients: the lm_head's, which is dense, and the tokens'.  :func:`token_embedding_grad`
 with ``accumulate=True`` adds the latter to the former and touches the named rows alone.
 """
+import functools
 import math
 
 import torch
@@ -26,13 +27,19 @@ def _check(ids, scale, vocab_start):
     return scale, vocab_start
 
 
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(n_tokens, vocab, hidden):
+    """mrl_embedding_bwd_workspace_bytes: a function of its arguments alone."""
+    return _lib.load().mrl_embedding_bwd_workspace_bytes(n_tokens, vocab, hidden)
+
+
 def _add_up(ids, dy, scale, vocab_start, out, accumulate):
     """mrl_embedding_bwd: ``dy`` of ``ids`` (both dense) into ``out`` ``[V, H]``."""
     dev = out.device
     vocab, hidden = out.shape
     n = ids.numel()
-    ws_bytes = _lib.load().mrl_embedding_bwd_workspace_bytes(n, vocab, hidden)
-    workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+    ws_bytes = _workspace_bytes(n, vocab, hidden)
+    workspace = out.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
     _lib.call("mrl_embedding_bwd", ids.data_ptr(), _lib.dtype_code(ids), n, vocab_start, dy.data_ptr(), _lib.dtype_code(dy), vocab,
               hidden, scale, out.data_ptr(), _lib.dtype_code(out), 1 if accumulate else 0, _lib.ptr(workspace), ws_bytes,
               _lib.stream(dev))
@@ -44,7 +51,7 @@ def _look_up(ids, weight, scale, vocab_start):
     dev = weight.device
     table, flat = weight.contiguous(), _lib.index_column(ids, dev)
     vocab, hidden = table.shape
-    out = torch.empty((*ids.shape, hidden), dtype=table.dtype, device=dev)
+    out = table.new_empty((*ids.shape, hidden))
     _lib.call("mrl_embedding_fwd", flat.data_ptr(), _lib.dtype_code(flat), flat.numel(), vocab_start, table.data_ptr(),
               _lib.dtype_code(table), vocab, hidden, scale, out.data_ptr(), _lib.stream(dev))
     return out, flat
@@ -53,7 +60,7 @@ def _look_up(ids, weight, scale, vocab_start):
 def _backward(ctx, dy):
     (flat,) = ctx.saved_tensors
     shape, dtype, scale, vocab_start = ctx.meta
-    out = torch.empty(shape, dtype=dtype, device=dy.device)
+    out = dy.new_empty(shape, dtype=dtype)
     return None, _add_up(flat, dy.contiguous(), scale, vocab_start, out, False), None, None
 
 
@@ -87,9 +94,9 @@ def token_embedding(ids, weight, scale=1.0, vocab_start=0):
         raise ValueError("weight must have shape (vocab, hidden_dim), not %s" % (tuple(weight.shape),))
     scale, vocab_start = _check(ids, scale, vocab_start)
     _lib.require_device(ids, weight)
-    if not (torch.is_grad_enabled() and weight.requires_grad) and not _transformed():
-        return _look_up(ids, weight, scale, vocab_start)[0]         # nothing for autograd to see
-    return _TokenEmbedding.apply(ids, weight, scale, vocab_start)
+    if torch.is_grad_enabled() and weight.requires_grad or _transformed():
+        return _TokenEmbedding.apply(ids, weight, scale, vocab_start)
+    return _look_up(ids, weight, scale, vocab_start)[0]             # nothing for autograd to see
 
 
 def token_embedding_grad(ids, grad, out, scale=1.0, vocab_start=0, accumulate=False):

@@ -3,6 +3,8 @@ that :func:`lmhead_logprob` and the loss objects with ``lm_head_weight=`` take.
 
 The reference leaves them to the model below it; the loss objects call them with ``final_norm_weight=``.
 """
+import functools
+
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -10,6 +12,12 @@ from . import _lib
 from .vocab_ops import _flat_rows, _transformed
 
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(n_rows, hidden):
+    """mrl_norm_bwd_workspace_bytes: a function of its arguments alone."""
+    return _lib.load().mrl_norm_bwd_workspace_bytes(n_rows, hidden)
 
 
 def _forward(x, weight, bias, eps, layer, keep):
@@ -23,7 +31,7 @@ def _forward(x, weight, bias, eps, layer, keep):
     w, b = weight.contiguous(), None if bias is None else bias.contiguous()
     stats = p_mean = p_rstd = None
     if keep:
-        stats = torch.empty((2 if layer else 1, n_rows), dtype=torch.float32, device=dev)
+        stats = weight.new_empty((2 if layer else 1, n_rows), dtype=torch.float32)
         p_rstd = stats.data_ptr()
         p_mean = p_rstd + 4 * n_rows if layer else None
     _lib.call("mrl_norm_fwd", flat.data_ptr(), _lib.dtype_code(x), n_rows, hidden, x_stride, w.data_ptr(), _lib.ptr(b),
@@ -47,8 +55,8 @@ def _backward(ctx, dy):
     if need_w or need_b:
         dw = torch.empty_like(w) if need_w else None
         db = torch.empty_like(w) if need_b else None
-        ws_bytes = _lib.load().mrl_norm_bwd_workspace_bytes(n_rows, hidden)
-        workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        ws_bytes = _workspace_bytes(n_rows, hidden)
+        workspace = w.new_empty(ws_bytes, dtype=torch.uint8)
     p_rstd = stats.data_ptr()
     _lib.call("mrl_norm_bwd", dy.data_ptr(), dy_stride, flat.data_ptr(), x_stride, _lib.dtype_code(flat), n_rows, hidden,
               w.data_ptr(), _lib.dtype_code(w), p_rstd + 4 * n_rows if layer else None, p_rstd, _lib.ptr(dx), _lib.ptr(dw),
@@ -90,10 +98,10 @@ def _norm(x, weight, bias, eps, layer):
     if not 0.0 < eps < float("inf"):
         raise ValueError("eps must be positive and finite, not %r" % eps)
     _lib.require_device(x, weight, bias)
-    if not _transformed() and not (torch.is_grad_enabled() and (
-            x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad))):
-        return _forward(x, weight, bias, eps, layer, False)[0]      # nothing for autograd to see
-    return _Norm.apply(x, weight, bias, eps, layer)
+    if (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad))
+            or _transformed()):
+        return _Norm.apply(x, weight, bias, eps, layer)
+    return _forward(x, weight, bias, eps, layer, False)[0]          # nothing for autograd to see
 
 
 def layer_norm(x, weight, bias=None, eps=1e-5):
