@@ -22,7 +22,7 @@ constexpr int kSortWaves = kSortBlock / 64;
 constexpr int kDigits = 512;
 constexpr int kDigitBits = 9;
 constexpr int kSortGroups = 128;            // most workgroups of a sort pass
-constexpr int kShares = 1024;               // most shares of the sorted list
+constexpr int kShares = 4096;               // most shares of the sorted list
 constexpr int kMinShare = 8;
 constexpr int kFewTokens = 2048;            // that one workgroup sorts in its LDS
 
@@ -161,7 +161,8 @@ struct Placing {
             base += c;
         }
     }
-    // put(t, key, at) for every token, in order within the wavefront: lanes of equal digit find each other by ballots.
+    // put(t, key, at, same) for every token, in order within the wavefront: lanes of equal digit (`same`) find each other by
+    // ballots.
     template <typename Key, typename Put>
     __device__ __forceinline__ void run(Key key_at, Put put) const {
         const int lane = threadIdx.x & 63;
@@ -180,7 +181,7 @@ struct Placing {
             __builtin_amdgcn_wave_barrier();
             if (active) {
                 if ((same >> lane) == 1ull) mine[digit] = at + 1;   // the last lane of this digit
-                put(t, key, at);
+                put(t, key, at, same);
             }
             __builtin_amdgcn_wave_barrier();
         }
@@ -241,11 +242,18 @@ __global__ __launch_bounds__(kSortBlock) void sort_pass_kernel(const void* __res
     step.start(base);
     __syncthreads();
     const uint32_t per_group = (uint32_t)p.per_group;
-    step.run(key_at, [&](int64_t t, int32_t key, int32_t at) {
+    step.run(key_at, [&](int64_t t, int32_t key, int32_t at, uint64_t same) {
         keys_out[at] = key;
         tokens_out[at] = kFirst ? (int32_t)t : tokens_in[t];
-        if (next_counts)
-            atomicAdd(&next_counts[(uint32_t)at / per_group * kDigits + ((key >> (step.shift + p.bits)) & ((1 << p.bits) - 1))], 1);
+        if (!next_counts) return;
+        // lanes that count what the first lane of their digit counts leave it to that: a token that is everywhere would
+        // have every lane add to one counter (49 152 tokens, most of two kinds: 15 us a pass without)
+        const uint32_t counter = (uint32_t)at / per_group * kDigits + ((key >> (step.shift + p.bits)) & ((1 << p.bits) - 1));
+        const int first = __ffsll((unsigned long long)same) - 1;
+        const bool with_first = counter == (uint32_t)__shfl((int)counter, first, 64);
+        const uint64_t counted = same & __ballot(with_first);
+        if ((int)(threadIdx.x & 63) == first) atomicAdd(&next_counts[counter], __popcll(counted));
+        else if (!with_first) atomicAdd(&next_counts[counter], 1);
     });
 }
 
@@ -278,7 +286,7 @@ __global__ __launch_bounds__(kSortBlock) void sort_few_kernel(const void* __rest
         for (int w = 0; w < kSortWaves; ++w) total += place[w][tid];
         step.start(sum_in_front(total, wave_sum));
         __syncthreads();
-        step.run(key_at, [&](int64_t t, int32_t key, int32_t at) {
+        step.run(key_at, [&](int64_t t, int32_t key, int32_t at, uint64_t) {
             if (last) {
                 keys_out[at] = key;
                 tokens_out[at] = tokens[from][t];
@@ -413,25 +421,44 @@ __global__ __launch_bounds__(kSumBlock) void sum_kernel(Sums s, const int32_t* _
     finish(next == key);
 }
 
-constexpr int kJoinWaves = 8, kJoinColumns = 64, kJoinGroups = 64, kJoinShort = 16;
-constexpr int kMaxShares = kJoinGroups * 64;
+constexpr int kJoinWaves = 8;
+constexpr int kJoinShort = 16;              // shares of a run that a wavefront joins alone
+constexpr int kJoinAhead = 16;              // parts that a wavefront has on its way
+static_assert(kShares <= 64 * 64, "two steps find where a run ends");
 
-// The runs that cross shares.  A workgroup takes a tile of columns and every kJoinGroups-th share, a lane for each at first:
+// kCols columns of a lane: one, or four with one access for all of them.
+template <int kCols>
+struct Few {
+    float v[kCols];
+    static __device__ __forceinline__ Few load(const float* p) {
+        Few f;
+        if constexpr (kCols == 1) f.v[0] = *p;
+        else mrl_vocab::Elem<MRL_F32>::unpack(mrl::Vec<MRL_F32>::load(p), f.v);
+        return f;
+    }
+    __device__ __forceinline__ void add(const Few& o, bool counts) {
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) v[i] += counts ? o.v[i] : 0.f;
+    }
+};
+
+// The runs that cross shares.  A workgroup takes a tile of columns and every gridDim.y-th share, a lane for each at first:
 // does such a run begin there, and in how many shares does it go on.  Short runs are joined by a wavefront each, long ones by
 // all of them, each taking every kJoinWaves-th part.
-template <int GT, bool kAdd>
-__global__ __launch_bounds__(kJoinWaves* kJoinColumns) void join_kernel(Sums s, const int32_t* __restrict__ keys,
-                                                                        typename Elem<GT>::T* __restrict__ dtable) {
-    __shared__ float lds[kJoinWaves][kJoinColumns];
+template <int GT, bool kAdd, int kCols>
+__global__ __launch_bounds__(kJoinWaves * 64) void join_kernel(Sums s, const int32_t* __restrict__ keys,
+                                                               typename Elem<GT>::T* __restrict__ dtable) {
+    __shared__ float lds[kJoinWaves][64 * kCols];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t j = (int64_t)blockIdx.x * kJoinColumns + lane;
-    const int64_t jc = j < s.hidden ? j : s.hidden - 1;
+    // a row that is not whole lanes ends with one that overlaps the one in front of it
+    const int64_t want = ((int64_t)blockIdx.x * 64 + lane) * kCols, col = want < s.hidden - kCols ? want : s.hidden - kCols;
+    const int skip = want >= s.hidden ? kCols : (int)(want - col);
     // whether the run of `key` goes on in share g
     const auto goes_on = [&](int64_t g, int32_t key) {
         const int64_t first = g * s.share;
         return first < s.n_tokens && keys[first < s.n_tokens ? first : 0] == key;
     };
-    const int64_t mine = blockIdx.y + (int64_t)lane * kJoinGroups, mine_end = (mine + 1) * s.share;
+    const int64_t mine = blockIdx.y + (int64_t)lane * gridDim.y, mine_end = (mine + 1) * s.share;
     int32_t my_key = s.vocab;
     int more = 0;                                                   // shares behind this one, kJoinShort: as many or more
     if (mine_end < s.n_tokens) {
@@ -445,51 +472,56 @@ __global__ __launch_bounds__(kJoinWaves* kJoinColumns) void join_kernel(Sums s, 
             }
         }
     }
-    const auto put = [&](int32_t key, float sum) {
-        if (j >= s.hidden) return;
-        typename Elem<GT>::T* at = dtable + key * s.hidden + j;
-        Elem<GT>::store(at, kAdd ? Elem<GT>::load(at) + sum * s.scale : sum * s.scale);
+    const auto put = [&](int32_t key, const Few<kCols>& sum) {
+        typename Elem<GT>::T* at = dtable + key * s.hidden + col;
+#pragma unroll
+        for (int i = 0; i < kCols; ++i)
+            if (i >= skip) Elem<GT>::store(at + i, kAdd ? Elem<GT>::load(at + i) + sum.v[i] * s.scale : sum.v[i] * s.scale);
     };
+    const auto part = [&](int64_t share, int slot) { return Few<kCols>::load(s.part + (share * 2 + slot) * s.hidden + col); };
     int nth = 0;
     for (uint64_t todo = __ballot(more > 0 && more < kJoinShort); todo != 0; todo &= todo - 1, ++nth) {
         if (nth % kJoinWaves != wave) continue;
         const int from = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)todo) - 1);
-        const int64_t share = blockIdx.y + (int64_t)from * kJoinGroups;
+        const int64_t share = blockIdx.y + (int64_t)from * gridDim.y;
         const int n = __shfl(more, from, 64);
-        float v[kJoinShort];
-        v[0] = s.part[(share * 2 + 1) * s.hidden + jc];
+        Few<kCols> sum = part(share, 1);
+        for (int i0 = 1; i0 <= n; i0 += 5) {
+            Few<kCols> v[5];
 #pragma unroll
-        for (int i = 1; i < kJoinShort; ++i) v[i] = s.part[(share + (i <= n ? i : n)) * 2 * s.hidden + jc];
-        float sum = v[0];
+            for (int i = 0; i < 5; ++i) v[i] = part(share + (i0 + i <= n ? i0 + i : n), 0);
 #pragma unroll
-        for (int i = 1; i < kJoinShort; ++i) sum += i <= n ? v[i] : 0.f;
+            for (int i = 0; i < 5; ++i) sum.add(v[i], i0 + i <= n);
+        }
         put(__shfl(my_key, from, 64), sum);
     }
     for (uint64_t todo = __ballot(more == kJoinShort); todo != 0; todo &= todo - 1) {       // the same in every wavefront
         const int from = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)todo) - 1);
-        const int64_t share = blockIdx.y + (int64_t)from * kJoinGroups;
+        const int64_t share = blockIdx.y + (int64_t)from * gridDim.y;
         const int32_t key = __shfl(my_key, from, 64);
+        // the last share that it goes on in: in steps of 64 shares (64 of them are more than kShares), then one by one
         int64_t last = share + kJoinShort;
-        for (uint64_t in = ~0ull; in == ~0ull;) {
-            in = __ballot(goes_on(last + 1 + lane, key));           // shares in a row from the front
-            last += in == ~0ull ? 64 : __ffsll((unsigned long long)~in) - 1;
-        }
-        float sum = 0.f;
-        for (int64_t g = share + wave; g <= last; g += kJoinWaves * 8) {
-            float v[8];
+        last += 64 * __popcll(__ballot(goes_on(last + 64 * (lane + 1), key)));
+        last += __popcll(__ballot(goes_on(last + 1 + lane, key)));
+        Few<kCols> sum = {};
+        for (int64_t g = share + wave; g <= last; g += kJoinWaves * kJoinAhead) {
+            Few<kCols> v[kJoinAhead];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int64_t part = g + i * kJoinWaves <= last ? g + i * kJoinWaves : last;
-                v[i] = s.part[(part * 2 + (part == share ? 1 : 0)) * s.hidden + jc];
+            for (int i = 0; i < kJoinAhead; ++i) {
+                const int64_t p = g + i * kJoinWaves <= last ? g + i * kJoinWaves : last;
+                v[i] = part(p, p == share ? 1 : 0);
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum += g + i * kJoinWaves <= last ? v[i] : 0.f;
+            for (int i = 0; i < kJoinAhead; ++i) sum.add(v[i], g + i * kJoinWaves <= last);
         }
-        lds[wave][lane] = sum;
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) lds[wave][i * 64 + lane] = sum.v[i];
         __syncthreads();
         if (wave == 0) {
 #pragma unroll
-            for (int w = 1; w < kJoinWaves; ++w) sum += lds[w][lane];
+            for (int w = 1; w < kJoinWaves; ++w)
+#pragma unroll
+                for (int i = 0; i < kCols; ++i) sum.v[i] += lds[w][i * 64 + lane];
             put(key, sum);
         }
         __syncthreads();
@@ -497,17 +529,20 @@ __global__ __launch_bounds__(kJoinWaves* kJoinColumns) void join_kernel(Sums s, 
 }
 
 // ------------------------------------------------------------------------------------ host
-int64_t round16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
-
-int64_t share_of(int64_t n_tokens) {
-    const int64_t s = (n_tokens + kShares - 1) / kShares;
-    return s < kMinShare ? kMinShare : s;
-}
-
 template <int N>
 struct Int {
     static constexpr int value = N;
 };
+
+int64_t round16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
+
+int64_t share_of(int64_t n_tokens, int64_t hidden) {
+    // as many as 256 CUs hold at a time, 32 wavefronts each, with a vector of eight entries a lane and at most 8 to a share
+    const int64_t waves = (hidden + 64 * 8 - 1) / (64 * 8), fit = 256 * (32 / (waves < 8 ? waves : 8));
+    const int64_t most = fit < kShares ? fit : kShares;
+    const int64_t s = (n_tokens + most - 1) / most;
+    return s < kMinShare ? kMinShare : s;
+}
 
 struct Workspace {
     int64_t keys[2], tokens[2], counts, part, bytes;
@@ -526,7 +561,7 @@ Workspace workspace_of(int64_t n_tokens, int64_t vocab, int64_t hidden) {
     w.counts = at;
     at += (int64_t)p.passes * kSortGroups * kDigits * 4;
     w.part = at;
-    const int64_t share = share_of(n_tokens);
+    const int64_t share = share_of(n_tokens, hidden);
     at += (n_tokens + share - 1) / share * 2 * hidden * 4;
     w.bytes = at;
     return w;
@@ -548,8 +583,6 @@ int check_sizes(const char* fn, const void* ids, int ids_dtype, int64_t n_tokens
     return MRL_OK;
 }
 
-static_assert(kShares <= kMaxShares, "a lane of the join for every share");
-
 template <int DT, int GT, bool kAdd>
 void launch_sums(const Sums& s, const int32_t* keys, const int32_t* tokens, const void* dy, void* dtable, hipStream_t stream) {
     using T = typename Elem<DT>::T;
@@ -563,11 +596,16 @@ void launch_sums(const Sums& s, const int32_t* keys, const int32_t* tokens, cons
         hipLaunchKernelGGL((sum_kernel<DT, GT, kAdd>), dim3((unsigned)shares, (unsigned)((nv + block - 1) / block)),
                            dim3((unsigned)block), 0, stream, s, keys, tokens, (const T*)dy, (G*)dtable);
     }
-    if (shares > 1)
-        hipLaunchKernelGGL((join_kernel<GT, kAdd>),
-                           dim3((unsigned)((s.hidden + kJoinColumns - 1) / kJoinColumns),
-                                (unsigned)(shares < kJoinGroups ? shares : kJoinGroups)),
-                           dim3(kJoinWaves * kJoinColumns), 0, stream, s, keys, (G*)dtable);
+    if (shares <= 1) return;
+    // 16 shares a workgroup, where there are few tiles of columns 8; a lane for each, so never more than 64
+    const auto join = [&](auto cols) {
+        constexpr int kCols = decltype(cols)::value;
+        const int64_t tiles = (s.hidden + 64 * kCols - 1) / (64 * kCols), each = tiles >= 8 ? 16 : 8;
+        hipLaunchKernelGGL((join_kernel<GT, kAdd, kCols>), dim3((unsigned)tiles, (unsigned)((shares + each - 1) / each)),
+                           dim3(kJoinWaves * 64), 0, stream, s, keys, (G*)dtable);
+    };
+    if (s.hidden >= 256) join(Int<4>());
+    else join(Int<1>());
 }
 
 template <int DT, int GT>
@@ -693,7 +731,7 @@ extern "C" int mrl_embedding_bwd(const void* ids, int ids_dtype, int64_t n_token
                                keys[from], tokens[from], keys[to], tokens[to], here, next, f);
     }
     const int sorted = (p.passes - 1) & 1;
-    const Sums sums = {(float*)(base + w.part), n_tokens, hidden, share_of(n_tokens), (int32_t)vocab, scale};
+    const Sums sums = {(float*)(base + w.part), n_tokens, hidden, share_of(n_tokens, hidden), (int32_t)vocab, scale};
     const int32_t *sk = keys[sorted], *st = tokens[sorted];
     const bool add = accumulate != 0;
     if (dtype == MRL_F32) launch_sums<MRL_F32, MRL_F32>(add, sums, sk, st, dy, dtable, s);
