@@ -25,6 +25,7 @@ constexpr int kSortGroups = 128;            // most workgroups of a sort pass
 constexpr int kShares = 4096;               // most shares of the sorted list
 constexpr int kMinShare = 8;
 constexpr int kFewTokens = 2048;            // that one workgroup sorts in its LDS
+constexpr int64_t kMostTokens = 1LL << 26;  // with a wavefront each, as many as a launch holds
 
 // the row that a token names, `vocab` where it is outside
 __device__ __forceinline__ int32_t row_of(const void* ids, int dtype, int64_t t, int64_t start, int64_t vocab) {
@@ -574,8 +575,8 @@ int check_sizes(const char* fn, const void* ids, int ids_dtype, int64_t n_tokens
     MRL_REQUIRE(n_tokens >= 0 && start >= 0 && vocab >= 1 && hidden >= 1, MRL_ERR_INVALID_ARG,
                 "%s: n_tokens=%lld vocab_start=%lld vocab=%lld hidden=%lld", fn, (long long)n_tokens, (long long)start,
                 (long long)vocab, (long long)hidden);
-    MRL_REQUIRE(n_tokens <= 0x7fffffffLL && vocab < 0x7fffffffLL && hidden <= MRL_NORM_MAX_HIDDEN, MRL_ERR_UNSUPPORTED,
-                "%s: n_tokens=%lld vocab=%lld hidden=%lld (at most 2^31 - 1, 2^31 - 2 and %d)", fn, (long long)n_tokens,
+    MRL_REQUIRE(n_tokens < kMostTokens && vocab < 0x7fffffffLL && hidden <= MRL_NORM_MAX_HIDDEN, MRL_ERR_UNSUPPORTED,
+                "%s: n_tokens=%lld vocab=%lld hidden=%lld (at most 2^26 - 1, 2^31 - 2 and %d)", fn, (long long)n_tokens,
                 (long long)vocab, (long long)hidden, MRL_NORM_MAX_HIDDEN);
     MRL_REQUIRE(scale - scale == 0.f, MRL_ERR_INVALID_ARG, "%s: scale=%g", fn, (double)scale);
     MRL_REQUIRE(n_tokens == 0 || ids, MRL_ERR_INVALID_ARG, "%s: NULL ids", fn);
@@ -667,7 +668,7 @@ extern "C" int mrl_embedding_fwd(const void* ids, int ids_dtype, int64_t n_token
 }
 
 extern "C" int64_t mrl_embedding_bwd_workspace_bytes(int64_t n_tokens, int64_t vocab, int64_t hidden) {
-    if (n_tokens <= 0 || vocab <= 0 || hidden <= 0 || n_tokens > 0x7fffffffLL || vocab >= 0x7fffffffLL ||
+    if (n_tokens <= 0 || vocab <= 0 || hidden <= 0 || n_tokens >= kMostTokens || vocab >= 0x7fffffffLL ||
         hidden > MRL_NORM_MAX_HIDDEN)
         return 0;
     return workspace_of(n_tokens, vocab, hidden).bytes;
@@ -689,6 +690,8 @@ extern "C" int mrl_embedding_bwd(const void* ids, int ids_dtype, int64_t n_token
                     mrl::aligned(workspace, 16),
                 MRL_ERR_MISALIGNED, "%s: misaligned buffer", fn);
     hipStream_t s = mrl::as_stream(stream);
+    MRL_REQUIRE(accumulate || vocab * hidden < (1LL << 34), MRL_ERR_UNSUPPORTED,
+                "%s: vocab=%lld hidden=%lld (a whole gradient of at most 2^34 - 1 entries)", fn, (long long)vocab, (long long)hidden);
     const int64_t fill_bytes = accumulate ? 0 : vocab * hidden * (int64_t)mrl::float_dtype_bytes(dtable_dtype);
     if (n_tokens == 0) {
         if (fill_bytes == 0) return MRL_OK;

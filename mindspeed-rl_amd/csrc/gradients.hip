@@ -25,6 +25,7 @@ constexpr int64_t kCached = 256 << 20;      // bytes that the memory-side cache 
 constexpr int chunk_bytes(int vecs) { return kBlock * vecs * 16; }  // of a tensor that a workgroup takes at a time
 constexpr int kMaxPartials = MRL_GRAD_NORM_PARTIALS;
 constexpr int kGroups = 2048;               // workgroups of a list: eight on each of 256 CUs
+constexpr int64_t kMostGroups = (1LL << 24) - 1;    // of a launch, which holds fewer than 2^32 threads
 
 struct Part {
     const void* data;
@@ -373,7 +374,7 @@ extern "C" int mrl_grad_clip(const mrl_grad* grads, int64_t n_grads, float max_n
     if (alone) hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(kBlock), 0, s, workspace, used, norm);
     int write_norm = alone ? 0 : 1;
     const auto launch = [&](const Table& t, auto kernel) {
-        const int64_t groups = t.in_place ? (t.n_chunks + each - 1) / each : t.n_chunks;
+        const int64_t groups = t.in_place ? (t.n_chunks + each - 1) / each : t.n_chunks < kMostGroups ? t.n_chunks : kMostGroups;
         hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(kBlock), 0, s, t, workspace, alone ? 0 : used, norm, max_norm,
                            write_norm);
         write_norm = 0;

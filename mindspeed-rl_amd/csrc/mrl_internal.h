@@ -124,6 +124,9 @@ inline int mask_dtype_bytes(int dt) {
     }
 }
 
+// A launch holds fewer than 2^32 threads in each dimension.
+inline bool launch_fits(int64_t groups, int64_t threads) { return groups * threads < (1LL << 32); }
+
 // Call right after a kernel launch: turns a rejected launch into MRL_ERR_LAUNCH.
 inline int check_launch(const char* what) {
     hipError_t e = hipGetLastError();

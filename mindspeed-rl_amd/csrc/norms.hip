@@ -589,15 +589,22 @@ void dispatch(int dtype, int wdtype, const BwdArgs& a) {
     else launch_bwd<MRL_F16, MRL_F16, kLayer>(a);
 }
 
+// Whether the launch that gives every row a team can hold them (the backward's stays within it).
+bool fwd_fits(int dtype, int64_t n_rows, int64_t hidden) {
+    const Team team = team_of(dtype, hidden);
+    const int64_t lanes = team.lanes > 0 ? team.lanes : kBlock, teams = lanes < 256 ? 256 / lanes : 1;
+    return n_rows <= 0x7fffffffLL && mrl::launch_fits((n_rows + teams - 1) / teams, lanes < 256 ? 256 : lanes);
+}
+
 int check_sizes(const char* fn, int dtype, int wdtype, int64_t n_rows, int64_t hidden) {
     MRL_REQUIRE(mrl::float_dtype_bytes(dtype) != 0, MRL_ERR_UNSUPPORTED, "%s: dtype %d (want F32, BF16 or F16)", fn, dtype);
     MRL_REQUIRE(wdtype == dtype || wdtype == MRL_F32, MRL_ERR_UNSUPPORTED, "%s: weight dtype %d (want the rows' or F32)", fn,
                 wdtype);
     MRL_REQUIRE(n_rows >= 0 && hidden >= 1, MRL_ERR_INVALID_ARG, "%s: n_rows=%lld hidden=%lld", fn, (long long)n_rows,
                 (long long)hidden);
-    MRL_REQUIRE(n_rows <= 0x7fffffffLL && hidden <= MRL_NORM_MAX_HIDDEN, MRL_ERR_UNSUPPORTED,
-                "%s: n_rows=%lld hidden=%lld (at most 2^31 - 1 and %d)", fn, (long long)n_rows, (long long)hidden,
-                MRL_NORM_MAX_HIDDEN);
+    MRL_REQUIRE(hidden <= MRL_NORM_MAX_HIDDEN && fwd_fits(dtype, n_rows, hidden), MRL_ERR_UNSUPPORTED,
+                "%s: n_rows=%lld hidden=%lld (hidden at most %d, and fewer rows: 2^32 threads hold at most one each)", fn,
+                (long long)n_rows, (long long)hidden, MRL_NORM_MAX_HIDDEN);
     return MRL_OK;
 }
 

@@ -9,6 +9,7 @@ import math
 
 import torch
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from .vocab_ops import _transformed
@@ -114,4 +115,6 @@ def token_embedding_grad(ids, grad, out, scale=1.0, vocab_start=0, accumulate=Fa
         raise ValueError("out is part of a graph: give its gradient or a detached tensor")
     scale, vocab_start = _check(ids, scale, vocab_start)
     dev = _lib.require_device(ids, grad, out)
-    return _add_up(_lib.index_column(ids, dev), grad.detach().contiguous(), scale, vocab_start, out, accumulate)
+    _add_up(_lib.index_column(ids, dev), grad.detach().contiguous(), scale, vocab_start, out, accumulate)
+    increment_version(out)
+    return out

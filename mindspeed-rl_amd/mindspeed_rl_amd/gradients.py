@@ -7,6 +7,7 @@ both from the training framework below it.  Here they work on the gradients that
 import array
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 
@@ -100,8 +101,9 @@ def clip_grad_norm_(grads, max_norm, out=None):
     if not max_norm >= 0.0:
         raise ValueError("max_norm must not be negative: %r" % max_norm)
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
-    words, back, tensors = [], [], []
+    words, back, tensors, written = [], [], [], []
     if out is None:
+        written = tensors
         for g in grads:
             if g is None:
                 continue
@@ -127,6 +129,7 @@ def clip_grad_norm_(grads, max_norm, out=None):
                 raise ValueError("an output must have the shape of its gradient, and its type or float32: %s %s and %s %s"
                                  % (tuple(g.shape), g.dtype, tuple(o.shape), o.dtype))
             tensors += (g, o)
+            written.append(o)
             p, q = g.data_ptr(), o.data_ptr()
             if not (g.is_contiguous() and o.is_contiguous()) and not (p == q and g.stride() == o.stride() and _fills(g)):
                 source, target = _spaced(g, o, False)
@@ -138,6 +141,7 @@ def clip_grad_norm_(grads, max_norm, out=None):
     norm, partial = _result(dev)
     _lib.call("mrl_grad_clip", table.buffer_info()[0], len(words) // 4, max_norm, norm.data_ptr(), partial.data_ptr(),
               _lib.stream(dev))
+    increment_version(written)              # autograd looks whether what it kept has been written to
     for o, target, *_ in back:
         if target is not o:
             o.detach().copy_(target)

@@ -100,7 +100,7 @@ def test_entry_points_refuse_and_launch_nothing():
         return lib.mrl_norm_fwd(x, dtype, rows, hidden, stride, w, b, wdtype, layer, eps, y, None, None, None)
 
     for rc, kw in [(-2, dict(dtype=_lib.I32)), (-2, dict(wdtype=_lib.BF16)), (-1, dict(rows=-1)), (-1, dict(hidden=0)),
-                   (-2, dict(hidden=most + 1, stride=most + 1)), (-2, dict(rows=1 << 31)), (-1, dict(stride=7)),
+                   (-2, dict(hidden=most + 1, stride=most + 1)), (-2, dict(rows=1 << 31)), (-2, dict(rows=(1 << 28), hidden=8)), (-1, dict(stride=7)),
                    (-1, dict(eps=0.0)), (-1, dict(eps=float("nan"))), (-1, dict(b=p, layer=0)), (-1, dict(x=None)),
                    (-1, dict(w=None)), (-1, dict(y=None)), (-3, dict(x=p + 2)), (-3, dict(y=p + 1)), (0, dict(rows=0, x=None))]:
         assert fwd(**kw) == rc, kw
@@ -283,6 +283,49 @@ def test_gradient_against_differences(dev, kind):
         slope = (ends[0] - ends[1]) / 2e-4
         got = (grads[k].double() * v).sum()
         assert abs(got - slope) <= (bounds[name][1] * v.abs()).sum() + 1e-6 * (grads[k].double() * v).abs().sum()
+
+
+@pytest.mark.gpu
+def test_differentiated_once(dev):
+    """Under create_graph the first gradient is the usual one and a second differentiation is refused; a vector alone;
+    rows overwritten before the backward are noticed."""
+    x, w, b, dy = make(dev, (6, 40), torch.float32, torch.float32, 12)
+    xl = x.clone().requires_grad_()
+    (plain,) = torch.autograd.grad(mrl.layer_norm(xl, w, b), [xl], dy)
+    up = dy.clone().requires_grad_()
+    (dx,) = torch.autograd.grad(mrl.layer_norm(xl, w, b), [xl], up, create_graph=True)
+    assert torch.equal(dx, plain)
+    with pytest.raises(RuntimeError):
+        dx.sum().backward()
+    assert torch.equal(mrl.rms_norm(x[2], w), mrl.rms_norm(x, w)[2])
+    h = xl * 2
+    y = mrl.rms_norm(h, w)
+    h.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once(dev):
+    """Steps that overlap in time, each with its own memory: the bits of a step alone."""
+    sets = [make(dev, (3000, 1024), torch.bfloat16, torch.bfloat16, 30 + k) for k in range(2)]
+
+    def step(x, w, b, dy):
+        ts = [t.detach().requires_grad_() for t in (x, w, b)]
+        y = mrl.layer_norm(*ts)
+        return (y.detach(), *torch.autograd.grad(y, ts, dy))
+
+    want = [step(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(5):
+        for k in range(2):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(step(*sets[k]))
+    torch.cuda.synchronize()
+    for k in range(2):
+        assert all(torch.equal(p, q) for g in got[k] for p, q in zip(g, want[k]))
 
 
 @pytest.mark.gpu

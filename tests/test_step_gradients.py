@@ -180,6 +180,13 @@ def test_strides(dev):
     with pytest.raises(_lib.MrlError):
         mrl.clip_grad_norm_([base.view(-1)[:2000]], 1.0, out=[base.view(-1)[700:2700]])
     check_norm(mrl.global_grad_norm([one, one]), [one, one])
+    # what is written counts as written to: autograd refuses a backward that kept it
+    leaf = torch.ones(5, device=dev, requires_grad=True)
+    kept = leaf * 2
+    y = kept.square().sum()
+    mrl.clip_grad_norm_([kept.detach()], 1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
 
 
 @pytest.mark.gpu

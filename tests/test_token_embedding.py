@@ -90,7 +90,7 @@ def test_entry_points_refuse_and_launch_nothing():
         return lib.mrl_embedding_fwd(ids, it, n, start, table, dtype, vocab, hidden, scale, out, None)
 
     for rc, kw in [(-2, dict(it=_lib.F32)), (-2, dict(dtype=_lib.I32)), (-1, dict(n=-1)), (-1, dict(start=-1)), (-1, dict(vocab=0)),
-                   (-1, dict(hidden=0)), (-2, dict(vocab=(1 << 31) - 1)), (-2, dict(n=1 << 31)), (-2, dict(hidden=(1 << 20) + 1)),
+                   (-1, dict(hidden=0)), (-2, dict(vocab=(1 << 31) - 1)), (-2, dict(n=1 << 26)), (-2, dict(hidden=(1 << 20) + 1)),
                    (-1, dict(scale=float("inf"))), (-1, dict(ids=None)), (-1, dict(table=None)), (-1, dict(out=None)),
                    (-3, dict(ids=p + 4)), (-3, dict(table=p + 2)), (-3, dict(out=p + 2)), (0, dict(n=0, ids=None))]:
         assert fwd(**kw) == rc, kw
@@ -101,7 +101,8 @@ def test_entry_points_refuse_and_launch_nothing():
             size=need):
         return lib.mrl_embedding_bwd(ids, it, n, start, dy, dtype, vocab, hidden, scale, out, ot, 0, ws, size, None)
 
-    for rc, kw in [(-2, dict(it=_lib.U8)), (-2, dict(dtype=_lib.F64)), (-2, dict(ot=_lib.F16)), (-1, dict(n=-1)),
+    for rc, kw in [(-2, dict(it=_lib.U8)), (-2, dict(dtype=_lib.F64)), (-2, dict(ot=_lib.F16)), (-1, dict(n=-1)), (-2, dict(n=1 << 26)),
+                   (-2, dict(vocab=1 << 30, hidden=16, size=1 << 40)),
                    (-1, dict(vocab=0)), (-1, dict(dy=None)), (-1, dict(out=None)), (-1, dict(ws=None)), (-1, dict(size=need - 1)),
                    (-3, dict(ws=p + 8)), (-3, dict(dy=p + 1)), (-3, dict(out=p + 2)), (-1, dict(scale=float("nan")))]:
         assert bwd(**kw) == rc, kw
@@ -261,6 +262,45 @@ def test_gradient_against_differences(dev):
     _, bound, _ = plain_grad(ids, dy, 30, 0.7, 0, torch.float32)
     # the scale itself is rounded to fp32: half a step of every product
     assert abs((dw.double() * v).sum() - slope) <= (bound * v.abs()).sum() * 1.01 + U * (dw.double() * v).abs().sum() + 1e-12
+
+
+@pytest.mark.gpu
+def test_differentiated_once_and_written_in_place(dev):
+    """A second differentiation is refused; a gradient that is added to counts as written to."""
+    w = torch.randn(9, 12, device=dev).requires_grad_()
+    ids = torch.tensor([3, 3, 0], device=dev)
+    dy = torch.randn(3, 12, device=dev).requires_grad_()
+    (dw,) = torch.autograd.grad(mrl.token_embedding(ids, w), [w], dy, create_graph=True)
+    assert torch.equal(dw[3], dy[0] + dy[1])
+    with pytest.raises(RuntimeError):
+        dw.sum().backward()
+    out = torch.zeros(9, 12, device=dev)
+    before = out._version
+    mrl.token_embedding_grad(ids, dy.detach(), out, accumulate=True)
+    assert out._version > before
+    with torch.inference_mode():
+        assert torch.equal(mrl.token_embedding(ids, w), w[ids])
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once(dev):
+    """Gradients that overlap in time, each with its own workspace: the bits of one alone."""
+    g = torch.Generator(device=dev).manual_seed(11)
+    sets = [(torch.randint(-9, 3000, (9000,), generator=g, device=dev), torch.randn(9000, 256, generator=g, device=dev)) for _ in range(2)]
+
+    def step(ids, dy):
+        return mrl.token_embedding_grad(ids, dy, torch.empty(3000, 256, device=dev))
+
+    want = [step(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(5):
+        for k in range(2):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(step(*sets[k]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, want[k]) for k in range(2) for p in got[k])
 
 
 @pytest.mark.gpu
