@@ -266,6 +266,7 @@ __global__ __launch_bounds__(1024) void norm_fwd_rows_kernel(const typename Elem
 // row would wait for that as well.
 constexpr int kBwdBlock = 512;              // threads of a workgroup that holds several teams
 constexpr int kBwdGroups = 512;             // most workgroups: two on each of 256 CUs
+constexpr int64_t kBwdManyVecs = 4 << 20;   // 64 MiB of rows
 constexpr int kBwdFewTurns = 4;             // that one workgroup takes alone: the second launch costs more
 
 template <int DT, int WDT, bool kLayer, int kVecs, int kBlockMost, bool kStream>
@@ -276,6 +277,7 @@ __global__ __launch_bounds__(kBlockMost) void norm_bwd_rows_kernel(
     typename Elem<WDT>::T* __restrict__ dweight, typename Elem<WDT>::T* __restrict__ dbias) {
     constexpr int kVec = Elem<DT>::kVec, kWVec = Elem<WDT>::kVec;
     constexpr bool kOne = kBlockMost > kBwdBlock;       // the team is the workgroup
+    constexpr bool kAhead = kVecs == 1;                 // the next row is requested before this one is summed
     extern __shared__ float columns[];                  // [kVecs * kVec][lanes] sums on their way between teams
     __shared__ float2 lds[2][16];
     const int teams = kOne ? 1 : blockDim.x / lanes, team = kOne ? 0 : threadIdx.x / lanes;
@@ -311,12 +313,13 @@ __global__ __launch_bounds__(kBlockMost) void norm_bwd_rows_kernel(
             gn[q] = kStream ? mrl::Vec<DT>::load_nt(dyr + col.at(q)) : mrl::Vec<DT>::load(dyr + col.at(q));
         }
     };
-    request((int64_t)blockIdx.x * teams + team);
+    if (kAhead) request((int64_t)blockIdx.x * teams + team);
     int turn = 0;
     for (int64_t base = (int64_t)blockIdx.x * teams; base < n_rows; base += step, turn ^= 1) {
         // teams behind the last row do that row again, without its share of the columns' sums
         const bool counts = kOne || base + team < n_rows;
         const int64_t row = counts ? base + team : n_rows - 1;
+        if (!kAhead) request(row);
         u32x4 xv[kVecs], gv[kVecs];
 #pragma unroll
         for (int q = 0; q < kVecs; ++q) {
@@ -324,7 +327,7 @@ __global__ __launch_bounds__(kBlockMost) void norm_bwd_rows_kernel(
             gv[q] = gn[q];
         }
         const float mu = mun, r = rn;
-        request(base + team + step);
+        if (kAhead) request(base + team + step);
         float sg = 0.f, sgn = 0.f;
 #pragma unroll
         for (int q = 0; q < kVecs; ++q) {
@@ -446,13 +449,16 @@ int64_t slab_rows_of(int64_t n_rows) {
     return rows < 16 ? 16 : rows;
 }
 
-// The backward's teams are larger, with one or two vectors a lane (four in rows of more than 2 048 vectors): it holds twice
-// the entries, and the sums of the columns besides.
-Team bwd_team_of(int dtype, int64_t hidden) {
+// The backward's teams hold twice the entries, and the sums of the columns besides: one or two vectors a lane (four in rows of
+// more than 2 048 vectors).  Two, where the next row is not requested ahead, are better served by the memory (us, one / two:
+// 32 768 x 3 584 bf16 140 / 122, 65 536 x 5 120 371 / 337, 65 536 x 2 048 143 / 133); of little data, where what follows the
+// rows counts, one (9 477 x 1 343 fp16 23 / 26, 2 500 x 1 024 fp32 13 / 14).
+Team bwd_team_of(int dtype, int64_t n_rows, int64_t hidden) {
     const int64_t nv = vectors_of(dtype, hidden);
     if (nv == 0) return {0, 0};
     if (nv <= 32) return team_that_fits(nv, 16, (int)((nv + 15) / 16));
-    for (int vecs = 1; vecs <= 4; vecs *= 2) {
+    const bool two = nv > 256 || (nv > 128 && n_rows * nv >= kBwdManyVecs);
+    for (int vecs = two ? 2 : 1; vecs <= 4; vecs *= 2) {
         const int64_t waves = (nv + 64 * vecs - 1) / (64 * vecs);
         if (waves <= 16) return team_that_fits(nv, waves * 64, vecs);
     }
@@ -528,7 +534,7 @@ template <int DT, int WDT, bool kLayer>
 void launch_bwd(const BwdArgs& a) {
     using T = typename Elem<DT>::T;
     using W = typename Elem<WDT>::T;
-    const Team team = bwd_team_of(DT, a.hidden);
+    const Team team = bwd_team_of(DT, a.n_rows, a.hidden);
     if (team.lanes > 0 && a.n_rows > 0 && a.dx) {
         const bool sums = a.dweight || a.dbias;
         const int groups = bwd_groups(team, a.n_rows);

@@ -173,6 +173,23 @@ def test_forward_and_backward(dev, shape, dtype, wdtype, kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind,dtype,rows,hidden", [("layer", torch.bfloat16, 26001, 1343), ("rms", torch.float32, 30000, 616),
+                                                    ("rms", torch.float16, 33000, 1032)])
+def test_much_data(dev, kind, dtype, rows, hidden):
+    """Rows of 64 MiB and more, whose backward deals them out differently."""
+    x, w, b, dy = make(dev, (rows, hidden), dtype, dtype, 13, kind == "layer")
+    want = formula(x, w, b, 1e-5, kind == "layer", dy)
+    leaves = [t.requires_grad_() for t in (x, w, b) if t is not None]
+    y = apply(kind, x, w, b, 1e-5)
+    grads = torch.autograd.grad(y, leaves, dy)
+    within(y.detach(), want["y"])
+    for name, g in zip(("dx", "dw", "db"), grads):
+        within(g, want[name])
+    again = torch.autograd.grad(apply(kind, x, w, b, 1e-5), leaves, dy)
+    assert all(torch.equal(p, q) for p, q in zip(again, grads))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["layer", "rms"])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
 def test_strides_and_places(dev, dtype, kind):
