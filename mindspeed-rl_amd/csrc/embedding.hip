@@ -384,39 +384,45 @@ __global__ __launch_bounds__(kSumBlock) void sum_kernel(Sums s, const int32_t* _
     };
     int32_t kn[kSumRows];
     u32x4 vn[kSumRows];
-    const auto request = [&](int64_t p) {
+    for (int64_t block = begin; block < end; block += 64) {
+        // the list's next 64 tokens, one in each lane: what a row waits for is then its own load alone
+        const int lane = threadIdx.x & 63, n = end - block < 64 ? (int)(end - block) : 64;
+        const int64_t mine = block + (lane < n ? lane : n - 1);
+        const int32_t lane_key = keys[mine], lane_token = tokens[mine];
+        const auto request = [&](int p) {
 #pragma unroll
-        for (int i = 0; i < kSumRows; ++i) {
-            const int64_t at = p + i < end ? p + i : end - 1;
-            kn[i] = keys[at];
-            vn[i] = mrl::Vec<DT>::load_nt(dy + (int64_t)tokens[at] * s.hidden + col);
-        }
-    };
-    request(begin);
-    for (int64_t p = begin; p < end; p += kSumRows) {
-        int32_t k[kSumRows];
-        u32x4 v[kSumRows];
-#pragma unroll
-        for (int i = 0; i < kSumRows; ++i) {
-            k[i] = kn[i];
-            v[i] = vn[i];
-        }
-        request(p + kSumRows);
-#pragma unroll
-        for (int i = 0; i < kSumRows; ++i) {
-            if (p + i >= end) break;
-            if (k[i] != key) {
-                finish(false);
-                key = k[i];
-                if (key >= s.vocab) return;
-                from_front = false;
-#pragma unroll
-                for (int c = 0; c < kVec; ++c) acc[c] = 0.f;
+            for (int i = 0; i < kSumRows; ++i) {
+                const int at = p + i < n ? p + i : n - 1;
+                kn[i] = __builtin_amdgcn_readlane(lane_key, at);
+                vn[i] = mrl::Vec<DT>::load_nt(dy + (int64_t)__builtin_amdgcn_readlane(lane_token, at) * s.hidden + col);
             }
-            float z[kVec];
-            Elem<DT>::unpack(v[i], z);
+        };
+        request(0);
+        for (int p = 0; p < n; p += kSumRows) {
+            int32_t k[kSumRows];
+            u32x4 v[kSumRows];
 #pragma unroll
-            for (int c = 0; c < kVec; ++c) acc[c] += z[c];
+            for (int i = 0; i < kSumRows; ++i) {
+                k[i] = kn[i];
+                v[i] = vn[i];
+            }
+            request(p + kSumRows);
+#pragma unroll
+            for (int i = 0; i < kSumRows; ++i) {
+                if (p + i >= n) break;
+                if (k[i] != key) {
+                    finish(false);
+                    key = k[i];
+                    if (key >= s.vocab) return;
+                    from_front = false;
+#pragma unroll
+                    for (int c = 0; c < kVec; ++c) acc[c] = 0.f;
+                }
+                float z[kVec];
+                Elem<DT>::unpack(v[i], z);
+#pragma unroll
+                for (int c = 0; c < kVec; ++c) acc[c] += z[c];
+            }
         }
     }
     finish(next == key);
