@@ -215,6 +215,26 @@ def test_strides_and_places(dev, dtype, kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_narrow_wide_and_frozen_rows(dev, dtype, kind):
+    """Rows of less than a vector, many of them; rows that no team holds, apart from one another; the vectors' gradients alone."""
+    for rows, h in ((3001, 3), (700, 7), (21, 20011), (40, 16396)):
+        x, w, b, dy = make(dev, (rows, h), dtype, dtype, 7, kind == "layer")
+        wide = torch.full((rows, h + 3), float("nan"), dtype=dtype, device=dev)
+        wide[:, 1:1 + h] = x
+        want = formula(x, w, b, 1e-5, kind == "layer", dy)
+        leaves = [wide[:, 1:1 + h].detach().requires_grad_()] + [t.requires_grad_() for t in (w, b) if t is not None]
+        y = apply(kind, leaves[0], w, b, 1e-5)
+        within(y.detach(), want["y"])
+        for name, g in zip(("dx", "dw", "db"), torch.autograd.grad(y, leaves, dy)):
+            within(g, want[name])
+        y = apply(kind, x, w, b, 1e-5)
+        for name, g in zip(("dw", "db"), torch.autograd.grad(y, leaves[1:], dy)):
+            within(g, want[name])
+
+
+@pytest.mark.gpu
 def test_asked_gradients_and_broadcast_upstream(dev):
     """Only what is asked for is computed; an upstream gradient of one value; a vector shared by two norms."""
     x, w, b, _ = make(dev, (40, 136), torch.float32, torch.float32, 3)
