@@ -710,7 +710,7 @@ int mrl_critic_loss_bwd_slope(const float* slope, int64_t batch, int64_t padded_
  * (mu = 0, bias NULL).  x: F32, BF16 or F16 with a row stride in elements, only read; y: the same type,
  * dense; weight and bias: the rows' type or F32.  mean and rstd [n_rows] fp32, nullable, are what
  * the backward takes.  A row with an infinity or NaN gives NaN in that row alone; squares of a row have to
- * stay in fp32.  hidden at most MRL_NORM_MAX_HIDDEN; rows as many as 2^32 threads hold, 16 to 1 024 for a row. */
+ * stay in fp32.  hidden at most MRL_NORM_MAX_HIDDEN; rows as many as 2^32 threads hold, 1 to 1 024 for a row. */
 #define MRL_NORM_MAX_HIDDEN 1048576
 int mrl_norm_fwd(const void* x, int dtype, int64_t n_rows, int64_t hidden, int64_t row_stride,
                  const void* weight, const void* bias, int weight_dtype, int subtract_mean, float eps,
@@ -739,7 +739,7 @@ int mrl_embedding_fwd(const void* ids, int ids_dtype, int64_t n_tokens, int64_t 
  * rounded once; accumulate != 0: added to what dtable holds, and rows that no token names are not touched.
  * dy [n_tokens, hidden] dense; dtable [vocab, hidden] of dy's type or F32.  Tokens are sorted by row and summed in
  * that order: the same call gives the same bits.  workspace: 16-byte aligned, no clearing needed.  dtable shares no
- * memory with anything else; fewer than 2^26 tokens, and without accumulate fewer than 2^34 entries of dtable. */
+ * memory with anything else; fewer than 2^26 tokens, and without accumulate a dtable of fewer than 2^36 - 2^21 bytes. */
 int64_t mrl_embedding_bwd_workspace_bytes(int64_t n_tokens, int64_t vocab, int64_t hidden);
 int mrl_embedding_bwd(const void* ids, int ids_dtype, int64_t n_tokens, int64_t vocab_start, const void* dy,
                       int dtype, int64_t vocab, int64_t hidden, float scale, void* dtable, int dtable_dtype,

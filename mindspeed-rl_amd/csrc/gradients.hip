@@ -5,6 +5,9 @@
 // Squares and their sums are held in 64 bits: no gradient that fp32 or bf16 holds overflows them, and the order of the sum
 // does not show in the norm's fp32 bits but for a tie.  The list travels in the kernel's arguments, so a captured graph
 // holds it, and nothing is copied to the device.
+//
+// Bound by memory.  1.4 GB: the norm 214 us (6.5 TB/s), clipped into other tensors 669 us (4.2 GB: 6.3 TB/s), bf16 into fp32
+// 892, in place 762; where the norm is within the bound nothing is written (207).  200 MB: 35, 93, 122, 99 us.
 #include <algorithm>
 
 #include "lane_ops.h"
@@ -19,7 +22,7 @@ using mrl_vocab::Elem;
 constexpr int kBlock = 256;
 constexpr int kTable = 112;                 // tensors of a launch: 4 KB of arguments
 constexpr int kSumVecs = 4;                 // vectors of 16 bytes that a thread has on its way where squares are summed
-constexpr int kScaleVecs = 1;               // ... and where gradients are scaled
+constexpr int kScaleVecs = 1;               // ... and where gradients are scaled: 1.4 GB of bf16 into fp32 892 us, by four 988
 constexpr int64_t kCached = 256 << 20;      // bytes that the memory-side cache holds
 
 constexpr int chunk_bytes(int vecs) { return kBlock * vecs * 16; }  // of a tensor that a workgroup takes at a time
@@ -213,8 +216,7 @@ __device__ __forceinline__ void widen_chunk(const Table& t, const Place& c, floa
 
 // The norm comes from the partial sums, formed by every workgroup for itself, or from where a launch in front left it
 // (n_partial == 0); the factor in fp32, as a caller would form it from the norm that is handed out (NaN, of a norm that
-// is none, stays NaN).  Chunks are taken from the last to the first: of a list larger than the memory-side cache the last
-// ones are still there.
+// is none, stays NaN).
 template <int DT, int OT>
 __global__ __launch_bounds__(kBlock, 8) void grad_scale_kernel(Table t, const double* __restrict__ partial, int n_partial,
                                                                float* norm, float max_norm, int write_norm) {
@@ -225,7 +227,7 @@ __global__ __launch_bounds__(kBlock, 8) void grad_scale_kernel(Table t, const do
     const float quotient = max_norm / (total + 1e-6f), f = quotient > 1.f ? 1.f : quotient;
     if (f == 1.f && t.in_place) return;
     load_ends(t, ends);
-    for (int c = t.n_chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {
+    for (int c = blockIdx.x; c < t.n_chunks; c += gridDim.x) {
         const Place at = place_of<DT, kScaleVecs>(t, ends, c);
         if constexpr (DT == OT) scale_chunk<DT>(t, at, f);
         else widen_chunk<DT>(t, at, f);
@@ -320,7 +322,8 @@ int64_t chunks_each(const mrl_grad* grads, int64_t n, int vecs) {
 }
 
 // Squares of all tensors into the workspace; the number of partial sums.  A list that is read again and that the
-// memory-side cache holds is left there, anything else goes past it.
+// memory-side cache holds is left there, anything else goes past it (us, left / past: clipping 200 MB 93 / 104; the norm of
+// 1.4 GB 241 / 214).
 int launch_squares(const mrl_grad* grads, int64_t n, bool read_again, double* partial, hipStream_t s) {
     const int64_t each = chunks_each(grads, n, kSumVecs);
     int64_t bytes = 0;
@@ -369,7 +372,8 @@ extern "C" int mrl_grad_clip(const mrl_grad* grads, int64_t n_grads, float max_n
     const int used = launch_squares(grads, n_grads, true, workspace, s);
     const int64_t each = chunks_each(grads, n_grads, kScaleVecs);
     // Lists of more chunks than workgroups fit: those that go elsewhere take a workgroup a chunk, which the memory serves
-    // best, and a launch in front forms the norm for them; in place the workgroups stay, for there may be nothing to do.
+    // best (1.4 GB 669 us; by workgroups that stay 740), and a launch in front forms the norm for them; in place the workgroups
+    // stay, for there may be nothing to do.  Of shorter lists every workgroup forms it (1 MB 7.4 us; with the launch 8.7).
     const bool alone = used == 0 || each > 1;
     if (alone) hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(kBlock), 0, s, workspace, used, norm);
     int write_norm = alone ? 0 : 1;

@@ -102,7 +102,7 @@ def test_entry_points_refuse_and_launch_nothing():
         return lib.mrl_embedding_bwd(ids, it, n, start, dy, dtype, vocab, hidden, scale, out, ot, 0, ws, size, None)
 
     for rc, kw in [(-2, dict(it=_lib.U8)), (-2, dict(dtype=_lib.F64)), (-2, dict(ot=_lib.F16)), (-1, dict(n=-1)), (-2, dict(n=1 << 26)),
-                   (-2, dict(vocab=1 << 30, hidden=16, size=1 << 40)),
+                   (-2, dict(vocab=1 << 30, hidden=16, size=1 << 40)), (-2, dict(vocab=(1 << 30) - 1, hidden=16, size=1 << 40)),
                    (-1, dict(vocab=0)), (-1, dict(dy=None)), (-1, dict(out=None)), (-1, dict(ws=None)), (-1, dict(size=need - 1)),
                    (-3, dict(ws=p + 8)), (-3, dict(dy=p + 1)), (-3, dict(out=p + 2)), (-1, dict(scale=float("nan")))]:
         assert bwd(**kw) == rc, kw
