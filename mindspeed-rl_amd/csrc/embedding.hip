@@ -433,7 +433,7 @@ __global__ __launch_bounds__(kSumBlock) void sum_kernel(Sums s, const int32_t* _
 }
 
 constexpr int kJoinWaves = 8;
-constexpr int kJoinShares = 16;             // shares of a workgroup, a lane each
+constexpr int kJoinShares = 2 * kJoinWaves; // shares of a workgroup for short runs
 constexpr int kJoinShort = 16;              // shares of a run that a wavefront joins alone
 constexpr int kJoinAhead = 16;              // parts that a wavefront has on its way
 static_assert(kShares <= 64 * 64, "two steps find where a run ends");
@@ -454,89 +454,113 @@ struct Few {
     }
 };
 
-// The runs that cross shares.  A workgroup takes a tile of columns and every gridDim.y-th share, a lane for each at first:
-// does such a run begin there, and in how many shares does it go on.  Short runs are joined by a wavefront each, long ones by
-// all of them, each taking every kJoinWaves-th part.  The size above: 14 us.
-template <int GT, bool kAdd, int kCols>
-__global__ __launch_bounds__(kJoinWaves * 64) void join_kernel(Sums s, const int32_t* __restrict__ keys,
-                                                               typename Elem<GT>::T* __restrict__ dtable) {
-    __shared__ float lds[kJoinWaves][64 * kCols];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    // a row that is not whole lanes ends with one that overlaps the one in front of it
-    const int64_t want = ((int64_t)blockIdx.x * 64 + lane) * kCols, col = want < s.hidden - kCols ? want : s.hidden - kCols;
-    const int skip = want >= s.hidden ? kCols : (int)(want - col);
-    // whether the run of `key` goes on in share g
-    const auto goes_on = [&](int64_t g, int32_t key) {
-        const int64_t first = g * s.share;
-        return first < s.n_tokens && keys[first < s.n_tokens ? first : 0] == key;
-    };
-    const int64_t mine = blockIdx.y + (int64_t)lane * gridDim.y, mine_end = (mine + 1) * s.share;
-    int32_t my_key = s.vocab;
-    int more = 0;                                                   // shares behind this one, kJoinShort: as many or more
-    if (mine_end < s.n_tokens) {
-        my_key = keys[mine_end - 1];
-        if (my_key < s.vocab && (mine == 0 || keys[mine * s.share - 1] != my_key)) {
-            bool in = true;
-#pragma unroll
-            for (int i = 0; i < kJoinShort; ++i) {
-                in = in && goes_on(mine + 1 + i, my_key);
-                more += in ? 1 : 0;
-            }
-        }
+// Runs that cross shares.
+struct Runs {
+    const int32_t* keys;
+    int64_t n_tokens, share;
+    int32_t vocab;
+
+    // whether the run of `key`, which is in a share in front of share g, goes on there
+    __device__ __forceinline__ bool goes_on(int64_t g, int32_t key) const {
+        const int64_t first = g * share;
+        const int32_t k = keys[first < n_tokens ? first : 0];
+        return (first < n_tokens) & (k == key);
     }
-    const auto put = [&](int32_t key, const Few<kCols>& sum) {
+    // whether a run that begins in share g goes on in share g + n
+    __device__ __forceinline__ bool begins(int64_t g, int n, int32_t* key) const {
+        const bool last = (g + 1) * share >= n_tokens;
+        const int32_t k = keys[last ? 0 : (g + 1) * share - 1], front = keys[g > 0 && !last ? g * share - 1 : 0];
+        *key = k;
+        return !last & (k < vocab) & (g == 0 || front != k) & goes_on(g + n, k);
+    }
+};
+
+// A lane's columns of a row; a row that is not whole lanes ends with one that overlaps the one in front of it.
+template <int GT, bool kAdd, int kCols>
+struct JoinedColumns {
+    const Sums& s;
+    typename Elem<GT>::T* dtable;
+    int64_t col;
+    int skip;
+
+    __device__ __forceinline__ JoinedColumns(const Sums& s, typename Elem<GT>::T* dtable, int64_t tile) : s(s), dtable(dtable) {
+        const int64_t want = (tile * 64 + (threadIdx.x & 63)) * kCols;
+        col = want < s.hidden - kCols ? want : s.hidden - kCols;
+        skip = want >= s.hidden ? kCols : (int)(want - col);
+    }
+    __device__ __forceinline__ Few<kCols> part(int64_t share, int slot) const {
+        return Few<kCols>::load(s.part + (share * 2 + slot) * s.hidden + col);
+    }
+    __device__ __forceinline__ void put(int32_t key, const Few<kCols>& sum) const {
         typename Elem<GT>::T* at = dtable + key * s.hidden + col;
 #pragma unroll
         for (int i = 0; i < kCols; ++i)
             if (i >= skip) Elem<GT>::store(at + i, kAdd ? Elem<GT>::load(at + i) + sum.v[i] * s.scale : sum.v[i] * s.scale);
-    };
-    const auto part = [&](int64_t share, int slot) { return Few<kCols>::load(s.part + (share * 2 + slot) * s.hidden + col); };
-    int nth = 0;
-    for (uint64_t todo = __ballot(more > 0 && more < kJoinShort); todo != 0; todo &= todo - 1, ++nth) {
-        if (nth % kJoinWaves != wave) continue;
-        const int from = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)todo) - 1);
-        const int64_t share = blockIdx.y + (int64_t)from * gridDim.y;
-        const int n = __shfl(more, from, 64);
-        Few<kCols> sum = part(share, 1);
+    }
+};
+
+// Long runs by workgroups of a tile of 64 columns and 64 shares, whose wavefronts take every kJoinWaves-th part; short ones by
+// a wavefront each of workgroups of 64 kCols columns and kJoinShares shares.
+template <int GT, bool kAdd, int kCols>
+__global__ __launch_bounds__(kJoinWaves * 64) void join_kernel(Sums s, const int32_t* __restrict__ keys, int long_tiles,
+                                                               int64_t long_groups, int tiles,
+                                                               typename Elem<GT>::T* __restrict__ dtable) {
+    __shared__ float lds[kJoinWaves][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const Runs runs = {keys, s.n_tokens, s.share, s.vocab};
+    int32_t my_key;
+    if (blockIdx.x < long_groups) {
+        const JoinedColumns<GT, kAdd, 1> row(s, dtable, blockIdx.x % long_tiles);
+        const int64_t base = (int64_t)(blockIdx.x / long_tiles) * 64;
+        for (uint64_t todo = __ballot(runs.begins(base + lane, kJoinShort, &my_key)); todo != 0; todo &= todo - 1) {   // the same in every wavefront
+            const int from = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)todo) - 1);
+            const int64_t share = base + from;
+            const int32_t key = __shfl(my_key, from, 64);
+            // the last share that it goes on in: in steps of 64 shares (64 of them are more than kShares), then one by one
+            int64_t last = share + kJoinShort;
+            last += 64 * __popcll(__ballot(runs.goes_on(last + 64 * (lane + 1), key)));
+            last += __popcll(__ballot(runs.goes_on(last + 1 + lane, key)));
+            Few<1> sum = {};
+            for (int64_t g = share + wave; g <= last; g += kJoinWaves * kJoinAhead) {
+                Few<1> v[kJoinAhead];
+#pragma unroll
+                for (int i = 0; i < kJoinAhead; ++i) {
+                    const int64_t p = g + i * kJoinWaves <= last ? g + i * kJoinWaves : last;
+                    v[i] = row.part(p, p == share ? 1 : 0);
+                }
+#pragma unroll
+                for (int i = 0; i < kJoinAhead; ++i) sum.add(v[i], g + i * kJoinWaves <= last);
+            }
+            lds[wave][lane] = sum.v[0];
+            __syncthreads();
+            if (wave == 0) {
+#pragma unroll
+                for (int w = 1; w < kJoinWaves; ++w) sum.v[0] += lds[w][lane];
+                row.put(key, sum);
+            }
+            __syncthreads();
+        }
+        return;
+    }
+    const int64_t group = blockIdx.x - long_groups;
+    const JoinedColumns<GT, kAdd, kCols> row(s, dtable, group % tiles);
+    // half a wavefront a share, a lane for each share that its run may go on in
+    const int64_t base = group / tiles * kJoinShares + wave * 2;
+    const int ahead = (lane & 31) + 1;
+    const uint64_t on = __ballot(runs.begins(base + (lane >> 5), ahead, &my_key) & (ahead <= kJoinShort));
+    for (int h = 0; h < 2; ++h) {
+        const int n = __popc((uint32_t)(on >> (32 * h)));           // sorted: none of them but the first ones
+        if (n == 0 || n == kJoinShort) continue;
+        const int64_t share = base + h;
+        Few<kCols> sum = row.part(share, 1);
         for (int i0 = 1; i0 <= n; i0 += 5) {
             Few<kCols> v[5];
 #pragma unroll
-            for (int i = 0; i < 5; ++i) v[i] = part(share + (i0 + i <= n ? i0 + i : n), 0);
+            for (int i = 0; i < 5; ++i) v[i] = row.part(share + (i0 + i <= n ? i0 + i : n), 0);
 #pragma unroll
             for (int i = 0; i < 5; ++i) sum.add(v[i], i0 + i <= n);
         }
-        put(__shfl(my_key, from, 64), sum);
-    }
-    for (uint64_t todo = __ballot(more == kJoinShort); todo != 0; todo &= todo - 1) {       // the same in every wavefront
-        const int from = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)todo) - 1);
-        const int64_t share = blockIdx.y + (int64_t)from * gridDim.y;
-        const int32_t key = __shfl(my_key, from, 64);
-        // the last share that it goes on in: in steps of 64 shares (64 of them are more than kShares), then one by one
-        int64_t last = share + kJoinShort;
-        last += 64 * __popcll(__ballot(goes_on(last + 64 * (lane + 1), key)));
-        last += __popcll(__ballot(goes_on(last + 1 + lane, key)));
-        Few<kCols> sum = {};
-        for (int64_t g = share + wave; g <= last; g += kJoinWaves * kJoinAhead) {
-            Few<kCols> v[kJoinAhead];
-#pragma unroll
-            for (int i = 0; i < kJoinAhead; ++i) {
-                const int64_t p = g + i * kJoinWaves <= last ? g + i * kJoinWaves : last;
-                v[i] = part(p, p == share ? 1 : 0);
-            }
-#pragma unroll
-            for (int i = 0; i < kJoinAhead; ++i) sum.add(v[i], g + i * kJoinWaves <= last);
-        }
-#pragma unroll
-        for (int i = 0; i < kCols; ++i) lds[wave][i * 64 + lane] = sum.v[i];
-        __syncthreads();
-        if (wave == 0) {
-#pragma unroll
-            for (int w = 1; w < kJoinWaves; ++w)
-#pragma unroll
-                for (int i = 0; i < kCols; ++i) sum.v[i] += lds[w][i * 64 + lane];
-            put(key, sum);
-        }
-        __syncthreads();
+        row.put(__builtin_amdgcn_readlane(my_key, 32 * h), sum);
     }
 }
 
@@ -611,9 +635,12 @@ void launch_sums(const Sums& s, const int32_t* keys, const int32_t* tokens, cons
     if (shares <= 1) return;
     const auto join = [&](auto cols) {
         constexpr int kCols = decltype(cols)::value;
-        const int64_t tiles = (s.hidden + 64 * kCols - 1) / (64 * kCols);
-        hipLaunchKernelGGL((join_kernel<GT, kAdd, kCols>), dim3((unsigned)tiles, (unsigned)((shares + kJoinShares - 1) / kJoinShares)),
-                           dim3(kJoinWaves * 64), 0, stream, s, keys, (G*)dtable);
+        const int64_t tiles = (s.hidden + 64 * kCols - 1) / (64 * kCols), long_tiles = (s.hidden + 63) / 64;
+        // runs of more shares than kJoinShort take as many, and one
+        const int64_t long_groups = shares > kJoinShort ? long_tiles * ((shares + 63) / 64) : 0;
+        const int64_t groups = long_groups + tiles * ((shares + kJoinShares - 1) / kJoinShares);
+        hipLaunchKernelGGL((join_kernel<GT, kAdd, kCols>), dim3((unsigned)groups), dim3(kJoinWaves * 64), 0, stream, s, keys,
+                           (int)long_tiles, long_groups, (int)tiles, (G*)dtable);
     };
     // 32 768 x 3 584 added: four columns 145 us, one 155; rows of fewer columns than a wavefront's four: 16 384 x 64 38, one 36
     if (s.hidden >= 256) join(Int<4>());
