@@ -500,7 +500,8 @@ struct JoinedColumns {
 };
 
 // Long runs by workgroups of a tile of 64 columns and 64 shares, whose wavefronts take every kJoinWaves-th part; short ones by
-// a wavefront each of workgroups of 64 kCols columns and kJoinShares shares.
+// a wavefront each of workgroups of 64 kCols columns and kJoinShares shares.  Joins of 32 768 x 3 584 bf16: 10 us; of 49 152 x
+// 2 048 added to fp32, most tokens of two kinds: 14.
 template <int GT, bool kAdd, int kCols>
 __global__ __launch_bounds__(kJoinWaves * 64) void join_kernel(Sums s, const int32_t* __restrict__ keys, int long_tiles,
                                                                int64_t long_groups, int tiles,

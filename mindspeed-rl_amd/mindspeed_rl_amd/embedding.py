@@ -23,8 +23,8 @@ def _check(ids, scale, vocab_start):
     scale, vocab_start = float(scale), int(vocab_start)
     if not math.isfinite(scale):
         raise ValueError("scale must be finite, not %r" % scale)
-    if vocab_start < 0:
-        raise ValueError("vocab_start must not be negative: %d" % vocab_start)
+    if not 0 <= vocab_start < 1 << 63:
+        raise ValueError("vocab_start must not be negative, nor beyond 64 bits: %d" % vocab_start)
     return scale, vocab_start
 
 
@@ -103,7 +103,7 @@ def token_embedding(ids, weight, scale=1.0, vocab_start=0):
 def token_embedding_grad(ids, grad, out, scale=1.0, vocab_start=0, accumulate=False):
     """The table's gradient without autograd, into ``out`` ``[V, H]`` (dense, of ``grad``'s type or fp32): ``out[v] = scale *
     sum of grad over the tokens with ids - vocab_start == v``, or ``out[v] +=`` that, with the other rows untouched, if
-    ``accumulate``.  ``grad`` is ``ids.shape + (H,)``.  Returns ``out``."""
+    ``accumulate``.  ``grad`` is ``ids.shape + (H,)`` and shares no memory with ``out``.  Returns ``out``."""
     if grad.dtype not in _FLOATS or (out.dtype is not grad.dtype and out.dtype is not torch.float32):
         raise TypeError("grad must be float32, bfloat16 or float16 and out of its type or float32: %s and %s"
                         % (grad.dtype, out.dtype))

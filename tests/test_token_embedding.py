@@ -68,6 +68,7 @@ def test_refused_arguments():
                        (lambda: mrl.token_embedding(ids, w[:, :0]), ValueError),
                        (lambda: mrl.token_embedding(ids, w, scale=float("nan")), ValueError),
                        (lambda: mrl.token_embedding(ids, w, vocab_start=-1), ValueError),
+                       (lambda: mrl.token_embedding(ids, w, vocab_start=1 << 64), ValueError),
                        (lambda: mrl.token_embedding(ids, w), RuntimeError),
                        (lambda: mrl.token_embedding_grad(ids, grad[:2], out), ValueError),
                        (lambda: mrl.token_embedding_grad(ids, grad[:, :4], out), ValueError),
