@@ -367,6 +367,46 @@ def test_streams_and_graphs(dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("hidden", [4, 64, 257, 520])
+def test_runs_that_cross_shares(dev, hidden):
+    """Tokens that are there 1 to 1 100 times, around every multiple of 8 of them at which a sum is taken another way.  Gradients of
+    small whole numbers: their sums are exact in whatever order, so equal bits are wanted."""
+    lengths = [8 * k + off for k in (1, 2, 3, 14, 15, 16, 17, 18, 31, 32, 33, 63, 64, 65, 79, 80, 81, 82, 136) for off in (-1, 0, 1, 9)]
+    vocab = len(lengths) + 3
+    g = torch.Generator(device=dev).manual_seed(8)
+    ids = torch.repeat_interleave(torch.arange(len(lengths), device=dev), torch.tensor(lengths, device=dev))
+    for left_out in (0, 1, 5):                      # the list's places against the shares' move
+        some = torch.cat([ids[left_out:], torch.full((100,), vocab + 7, device=dev)])
+        some = some[torch.randperm(some.numel(), generator=g, device=dev)]
+        dy = torch.randint(-2, 3, (some.numel(), hidden), generator=g, device=dev).float()
+        inside = some < vocab
+        want = torch.zeros(vocab, hidden, device=dev).index_add_(0, some[inside], dy[inside])
+        out = torch.full((vocab, hidden), float("nan"), device=dev)
+        assert torch.equal(mrl.token_embedding_grad(some, dy, out), want)
+        assert torch.equal(mrl.token_embedding_grad(some, dy, out, scale=-3.0, accumulate=True), want - 3.0 * want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1500, 30000])
+def test_the_largest_table(dev, n):
+    """2^31 - 2 rows, of one entry: row numbers of 31 bits, and the largest of them next to the ids that are outside."""
+    vocab = (1 << 31) - 2
+    ids = torch.randint(0, vocab + 1, (n,), device=dev)
+    ids[:40], ids[40:80] = vocab - 1, vocab
+    ids[80:90], ids[90:100] = 0, -1
+    table = torch.zeros(vocab, 1, dtype=torch.bfloat16, device=dev)
+    table[-1], table[0] = 3.0, 5.0
+    y = mrl.token_embedding(ids, table)
+    assert (y[:40] == 3).all() and not y[40:80].any() and (y[80:90] == 5).all() and not y[90:100].any()
+    mrl.token_embedding_grad(ids, torch.ones(n, 1, dtype=torch.bfloat16, device=dev), table, accumulate=True)
+    rows, counts = ids[(ids >= 0) & (ids < vocab)].unique(return_counts=True)
+    want = counts.float() + 3.0 * (rows == vocab - 1) + 5.0 * (rows == 0)
+    assert torch.equal(table[rows, 0].float(), want)            # whole numbers below 256
+    table[rows] = 0
+    assert not table.any()
+
+
+@pytest.mark.gpu
 def test_more_entries_than_31_bits(dev):
     """A table of more than 2^31 entries, and a gradient of as many."""
     vocab, h = 600011, 3584
