@@ -7,7 +7,7 @@
 // holds it, and nothing is copied to the device.
 //
 // Bound by memory.  1.4 GB: the norm 214 us (6.5 TB/s), clipped into other tensors 669 us (4.2 GB: 6.3 TB/s), bf16 into fp32
-// 892, in place 762; where the norm is within the bound nothing is written (207).  200 MB: 35, 93, 122, 99 us.
+// 892, in place 715; where the norm is within the bound nothing is written (207).  200 MB: 35, 93, 122, 96 us.
 #include <algorithm>
 
 #include "lane_ops.h"
@@ -373,12 +373,13 @@ extern "C" int mrl_grad_clip(const mrl_grad* grads, int64_t n_grads, float max_n
     const int64_t each = chunks_each(grads, n_grads, kScaleVecs);
     // Lists of more chunks than workgroups fit: those that go elsewhere take a workgroup a chunk, which the memory serves
     // best (1.4 GB 669 us; by workgroups that stay 740), and a launch in front forms the norm for them; in place the workgroups
-    // stay, for there may be nothing to do.  Of shorter lists every workgroup forms it (1 MB 7.4 us; with the launch 8.7).
+    // stay, half as many (1.4 GB 715 us, all of them 752), for there may be nothing to do: a workgroup a chunk takes 673, but 286
+    // instead of 214 where nothing is.  Of shorter lists every workgroup forms it (1 MB 7.4 us; with the launch 8.7).
     const bool alone = used == 0 || each > 1;
     if (alone) hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(kBlock), 0, s, workspace, used, norm);
     int write_norm = alone ? 0 : 1;
     const auto launch = [&](const Table& t, auto kernel) {
-        const int64_t groups = t.in_place ? (t.n_chunks + each - 1) / each : t.n_chunks < kMostGroups ? t.n_chunks : kMostGroups;
+        const int64_t groups = t.in_place ? (t.n_chunks + 2 * each - 1) / (2 * each) : t.n_chunks < kMostGroups ? t.n_chunks : kMostGroups;
         hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(kBlock), 0, s, t, workspace, alone ? 0 : used, norm, max_norm,
                            write_norm);
         write_norm = 0;
