@@ -719,8 +719,8 @@ int mrl_norm_fwd(const void* x, int dtype, int64_t n_rows, int64_t hidden, int64
 /* mrl_norm_bwd: dx (dense, the rows' type), dweight and dbias (the weight's type), each nullable:
  *   g = dy * weight, n = (x - mu) * rstd, dx = rstd * (g - mean g - n * mean(g n))   (RMS: without mean g)
  *   dweight = sum over rows of dy * n, dbias = sum over rows of dy
- * mean: the forward's, NULL for RMS norm.  Sums over rows are fp32, in an order that the sizes set: the same
- * call gives the same bits.  workspace (for dweight or dbias): 16-byte aligned, no clearing needed.  Outputs share
+ * mean: the forward's, NULL for RMS norm (dbias is that sum all the same, by a pass of its own over dy where dx is asked
+ * for too).  Sums over rows are fp32, in an order that the sizes set: the same call gives the same bits.  workspace (for dweight or dbias): 16-byte aligned, no clearing needed.  Outputs share
  * no memory with anything else. */
 int64_t mrl_norm_bwd_workspace_bytes(int64_t n_rows, int64_t hidden);
 int mrl_norm_bwd(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, int dtype,

@@ -651,12 +651,30 @@ void launch_bwd(const BwdArgs& a) {
     using T = typename Elem<DT>::T;
     using W = typename Elem<WDT>::T;
     const Team team = bwd_team_of(DT, a.n_rows, a.hidden);
-    const auto sum_parts = [&](int n_parts) {
-        hipLaunchKernelGGL((norm_part_sum_kernel<WDT>), dim3((unsigned)((a.hidden + 31) / 32), a.dbias ? 2 : 1), dim3(1024), 0,
-                           a.stream, a.part, n_parts, a.hidden, (W*)a.dweight, (W*)a.dbias);
+    const auto sum_parts = [&](int n_parts, void* dweight, void* dbias) {
+        hipLaunchKernelGGL((norm_part_sum_kernel<WDT>), dim3((unsigned)((a.hidden + 31) / 32), dbias ? 2 : 1), dim3(1024), 0,
+                           a.stream, a.part, n_parts, a.hidden, (W*)dweight, (W*)dbias);
+    };
+    const bool narrow = a.hidden < Elem<DT>::kVec;
+    const auto sum_columns = [&](void* dweight, void* dbias) {
+        const int64_t slab = slab_rows_of(a.n_rows);
+        const int n_slabs = (int)((a.n_rows + slab - 1) / slab);
+        const auto columns_kernel = [&](auto cols) {
+            constexpr int kCols = decltype(cols)::value;
+            const int64_t threads = (a.hidden + kCols - 1) / kCols;
+            hipLaunchKernelGGL((norm_columns_kernel<DT, kLayer, kCols>), dim3((unsigned)((threads + kBlock - 1) / kBlock), (unsigned)n_slabs),
+                               dim3(kBlock), 0, a.stream, (const T*)a.dy, a.dy_stride, (const T*)a.x, a.x_stride, a.n_rows, a.hidden, slab,
+                               a.mean, a.rstd, a.part);
+        };
+        if (n_slabs > 0 && narrow) columns_kernel(Int<1>());
+        else if (n_slabs > 0) columns_kernel(Int<Elem<DT>::kVec>());
+        sum_parts(n_slabs, dweight, dbias);
     };
     if (team.lanes > 0 && a.n_rows > 0 && a.dx) {
-        const bool sums = a.dweight || a.dbias;
+        // the one pass sums dy for layer norm alone: an RMS norm has no bias, so registers and adds for one would serve
+        // nobody but a caller who adds a bias behind it, and that one's dbias comes from a pass over the columns
+        void* const dbias = kLayer ? a.dbias : nullptr;
+        const bool sums = a.dweight || dbias;
         const int groups = bwd_groups(team, a.n_rows);
         const auto launch = [&](auto vecs, auto most, auto stream) {
             const int block = bwd_block(team);
@@ -666,7 +684,7 @@ void launch_bwd(const BwdArgs& a) {
                                dim3((unsigned)groups), dim3(block), lds, a.stream,
                                (const T*)a.dy, a.dy_stride, (const T*)a.x, a.x_stride, a.n_rows, (int)a.hidden, team.lanes,
                                (const W*)a.weight, a.mean, a.rstd, (T*)a.dx, sums && groups > 1 ? a.part : nullptr,
-                               groups > 1 ? (W*)nullptr : (W*)a.dweight, groups > 1 ? (W*)nullptr : (W*)a.dbias);
+                               groups > 1 ? (W*)nullptr : (W*)a.dweight, groups > 1 ? (W*)nullptr : (W*)dbias);
         };
         const auto launch_block = [&](auto stream) {
             if constexpr (DT == MRL_F32) {
@@ -679,10 +697,10 @@ void launch_bwd(const BwdArgs& a) {
         };
         if (team.lanes >= 64 && a.hidden * (int64_t)sizeof(T) % 128 == 0) launch_block(Int<1>());
         else launch_block(Int<0>());
-        if (sums && groups > 1) sum_parts(groups);
+        if (sums && groups > 1) sum_parts(groups, a.dweight, dbias);
+        if (a.dbias && !dbias) sum_columns(nullptr, a.dbias);
         return;
     }
-    const bool narrow = a.hidden < Elem<DT>::kVec;
     if (a.dx && a.n_rows > 0 && narrow)
         hipLaunchKernelGGL((norm_dx_narrow_kernel<DT, WDT, kLayer>), dim3((unsigned)((a.n_rows + kBlock - 1) / kBlock)), dim3(kBlock), 0,
                            a.stream, (const T*)a.dy, a.dy_stride, (const T*)a.x, a.x_stride, a.n_rows, (int)a.hidden,
@@ -690,19 +708,7 @@ void launch_bwd(const BwdArgs& a) {
     else if (a.dx && a.n_rows > 0)
         hipLaunchKernelGGL((norm_dx_kernel<DT, WDT, kLayer>), dim3((unsigned)a.n_rows), dim3(kWideBlock), 0, a.stream, (const T*)a.dy,
                            a.dy_stride, (const T*)a.x, a.x_stride, a.hidden, (const W*)a.weight, a.mean, a.rstd, (T*)a.dx);
-    if (!a.dweight && !a.dbias) return;
-    const int64_t slab = slab_rows_of(a.n_rows);
-    const int n_slabs = (int)((a.n_rows + slab - 1) / slab);
-    const auto columns_kernel = [&](auto cols) {
-        constexpr int kCols = decltype(cols)::value;
-        const int64_t threads = (a.hidden + kCols - 1) / kCols;
-        hipLaunchKernelGGL((norm_columns_kernel<DT, kLayer, kCols>), dim3((unsigned)((threads + kBlock - 1) / kBlock), (unsigned)n_slabs),
-                           dim3(kBlock), 0, a.stream, (const T*)a.dy, a.dy_stride, (const T*)a.x, a.x_stride, a.n_rows, a.hidden, slab,
-                           a.mean, a.rstd, a.part);
-    };
-    if (n_slabs > 0 && narrow) columns_kernel(Int<1>());
-    else if (n_slabs > 0) columns_kernel(Int<Elem<DT>::kVec>());
-    sum_parts(n_slabs);
+    if (a.dweight || a.dbias) sum_columns(a.dweight, a.dbias);
 }
 
 // The instance of a launch for the types of rows and vectors: vectors have the rows' type or fp32.

@@ -443,3 +443,32 @@ def test_more_entries_than_31_bits(dev):
     within(y[-64:].detach(), want["y"])
     within(dx[-64:], want["dx"])
     assert not y[:-64].any() and not dx[:-64].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_rms_norm_with_the_gradient_of_a_bias(dev, dtype):
+    """Through the C ABI: dbias is the columns' sum of dy without a mean too, whatever else is asked for, in rows of every kind,
+    and what is asked for beside it has the bits that it has alone.  The workspace holds NaN where nothing was written."""
+    code = _lib.dtype_code(torch.empty(0, dtype=dtype))
+    for rows, h in ((1, 64), (3, 3), (5, 64), (40, 136), (700, 1000), (2500, 1024), (33, 3584), (9, 20011)):
+        x, w, _, dy = make(dev, (rows, h), dtype, dtype, 14)
+        want = formula(x, w, None, 1e-5, False, dy)
+        y, rstd, s = torch.empty_like(x), torch.empty(rows, device=dev), _lib.stream(dev)
+        _lib.call("mrl_norm_fwd", x.data_ptr(), code, rows, h, h, w.data_ptr(), None, code, 0, 1e-5, y.data_ptr(), None,
+                  rstd.data_ptr(), s)
+        n = _lib.load().mrl_norm_bwd_workspace_bytes(rows, h)
+
+        def backward(need):
+            out = {k: torch.full_like(like, float("nan")) for k, like, on in zip(("dx", "dw", "db"), (x, w, w), need) if on}
+            ws = torch.full((n,), 255, dtype=torch.uint8, device=dev)
+            _lib.call("mrl_norm_bwd", dy.data_ptr(), h, x.data_ptr(), h, code, rows, h, w.data_ptr(), code, None, rstd.data_ptr(),
+                      *[out[k].data_ptr() if k in out else None for k in ("dx", "dw", "db")], ws.data_ptr(), n, s)
+            return out
+
+        for need in ((1, 1), (1, 0), (0, 1), (0, 0)):
+            got = backward(need + (1,))
+            for name, g in got.items():
+                within(g, want[name])
+            if any(need):
+                assert all(torch.equal(g, got[name]) for name, g in backward(need + (0,)).items())
