@@ -28,7 +28,8 @@ constexpr int kSortGroups = 128;            // most workgroups of a sort pass
 constexpr int kShares = 4096;               // most shares of the sorted list
 constexpr int kMinShare = 8;
 constexpr int kFewTokens = 2048;            // that one workgroup sorts in its LDS: 500 tokens 17 us in all, 2 000 24; by passes 25, 27
-constexpr int64_t kMostTokens = 1LL << 26;  // with a wavefront each, as many as a launch holds
+constexpr int64_t kMostTokens = 1LL << 26;  // of a call, and one more
+constexpr int64_t kLaunchTokens = kMostTokens - kBlock / 64;        // with a wavefront each, as many as a launch holds
 
 // the row that a token names, `vocab` where it is outside
 __device__ __forceinline__ int32_t row_of(const void* ids, int dtype, int64_t t, int64_t start, int64_t vocab) {
@@ -702,9 +703,14 @@ extern "C" int mrl_embedding_fwd(const void* ids, int ids_dtype, int64_t n_token
     const size_t es = mrl::float_dtype_bytes(dtype);
     MRL_REQUIRE(mrl::aligned(table, es) && mrl::aligned(out, es), MRL_ERR_MISALIGNED, "%s: misaligned buffer", fn);
     hipStream_t s = mrl::as_stream(stream);
-    if (dtype == MRL_F32) launch_lookup<MRL_F32>(ids, ids_dtype, n_tokens, vocab_start, table, vocab, hidden, scale, out, s);
-    else if (dtype == MRL_BF16) launch_lookup<MRL_BF16>(ids, ids_dtype, n_tokens, vocab_start, table, vocab, hidden, scale, out, s);
-    else launch_lookup<MRL_F16>(ids, ids_dtype, n_tokens, vocab_start, table, vocab, hidden, scale, out, s);
+    for (int64_t t = 0; t < n_tokens; t += kLaunchTokens) {         // a second launch for the last three tokens of the most
+        const int64_t n = n_tokens - t < kLaunchTokens ? n_tokens - t : kLaunchTokens;
+        const void* some = (const char*)ids + t * mrl::int_dtype_bytes(ids_dtype);
+        void* to = (char*)out + t * hidden * (int64_t)es;
+        if (dtype == MRL_F32) launch_lookup<MRL_F32>(some, ids_dtype, n, vocab_start, table, vocab, hidden, scale, to, s);
+        else if (dtype == MRL_BF16) launch_lookup<MRL_BF16>(some, ids_dtype, n, vocab_start, table, vocab, hidden, scale, to, s);
+        else launch_lookup<MRL_F16>(some, ids_dtype, n, vocab_start, table, vocab, hidden, scale, to, s);
+    }
     return mrl::check_launch(fn);
 }
 

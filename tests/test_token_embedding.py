@@ -433,3 +433,22 @@ def test_more_entries_than_31_bits(dev):
     sums = torch.empty(10, h, device=dev)
     mrl.token_embedding_grad(ids, y, sums)
     assert torch.equal(sums[0], dy[0].float() + dy[2].float()) and torch.equal(sums[1], dy[1].float()) and not sums[2:].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,h", [(torch.bfloat16, 8), (torch.float32, 4), (torch.bfloat16, 3)], ids=["8xbf16", "4xf32", "3xbf16"])
+def test_the_most_tokens(dev, dtype, h):
+    """2^26 - 1 tokens, three more than a launch holds wavefronts in workgroups of four: all of them looked up, and summed.
+    The gradient of ones: counts below 2^24, exact in fp32."""
+    n, vocab = (1 << 26) - 1, 50
+    g = torch.Generator(device=dev).manual_seed(12)
+    table = torch.randn(vocab, h, generator=g, device=dev).to(dtype)
+    ids = torch.randint(0, vocab, (n,), generator=g, device=dev, dtype=torch.int32)
+    for some in (ids, ids[:-2], ids[:-3]):              # one launch holds the last of them
+        y = mrl.token_embedding(some, table)
+        assert all(torch.equal(part, table[i.long()]) for part, i in zip(y.split(1 << 23), some.split(1 << 23)))
+        del y
+    out = torch.empty(vocab, h, device=dev)
+    mrl.token_embedding_grad(ids, torch.ones(n, h, dtype=dtype, device=dev), out)
+    counts = torch.bincount(ids, minlength=vocab)
+    assert counts.max() < 1 << 24 and torch.equal(out, counts.float()[:, None].expand(vocab, h))
