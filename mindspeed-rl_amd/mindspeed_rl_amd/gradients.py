@@ -79,6 +79,58 @@ def global_grad_norm(grads):
     return norm
 
 
+def _places(t):
+    """(first byte, bytes that lie together, [(step in bytes, how many), the widest first]) of the entries."""
+    together, steps = t.element_size(), []
+    for st, n in _steps(t):
+        st *= t.element_size()
+        if st == together and not steps:
+            together *= n
+        elif st > 0:                        # entries of an expanded dimension are the same ones
+            steps.insert(0, (st, n))
+    return t.data_ptr(), together, steps
+
+
+def _end(places):
+    at, together, steps = places
+    return at + together + sum((n - 1) * st for st, n in steps)
+
+
+def _meet(a, b):
+    """Whether two :func:`_places` have a byte in common."""
+    if a[0] >= _end(b) or b[0] >= _end(a):
+        return False
+    if not a[2] or (b[2] and b[2][0][0] > a[2][0][0]):
+        a, b = b, a
+    if not a[2]:
+        return True
+    (st, n), least = a[2][0], 0
+    a = a[0], a[1], a[2][1:]
+    if b[2] and b[2][0][0] == st:           # of two equal steps their difference counts
+        least, b = 1 - b[2][0][1], (b[0], b[1], b[2][1:])
+    # the blocks of a that begin in front of b's end and end behind its begin
+    first, last = max(least, (b[0] - _end(a)) // st + 1), min(n - 1, (_end(b) - 1 - a[0]) // st)
+    return any(_meet((a[0] + d * st, a[1], a[2]), b) for d in range(first, last + 1))
+
+
+def _refuse_shared(pairs):
+    """What the entry point sees to for dense tensors, for (gradient, output) some of which it gets as copies."""
+    everything = []
+    for g, o in pairs:
+        if g.numel() > 0:
+            everything.append((_places(o), True))
+            if g.data_ptr() != o.data_ptr() or g.dtype is not o.dtype or any(
+                    n > 1 and p != q for p, q, n in zip(g.stride(), o.stride(), g.shape)):
+                everything.append((_places(g), False))
+    everything.sort()
+    reach = []                              # those that may reach the next one
+    for places, written in everything:
+        reach = [r for r in reach if _end(r[0]) > places[0]]
+        if any((written or r[1]) and _meet(r[0], places) for r in reach):
+            raise ValueError("a tensor shares memory with another that is written")
+        reach.append((places, written))
+
+
 def _spaced(g, o, in_place):
     """(gradient, output) as dense tensors of one order, by copies where they are not."""
     source = g.detach().contiguous()
@@ -136,6 +188,8 @@ def clip_grad_norm_(grads, max_norm, out=None):
                 back.append((o, target, source))
                 p, q = source.data_ptr(), target.data_ptr()
             words += (p, q, g.numel(), code | to << 32)
+    if back:
+        _refuse_shared(zip(tensors, tensors) if out is None else zip(tensors[::2], written))
     dev = _device(tensors)
     table = array.array("q", words)
     norm, partial = _result(dev)

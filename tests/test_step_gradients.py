@@ -2,6 +2,7 @@
 together: token table, final norm, loss from the hidden states, a shared table's gradient, clipping."""
 import ctypes
 import math
+import random
 
 import pytest
 import torch
@@ -55,6 +56,57 @@ def test_refused_arguments():
                        (lambda: mrl.clip_grad_norm_([a], 1.0, out=[b[:4]]), RuntimeError)]:
         with pytest.raises(error):
             bad()
+
+
+def test_shared_memory_of_spaced_tensors():
+    """Entries apart: what is written and meets something else is refused, also where the entry point would get copies; what
+    lies between one another's entries is not (and is refused for its device here)."""
+    a, z = torch.zeros(6, 8), lambda *s: torch.zeros(s)  # noqa: E731
+    flat = torch.zeros(200)
+    shared = [([a[:, ::2], a[:, ::2]], None), ([a[:, :5], a[:, 4:]], None), ([a[:, 3:], a[2]], None), ([a[1:, 2:4], a.t()[3:]], None),
+              ([a[::2, :3], a[::4, 2:]], None), ([a[:, 3], a[4, 3:4]], None), ([flat.as_strided((5, 2), (21, 1)), flat[85:87]], None),
+              ([flat.as_strided((5, 2), (21, 1)), flat.as_strided((9, 1), (17, 1), 5)], None),      # 21 + 1 = 5 + 17
+              ([a[:, :4]], [a[:, 2:6]]), ([a[:, :4]], [a[:, 1:].t()[:4].t()]), ([z(6, 4), z(6, 5)], [a[:, :4], a[:, 3:]]),
+              ([z(6, 4), a[:, 3:5]], [a[:, :4], z(6, 2)]), ([z(6, 4), a[1, 3].expand(5, 4)], [a[:, :4], z(5, 4)]),
+              ([z(6, 6), a[:6, :6]], [z(6, 6), a[:6, :6].t()])]
+    apart = [([a[:, ::2], a[:, 1::2]], None), ([a[:, :3], a[:, 3:]], None), ([a[::2, :3], a[1::2, :3]], None), ([a[:, 3:], a[2, :3]], None),
+             ([a[::2, 3:], a[1]], None), ([a[:, 7], a[4, :7], a[0, :7]], None), ([a[:, :4]], [a[:, :4]]), ([a[:, :4], a[:, :4]], [z(6, 4), z(6, 4)]),
+             ([flat.as_strided((5, 2), (21, 1)), flat.as_strided((9, 1), (17, 1), 6)], None),
+             ([a[:, :4], a[1, :2].expand(5, 2)], [a[:, 4:], z(5, 2)]), ([a[:0, :4], a[:, :4]], None)]
+    for lists, error in ((shared, ValueError), (apart, RuntimeError)):
+        for grads, outs in lists:
+            for order in (1, -1):
+                with pytest.raises(error, match="shares memory" if error is ValueError else "GPU only"):
+                    mrl.clip_grad_norm_(grads[::order], 1.0, out=outs and outs[::order])
+
+
+def test_which_entries_share_memory():
+    """Against the sets of bytes, over views of one buffer in two types: any steps, expanded and overlapping ones among them."""
+    from mindspeed_rl_amd.gradients import _meet, _places
+    rng, base = random.Random(1), torch.zeros(300)
+
+    def view():
+        b = base if rng.random() < 0.7 else base.view(torch.bfloat16)
+        shape = [rng.randint(1, 5) for _ in range(rng.randint(0, 3))]
+        steps = [rng.choice([0, 1, 1, 2, 3, 4, 5, 7, 10, 14, 20, 35]) for _ in shape]
+        return b.as_strided(shape, steps, rng.randint(0, b.numel() // 3))
+
+    def touched(t):
+        places = [t.data_ptr()]
+        for st, n in zip(t.stride(), t.shape):
+            places = [p + st * i * t.element_size() for p in places for i in range(n)]
+        return {p + k for p in places for k in range(t.element_size())}
+
+    seen = [0, 0]
+    for _ in range(4000):
+        try:
+            p, q = view(), view()
+        except RuntimeError:                    # behind the buffer's end
+            continue
+        want = bool(touched(p) & touched(q))
+        assert _meet(_places(p), _places(q)) == _meet(_places(q), _places(p)) == want
+        seen[want] += 1
+    assert min(seen) > 100
 
 
 class Grad(ctypes.Structure):
@@ -187,6 +239,28 @@ def test_strides(dev):
     mrl.clip_grad_norm_([kept.detach()], 1.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+@pytest.mark.gpu
+def test_spaced_tensors_between_one_another(dev):
+    """Columns and rows of one matrix that share no entry, in place and into one another's gaps; what is refused is untouched."""
+    g = torch.Generator(device=dev).manual_seed(7)
+    base = torch.randn(30, 40, generator=g, device=dev)
+    for cut in (lambda t: [t[:, ::2], t[:, 1::2]], lambda t: [t[:, :13], t[:, 13:]], lambda t: [t[::2, :9], t[1::2, :9], t[:, 9:].t()]):
+        mine = base.clone()
+        parts = cut(mine)
+        norm = plain_norm(cut(base))
+        check_norm(mrl.clip_grad_norm_(parts, 0.5 * norm), cut(base))
+        for p, q in zip(parts, cut(base)):
+            check_scaled(p, q, norm, 0.5 * norm)
+    mine = base.clone()
+    check_norm(mrl.clip_grad_norm_([mine[:, ::2]], 1.0, out=[mine[:, 1::2]]), [base[:, ::2]])
+    assert torch.equal(mine[:, ::2], base[:, ::2])
+    check_scaled(mine[:, 1::2], base[:, ::2], plain_norm([base[:, ::2]]), 1.0)
+    mine = base.clone()
+    with pytest.raises(ValueError, match="shares memory"):
+        mrl.clip_grad_norm_([mine[:, ::2], mine[:, ::2]], 1.0)
+    assert torch.equal(mine, base)
 
 
 @pytest.mark.gpu
