@@ -5,6 +5,7 @@ both from the training framework below it.  Here they work on the gradients that
 :func:`token_embedding` and the norms leave behind, whatever their types.
 """
 import array
+import operator
 
 import torch
 from torch.autograd.graph import increment_version
@@ -12,6 +13,7 @@ from torch.autograd.graph import increment_version
 from . import _lib
 
 _PARTIALS = 2304            # MRL_GRAD_NORM_PARTIALS
+_REQUIRES_GRAD = operator.attrgetter("requires_grad")
 _CODES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 
 
@@ -148,7 +150,8 @@ def clip_grad_norm_(grads, max_norm, out=None):
     """Scales all ``grads`` by ``min(1, max_norm / (norm + 1e-6))`` and returns ``norm`` (:func:`global_grad_norm`), without
     a host synchronisation.  In place - gradients below the limit are then not touched - or into the tensors of ``out``, one
     for each of ``grads``, of the same shape and of the gradient's type or fp32 (an optimizer's main gradients).  What is written
-    may not share memory with anything else in the lists.  A norm that is not finite gives what the formula gives."""
+    may not share memory with anything else in the lists, nor be part of a graph (the gradients are meant, not the parameters).
+    A norm that is not finite gives what the formula gives."""
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError("max_norm must not be negative: %r" % max_norm)
@@ -190,6 +193,8 @@ def clip_grad_norm_(grads, max_norm, out=None):
             words += (p, q, g.numel(), code | to << 32)
     if back:
         _refuse_shared(zip(tensors, tensors) if out is None else zip(tensors[::2], written))
+    if True in map(_REQUIRES_GRAD, written):
+        raise ValueError("what is written is part of a graph: give the gradients (p.grad, not p) or detached tensors")
     dev = _device(tensors)
     table = array.array("q", words)
     norm, partial = _result(dev)

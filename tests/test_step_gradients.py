@@ -58,6 +58,21 @@ def test_refused_arguments():
             bad()
 
 
+def test_clipping_writes_to_no_part_of_a_graph():
+    """Parameters in the place of their gradients, gradients that are differentiated on: refused and left as they were."""
+    p = torch.full((4,), 3.0, requires_grad=True)
+    (g,) = torch.autograd.grad(p.square().sum(), [p], create_graph=True)
+    kept = (p * 2, p.detach() * 2)
+    for bad in (lambda: mrl.clip_grad_norm_([p], 1.0), lambda: mrl.clip_grad_norm_([kept[1], g], 1.0), lambda: mrl.clip_grad_norm_(kept[0], 1.0),
+                lambda: mrl.clip_grad_norm_([kept[1]], 1.0, out=[p]), lambda: mrl.clip_grad_norm_([p.unfold(0, 2, 2).t()], 1.0)):
+        with pytest.raises(ValueError, match="part of a graph"):
+            bad()
+    assert (p == 3).all()
+    # what is only read may be
+    with pytest.raises(RuntimeError, match="GPU only"):
+        mrl.clip_grad_norm_([g], 1.0, out=[torch.zeros(4)])
+
+
 def test_shared_memory_of_spaced_tensors():
     """Entries apart: what is written and meets something else is refused, also where the entry point would get copies; what
     lies between one another's entries is not (and is refused for its device here)."""
