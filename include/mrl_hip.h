@@ -709,8 +709,9 @@ int mrl_critic_loss_bwd_slope(const float* slope, int64_t batch, int64_t padded_
  * + eps)^(-1/2), in fp32, rounded once.  subtract_mean = 1: layer norm (bias nullable); 0: RMS norm
  * (mu = 0, bias NULL).  x: F32, BF16 or F16 with a row stride in elements, only read; y: the same type,
  * dense; weight and bias: the rows' type or F32.  mean and rstd [n_rows] fp32, nullable, are what
- * the backward takes.  A row with an infinity or NaN gives NaN in that row alone; squares of a row have to
- * stay in fp32.  hidden at most MRL_NORM_MAX_HIDDEN; rows as many as 2^32 threads hold, 1 to 1 024 for a row. */
+ * the backward takes.  A row with an infinity or NaN gives NaN in that row alone; the squares of a row have to
+ * add up inside fp32 (a root mean square of 1.8e19 / sqrt(hidden)), beyond which rstd is 0 and y the bias, or NaN
+ * where the mean overflows too.  hidden at most MRL_NORM_MAX_HIDDEN; rows as many as 2^32 threads hold, 1 to 1 024 for a row. */
 #define MRL_NORM_MAX_HIDDEN 1048576
 int mrl_norm_fwd(const void* x, int dtype, int64_t n_rows, int64_t hidden, int64_t row_stride,
                  const void* weight, const void* bias, int weight_dtype, int subtract_mean, float eps,

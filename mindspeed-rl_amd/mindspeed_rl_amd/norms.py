@@ -108,7 +108,8 @@ def layer_norm(x, weight, bias=None, eps=1e-5):
     """``(x - mean) * (var + eps)^(-1/2) * weight + bias`` over the last dimension of ``x`` ``[..., H]`` (fp32, bf16
     or fp16; rows of any stride), in fp32, rounded once to the type of ``x``.  ``weight`` and ``bias`` ``[H]`` have the type of
     ``x`` or fp32.  Differentiable (once) with respect to all three; sums over rows are taken in an order that the
-    sizes set.  A row's squares have to stay in fp32: entries above 1.8e19 do not."""
+    sizes set.  A row's squares have to add up inside fp32, which they do up to a root mean square of 1.8e19 / sqrt(H); a row
+    beyond it gives zeros (and the bias) and no gradient, or NaN where its mean overflows too."""
     return _norm(x, weight, bias, eps, True)
 
 

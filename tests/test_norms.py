@@ -472,3 +472,24 @@ def test_rms_norm_with_the_gradient_of_a_bias(dev, dtype):
                 within(g, want[name])
             if any(need):
                 assert all(torch.equal(g, got[name]) for name, g in backward(need + (0,)).items())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_rows_at_the_end_of_the_range(dev, dtype, kind):
+    """3 584 squares of at most 2.9e17 add up to at most 3.02e38, inside fp32; of twice as large entries they do not: zeros, and
+    the bias."""
+    for h in (3584, 20011):
+        x, w, b, dy = make(dev, (4, h), dtype, dtype, 15, kind == "layer")
+        top = 2.9e17 * (3584 / h) ** 0.5
+        x = (torch.sign(x.float()) * top * torch.linspace(0.5, 1.0, h, device=dev)).to(dtype)
+        want = formula(x, w, b, 1e-5, kind == "layer", dy)
+        xl = x.clone().requires_grad_()
+        y = apply(kind, xl, w, b, 1e-5)
+        within(y.detach(), want["y"])
+        within(torch.autograd.grad(y, [xl], dy)[0], want["dx"])
+        far = (x * 2).requires_grad_()
+        y = apply(kind, far, w, b, 1e-5)
+        assert torch.equal(y.detach(), torch.zeros_like(x) if b is None else b.expand(4, h))
+        assert not torch.autograd.grad(y, [far], dy)[0].any()
