@@ -776,8 +776,9 @@ extern "C" int mrl_norm_fwd(const void* x, int dtype, int64_t n_rows, int64_t hi
 
 extern "C" int64_t mrl_norm_bwd_workspace_bytes(int64_t n_rows, int64_t hidden) {
     if (n_rows <= 0 || hidden <= 0 || n_rows > 0x7fffffffLL || hidden > MRL_NORM_MAX_HIDDEN) return 0;
-    const int64_t slab = slab_rows_of(n_rows), slabs = (n_rows + slab - 1) / slab;
-    return (slabs > kBwdGroups ? slabs : kBwdGroups) * 2 * hidden * 4;
+    // two sums of a column for each workgroup of the one pass or each slab of rows: neither are more than the rows
+    static_assert(kColumnSlabs <= kBwdGroups, "a place for every slab");
+    return (n_rows < kBwdGroups ? n_rows : kBwdGroups) * 2 * hidden * 4;
 }
 
 extern "C" int mrl_norm_bwd(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, int dtype, int64_t n_rows,

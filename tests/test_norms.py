@@ -117,6 +117,14 @@ def test_entry_points_refuse_and_launch_nothing():
         assert bwd(**kw) == rc, kw
 
 
+def test_workspace_of_few_rows():
+    """Two sums of a column for every row, and for no more than the most workgroups."""
+    size = _lib.load().mrl_norm_bwd_workspace_bytes
+    for h in (1, 1000, 1 << 20):
+        assert size(1, h) == 8 * h and size(4, h) == 32 * h
+        assert all(size(n, h) <= size(n + 1, h) <= size(1 << 20, h) <= 512 * 8 * h for n in (1, 15, 16, 17, 255, 256, 511, 512, 513, 4096))
+
+
 def test_loss_objects_refuse_a_norm_that_is_not_applied():
     fn = mrl.LossFuncFactory.get_instance("ray_grpo", "actor")
     fn.add_loss_meta_info({"clip_ratio": 0.2, "kl_ctrl": mrl.FixedKLController(0.0), "kl_penalty": "low_var_kl",
