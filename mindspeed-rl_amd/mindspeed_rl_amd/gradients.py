@@ -13,16 +13,18 @@ from torch.autograd.graph import increment_version
 from . import _lib
 
 _PARTIALS = 2304            # MRL_GRAD_NORM_PARTIALS
+# names that every tensor of a list is met with: the host's time is what a short list takes
+_TENSOR, _STRIDED, _GET_DEVICE = torch.Tensor, torch.strided, torch.Tensor.get_device
 _REQUIRES_GRAD = operator.attrgetter("requires_grad")
 _CODES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 
 
 def _code(g):
     """The dtype code of a gradient that can be taken."""
-    if not isinstance(g, torch.Tensor):
+    if not isinstance(g, _TENSOR):
         raise TypeError("gradients must be tensors, not %s" % type(g).__name__)
     code = _CODES.get(g.dtype)
-    if code is None or g.layout is not torch.strided:
+    if code is None or g.layout is not _STRIDED:
         raise TypeError("gradients must be dense float32, bfloat16 or float16 tensors, not %s of %s" % (g.layout, g.dtype))
     return code
 
@@ -48,11 +50,8 @@ def _device(tensors):
     """Their one device, as :func:`_lib.require_device` would have it."""
     if not tensors:
         raise ValueError("no gradients")
-    index = tensors[0].get_device()
-    for t in tensors:
-        if t.get_device() != index:
-            index = -1
-    if index < 0:
+    indices = set(map(_GET_DEVICE, tensors))
+    if len(indices) != 1 or -1 in indices:
         _lib.require_device(*tensors)       # raises
     return _lib.require_device(tensors[0])
 
