@@ -8,8 +8,9 @@
 // joined afterwards: the same tokens give the same bits, a row that many tokens name is summed by many workgroups, and
 // every row is rounded once.  Bound by memory, and by the sort's few launches where tokens are few.
 //
-// 32 768 tokens of 12 242 rows of 152 064 x 3 584 bf16: lookup 57 us (5.7 TB/s), gradient 261 us (1.1 GB of zeros, 235 MB read:
-// 5.1 TB/s), added to fp32 145 us.  64 tokens: 8, 176 (6.2 TB/s) and 15 us.
+// 32 768 tokens of 12 242 rows of 152 064 x 3 584 bf16: lookup 57 us (5.7 TB/s), gradient 257 us (1.1 GB of zeros, 235 MB read:
+// 5.2 TB/s), added to fp32 141 us.  64 tokens: 8, 175 (6.2 TB/s) and 15 us.  (Here and below: calls that follow each other in a
+// replayed graph.)
 #include "lane_ops.h"
 #include "mrl_internal.h"
 #include "vector_access.h"
@@ -27,7 +28,7 @@ constexpr int kDigitBits = 9;
 constexpr int kSortGroups = 128;            // most workgroups of a sort pass
 constexpr int kShares = 4096;               // most shares of the sorted list
 constexpr int kMinShare = 8;
-constexpr int kFewTokens = 2048;            // that one workgroup sorts in its LDS: 500 tokens 17 us in all, 2 000 24; by passes 25, 27
+constexpr int kFewTokens = 2048;            // that one workgroup sorts in its LDS: 500 tokens 18 us in all, 2 000 23; by passes 25, 26
 constexpr int64_t kMostTokens = 1LL << 26;  // of a call, and one more
 constexpr int64_t kLaunchTokens = kMostTokens - kBlock / 64;        // with a wavefront each, as many as a launch holds
 
@@ -103,7 +104,7 @@ __host__ SortPlan sort_plan(int64_t n_tokens, int64_t vocab) {
 
 // Zeros for the gradient's rows that no token names: workgroups behind the sort's, which is bound by latency and leaves the
 // memory to them.  Rows that are named are written later.  Spread over the sort's launches, 32 768 tokens of 152 064 x 3 584
-// bf16 take 260 us; all behind the first 277.
+// bf16 take 257 us; all behind the first 274.
 struct Fill {
     char* at;                               // 2-byte aligned at least
     int64_t bytes;                          // this launch's part
@@ -502,7 +503,7 @@ struct JoinedColumns {
 
 // Long runs by workgroups of a tile of 64 columns and 64 shares, whose wavefronts take every kJoinWaves-th part; short ones by
 // a wavefront each of workgroups of 64 kCols columns and kJoinShares shares.  Joins of 32 768 x 3 584 bf16: 10 us; of 49 152 x
-// 2 048 added to fp32, most tokens of two kinds: 14.
+// 2 048 added to fp32, most tokens of two kinds: 13.
 template <int GT, bool kAdd, int kCols>
 __global__ __launch_bounds__(kJoinWaves * 64) void join_kernel(Sums s, const int32_t* __restrict__ keys, int long_tiles,
                                                                int64_t long_groups, int tiles,
@@ -644,7 +645,8 @@ void launch_sums(const Sums& s, const int32_t* keys, const int32_t* tokens, cons
         hipLaunchKernelGGL((join_kernel<GT, kAdd, kCols>), dim3((unsigned)groups), dim3(kJoinWaves * 64), 0, stream, s, keys,
                            (int)long_tiles, long_groups, (int)tiles, (G*)dtable);
     };
-    // 32 768 x 3 584 added: four columns 145 us, one 155; rows of fewer columns than a wavefront's four: 16 384 x 64 38, one 36
+    // 32 768 x 3 584 added: four columns 141 us, one 146; rows of fewer columns than a wavefront's four leave lanes idle (16 384 x 64
+    // 34.5 either way)
     if (s.hidden >= 256) join(Int<4>());
     else join(Int<1>());
 }
@@ -682,7 +684,7 @@ void launch_lookup(const void* ids, int ids_dtype, int64_t n_tokens, int64_t sta
                            (const T*)table, vocab, (int)hidden, scale, (T*)out);
     };
     // Few tokens are spread over the chip.  Of many, a lane takes as many vectors as divide the row's, so that none reads over:
-    // 32 768 x 3 584 bf16 57 us, one vector 76; 9 477 x 1 343 fp16 8.5, by four 9.9; 32 768 x 2 560 bf16 38.7, by four 40.8.
+    // 32 768 x 3 584 bf16 57 us, one vector 76; 9 477 x 1 343 fp16 8.5, by four 9.8; 32 768 x 2 560 bf16 38.7, by four 40.9.
     if (n_tokens * waves <= 4096 || waves == 1) launch(Int<1>());
     else if (waves % 7 == 0) launch(Int<7>());
     else if (waves % 5 == 0) launch(Int<5>());

@@ -6,8 +6,9 @@
 // does not show in the norm's fp32 bits but for a tie.  The list travels in the kernel's arguments, so a captured graph
 // holds it, and nothing is copied to the device.
 //
-// Bound by memory.  1.4 GB: the norm 214 us (6.5 TB/s), clipped into other tensors 669 us (4.2 GB: 6.3 TB/s), bf16 into fp32
-// 892, in place 715; where the norm is within the bound nothing is written (207).  200 MB: 35, 93, 122, 96 us.
+// Bound by memory.  1.4 GB: the norm 214 us (6.5 TB/s), clipped into other tensors 658 us (2.8 GB and the second read: 6.4 TB/s), bf16
+// into fp32 880, in place 703; where the norm is within the bound nothing is written (205).  200 MB: 35, 92, 122, 96 us.  (Here and
+// below: bf16, calls that follow each other in a replayed graph.)
 #include <algorithm>
 
 #include "lane_ops.h"
@@ -22,7 +23,7 @@ using mrl_vocab::Elem;
 constexpr int kBlock = 256;
 constexpr int kTable = 112;                 // tensors of a launch: 4 KB of arguments
 constexpr int kSumVecs = 4;                 // vectors of 16 bytes that a thread has on its way where squares are summed
-constexpr int kScaleVecs = 1;               // ... and where gradients are scaled: 1.4 GB of bf16 into fp32 892 us, by four 988
+constexpr int kScaleVecs = 1;               // ... and where gradients are scaled: 1.4 GB of bf16 into fp32 880 us, by four 974
 constexpr int64_t kCached = 256 << 20;      // bytes that the memory-side cache holds
 
 constexpr int chunk_bytes(int vecs) { return kBlock * vecs * 16; }  // of a tensor that a workgroup takes at a time
@@ -322,8 +323,8 @@ int64_t chunks_each(const mrl_grad* grads, int64_t n, int vecs) {
 }
 
 // Squares of all tensors into the workspace; the number of partial sums.  A list that is read again and that the
-// memory-side cache holds is left there, anything else goes past it (us, left / past: clipping 200 MB 93 / 104; the norm of
-// 1.4 GB 241 / 214).
+// memory-side cache holds is left there, anything else goes past it (us, left / past: clipping 200 MB 92 / 103; the norm of
+// 1.4 GB 240 / 214).
 int launch_squares(const mrl_grad* grads, int64_t n, bool read_again, double* partial, hipStream_t s) {
     const int64_t each = chunks_each(grads, n, kSumVecs);
     int64_t bytes = 0;
@@ -372,9 +373,9 @@ extern "C" int mrl_grad_clip(const mrl_grad* grads, int64_t n_grads, float max_n
     const int used = launch_squares(grads, n_grads, true, workspace, s);
     const int64_t each = chunks_each(grads, n_grads, kScaleVecs);
     // Lists of more chunks than workgroups fit: those that go elsewhere take a workgroup a chunk, which the memory serves
-    // best (1.4 GB 669 us; by workgroups that stay 740), and a launch in front forms the norm for them; in place the workgroups
-    // stay, half as many (1.4 GB 715 us, all of them 752), for there may be nothing to do: a workgroup a chunk takes 673, but 286
-    // instead of 214 where nothing is.  Of shorter lists every workgroup forms it (1 MB 7.4 us; with the launch 8.7).
+    // best (1.4 GB 658 us; by workgroups that stay 723), and a launch in front forms the norm for them; in place the workgroups
+    // stay, half as many (1.4 GB 703 us, all of them 734), for there may be nothing to do: a workgroup a chunk takes 655, but 278
+    // instead of 205 where nothing is.  Of shorter lists every workgroup forms it (1 MB into fp32 7.3 us; with the launch 8.7).
     const bool alone = used == 0 || each > 1;
     if (alone) hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(kBlock), 0, s, workspace, used, norm);
     int write_norm = alone ? 0 : 1;

@@ -6,8 +6,9 @@
 //   dw_j = sum_rows dy_j n_j,  db_j = sum_rows dy_j
 //
 // Everything is held in fp32 and rounded once, to the output's type.  Both passes are bound by memory: the forward reads and
-// writes a row once, the backward reads two and writes one.  32 768 x 3 584 bf16 RMS: forward 77 us (6.1 TB/s), backward
-// with the weight's gradient 122 us (5.8 TB/s; 117 without); 65 536 x 5 120: 220 and 340 us.
+// writes a row once, the backward reads two and writes one.  32 768 x 3 584 bf16 RMS: forward 78 us (6.0 TB/s), backward
+// with the weight's gradient 122 us (5.8 TB/s; 114 without); 65 536 x 5 120: 226 and 348 us.  Layer norm with all its gradients:
+// 82 and 128 us.  (Here and below: calls that follow each other in a replayed graph.)
 #include "lane_ops.h"
 #include "mrl_internal.h"
 #include "vector_access.h"
@@ -23,8 +24,8 @@ constexpr int kColumnSlabs = 256;           // most partial sums of a column
 
 // ------------------------------------------------------------------------------------ rows of any width
 // Rows longer than registers hold, or shorter than a vector: a workgroup a row, read again for every sum (from the caches:
-// a row is 4 MB at most), in vectors by 1 024 threads.  2 048 x 40 960 bf16 layer norm: forward 98 us (3.4 TB/s of what
-// has to move; 264 by 256 threads an entry at a time), dx alone 124, backward 221.
+// a row is 4 MB at most), in vectors by 1 024 threads.  2 048 x 40 960 bf16 layer norm: forward 102 us (3.3 TB/s of what
+// has to move; 264 by 256 threads an entry at a time), dx alone 127, backward 227.
 
 // Sums of two values over the workgroup, the same in every thread.
 __device__ __forceinline__ float2 block_sum2(float a, float b, float2* lds) {
@@ -147,7 +148,7 @@ __global__ __launch_bounds__(kWideBlock) void norm_dx_kernel(const typename Elem
     });
 }
 
-// Rows shorter than a vector: a thread a row.  100 000 x 7 bf16 layer norm: forward 5.3 us, a workgroup a row 91.
+// Rows shorter than a vector: a thread a row.  100 000 x 7 bf16 layer norm: forward 6.4 us, a workgroup a row 91.
 template <int DT, int WDT, bool kLayer>
 __global__ __launch_bounds__(kBlock) void norm_fwd_narrow_kernel(const typename Elem<DT>::T* __restrict__ x, int64_t x_stride,
                                                                  int64_t n_rows, int hidden,
@@ -199,7 +200,7 @@ __global__ __launch_bounds__(kBlock) void norm_dx_narrow_kernel(const typename E
 }
 
 // Partial sums of the columns, of such rows or where nothing else is asked for: kCols columns a thread (a vector, the last of
-// which ends with the row, or one), a slab of rows per workgroup in y.  4 096 x 28 672 bf16: 132 us with the sum of the slabs (3.6 TB/s).
+// which ends with the row, or one), a slab of rows per workgroup in y.  4 096 x 28 672 bf16: 123 us with the sum of the slabs (3.8 TB/s).
 template <int DT, bool kLayer, int kCols>
 __global__ __launch_bounds__(kBlock) void norm_columns_kernel(const typename Elem<DT>::T* __restrict__ dy, int64_t dy_stride,
                                                               const typename Elem<DT>::T* __restrict__ x, int64_t x_stride,
@@ -247,7 +248,7 @@ struct Team {
 };
 
 // Rows of whole lines that wavefronts hold go past the caches (kStream): nobody reads a line's other half later.  Through them,
-// 32 768 x 3 584 bf16: forward 84 us for 78, backward 138 for 123; 16 384 x 4 096 fp32 152 for 135.  Rows that share lines
+// 32 768 x 3 584 bf16: forward 84 us for 78, backward 138 for 122; 16 384 x 4 096 fp32 154 for 134.  Rows that share lines
 // with their neighbours, and the small ones of 16 lanes, go through.
 
 // Of a lane's vectors the last alone may lie behind the row.
@@ -559,11 +560,11 @@ int64_t slab_rows_of(int64_t n_rows) {
 }
 
 // The backward's teams hold twice the entries, and the sums of the columns besides: one or two vectors a lane.  Two, where the
-// next row is not requested ahead, are better served by the memory (us, one / two: 32 768 x 3 584 bf16 140 / 122, 65 536 x
-// 5 120 371 / 337, 65 536 x 2 048 143 / 133); of little data, where what follows the rows counts, one (9 477 x 1 343 fp16
-// 23 / 26, 2 500 x 1 024 fp32 13 / 14).  Rows of more than 2 048 vectors take four of fp32 (8 192 x 16 000 280 us, by the
+// next row is not requested ahead, are better served by the memory (us, one / two: 32 768 x 3 584 bf16 139 / 122, 65 536 x
+// 5 120 381 / 348, 65 536 x 2 048 147 / 136); of little data, where what follows the rows counts, one (9 477 x 1 343 fp16
+// 26 / 29, 2 500 x 1 024 fp32 14.7 / 15.7).  Rows of more than 2 048 vectors take four of fp32 (8 192 x 16 000 281 us, by the
 // kernels for any width 648); of 16 bits, eight entries each, four do not fit the registers (4 096 x 28 672 521 us, by
-// those kernels 294).
+// those kernels 298).
 Team bwd_team_of(int dtype, int64_t n_rows, int64_t hidden) {
     const int64_t nv = vectors_of(dtype, hidden);
     if (nv == 0) return {0, 0};
