@@ -769,6 +769,87 @@ int mrl_grad_clip(const mrl_grad* grads, int64_t n_grads, float max_norm, float*
                   void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * What surrounds the products of a decoder layer in an update, and the update's last step.  The reference leaves these to the
+ * training framework below it.
+ *
+ * mrl_add_norm_fwd: h = x + residual, rounded to the residual's type (the rows' or F32), and y = h * rstd * weight, rstd = (mean h^2
+ * + eps)^(-1/2) per row of `hidden` entries, in fp32, rounded to the rows' type: what an addition and mrl_norm_fwd (subtract_mean = 0)
+ * behind it give.  x and residual: row strides in elements, only read; h and y dense, each of its input's type; weight: the rows'
+ * type or F32; rstd [n_rows] fp32, nullable, is what the backward takes.  hidden at most MRL_NORM_MAX_HIDDEN, fewer than 2^24 rows.
+ * Outputs share no memory with anything else.
+ *
+ * mrl_norm_fp8_fwd: the same, or (residual and h NULL) the norm of x itself, with y as OCP e4m3 codes q [n_rows, hidden] and
+ * scales: scale = max(max |y| / 448, 2^-126) over a row (block 0: scale [n_rows]) or over 128 entries (block 128, hidden
+ * whole blocks: scale [n_rows, hidden / 128]), q = y / scale to the nearest, ties to even.  A row (block) with an infinity or NaN has
+ * that, or NaN, as its scale. */
+int mrl_add_norm_fwd(const void* x, int dtype, int64_t x_stride, const void* residual, int residual_dtype,
+                     int64_t residual_stride, int64_t n_rows, int64_t hidden, const void* weight,
+                     int weight_dtype, float eps, void* h, void* y, float* rstd, void* stream);
+int mrl_norm_fp8_fwd(const void* x, int dtype, int64_t x_stride, const void* residual, int residual_dtype,
+                     int64_t residual_stride, int64_t n_rows, int64_t hidden, const void* weight,
+                     int weight_dtype, float eps, int64_t block, void* h, void* q, float* scale, void* stream);
+
+/* mrl_add_norm_bwd: the gradient of the sum, d = dh + rstd * (g - n * mean(g n)), g = dy * weight, n = h * rstd (dh nullable: 0), as
+ * dx (the rows' type) and dresidual (the residual's), and dweight = sum over rows of dy * n (the weight's type), each
+ * nullable and dense; where the types are one, dx and dresidual are the same numbers and one of them will do.  Sums over rows are
+ * fp32, in an order that the sizes set: the same call gives the same bits.  workspace (for dweight): 16-byte aligned, no clearing needed.
+ * Outputs share no memory with anything else. */
+int64_t mrl_add_norm_bwd_workspace_bytes(int64_t n_rows, int64_t hidden);
+int mrl_add_norm_bwd(const void* dy, int64_t dy_stride, const void* dh, int64_t dh_stride, const void* h,
+                     int residual_dtype, int dtype, int64_t n_rows, int64_t hidden, const void* weight,
+                     int weight_dtype, const float* rstd, void* dx, void* dresidual, void* dweight,
+                     void* workspace, int64_t workspace_bytes, void* stream);
+
+/* mrl_rotary: turns pairs of entries of every head by the angle t = position * inv_freq[i], i = 0 .. part/2 - 1:
+ *   (a, b) -> scale * (a cos t - b sin t, b cos t + a sin t);  back != 0: by -t, which is the gradient
+ * Of a head the `part` entries from `start` on are turned - pairs are i and i + part/2 of them, or (interleaved) 2i and 2i + 1 -
+ * and the others copied.  Tokens are [n_outer, n_inner], fewer than 2^26; x: strides in elements of outer, inner and head, entries of a head
+ * dense, only read; out: dense [n_outer, n_inner, heads, dim] of the same type, F32, BF16 or F16.  k is nullable.
+ * positions: I32 or I64 of any sign, strides in elements (0: shared); inv_freq: part/2 doubles, in radians.  Angles are formed in 64 bits.
+ * part at most MRL_ROTARY_MAX_PART, heads * dim at most MRL_ROTARY_MAX_ROW.  Outputs share no memory with anything else. */
+#define MRL_ROTARY_MAX_PART 2048
+#define MRL_ROTARY_MAX_ROW 16777216
+typedef struct mrl_rotary_side {
+    const void* x;
+    void* out;
+    int64_t heads, dim, start;
+    int64_t stride_outer, stride_inner, stride_head;
+} mrl_rotary_side;
+int mrl_rotary(const mrl_rotary_side* q, const mrl_rotary_side* k, int dtype, const void* positions,
+               int positions_dtype, int64_t pos_outer, int64_t pos_inner, int64_t n_outer, int64_t n_inner,
+               const double* inv_freq, int64_t part, int interleaved, float scale, int back, void* stream);
+
+/* mrl_adamw_step: one step of AdamW for every tensor of a list (at most MRL_GRAD_TENSORS), t = step + 1, which is left in `step`:
+ *   g' = g * min(1, max_norm / (grad_norm + 1e-6))  (grad_norm NULL: g);  m = beta1 m + (1 - beta1) g';  v = beta2 v + (1 - beta2) g'^2
+ *   p = p (1 - lr weight_decay) - m / (sqrt(v) / sqrt(1 - beta2^t) + eps) * lr / (1 - beta1^t)
+ * in fp32.  p is `master` (fp32; param is then p rounded) or, without one, param itself (F32, BF16 or F16); grad has the parameter's type or
+ * F32 and is only read.  lr: lr_at[0], a device scalar, where that is given.  Nothing is read back: step, lr_at and grad_norm are device
+ * memory, so that a captured graph can be replayed.  The list is host memory and may be freed when the call returns.
+ *
+ * bits 32: exp_avg is m and exp_avg_sq is v, fp32.  bits 8: every 128 entries of a tensor in a row (the last ones: fewer) have fp32 scales s =
+ * max(max |x| / 448, 2^-126) in exp_avg_scale and exp_avg_sq_scale, and exp_avg and exp_avg_sq hold OCP e4m3 codes of x / s for x
+ * = m and x = sqrt(v): |x / s| is floor(|x / s| / step + u) steps of its binade, u the 16-bit fraction of a hash of t and the
+ * entry's place; a sqrt(v) above zero keeps at least the least code.  Gradients have to be finite: where one is not, its entry (8 bits: its
+ * block) holds NaN or an infinity afterwards.
+ * What is written shares no memory with anything else in the list.  workspace: MRL_ADAMW_WORKSPACE_BYTES, 16-byte aligned, no clearing needed. */
+#define MRL_ADAMW_WORKSPACE_BYTES 32
+typedef struct mrl_adamw_tensor {
+    void* param;
+    const void* grad;
+    void* master;
+    void* exp_avg;
+    void* exp_avg_sq;
+    float* exp_avg_scale;
+    float* exp_avg_sq_scale;
+    int64_t n;
+    int32_t dtype;
+    int32_t grad_dtype;
+} mrl_adamw_tensor;
+int mrl_adamw_step(const mrl_adamw_tensor* tensors, int64_t n_tensors, int bits, int64_t* step, double lr,
+                   const float* lr_at, double beta1, double beta2, double eps, double weight_decay,
+                   const float* grad_norm, float max_norm, void* workspace, void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * Plain device-to-device copy kernel of n_bytes (multiple of 16, 16-byte aligned pointers);
  * used to calibrate the rocprofv3 FETCH_SIZE / WRITE_SIZE counters and as the measured
  * bandwidth ceiling next to the 8 TB/s vendor peak.  No counterpart in the reference. */

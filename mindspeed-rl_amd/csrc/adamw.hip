@@ -1,0 +1,373 @@
+// A step of AdamW over a list of tensors for gfx950, clipped on the way, with moments in 32 or in 8 bits.
+//
+//   g' = g min(1, max_norm / (norm + 1e-6)),  m = b1 m + (1 - b1) g',  v = b2 v + (1 - b2) g'^2
+//   p = p (1 - lr wd) - m / (sqrt(v) / sqrt(1 - b2^t) + eps) lr / (1 - b1^t)
+//
+// Everything is held in fp32 (the powers of the betas in 64 bits) and the operations that lead to the moments are rounded one by
+// one, so that their bits do not depend on how the compiler joins them.  fp32 main weights are where there are any what p is, and the
+// parameter is p rounded.
+//
+// 8 bits: 128 entries of a tensor in a row share an fp32 scale s = max(max |x| / 448, 2^-126), x being m and sqrt(v) (whose
+// range is half of v's in its logarithm), and are held as e4m3 codes of x / s.  Moments change by less than half a step of such a
+// code from one update to the next, and rounding to the nearest would leave them where they are, so a value goes up or down by a
+// dither u in [0, 1), floor(|x / s| / step + u): on average it moves as it should.  u is the hash of the step's number and
+// the entry's place, the same for both moments; the same call gives the same bits.  A sqrt(v) above zero keeps at least
+// the least code, so that no m is divided by eps alone because its v was lost.
+#include <algorithm>
+#include <memory>
+#include <new>
+
+#include "lane_ops.h"
+#include "mrl_internal.h"
+#include "vector_access.h"
+#include "vocab_common.h"
+
+namespace {
+
+using mrl_vocab::Elem;
+
+constexpr int kBlock = 256;
+constexpr int kUnit = 8;                    // entries of a lane: 16 lanes a block of 128
+constexpr int kChunk = kBlock * kUnit;      // entries of a workgroup
+constexpr int kTable = 54;                  // tensors of a launch: 4 KB of arguments
+constexpr int64_t kMostGroups = (1LL << 24) - 1;    // of a launch, which holds fewer than 2^32 threads
+constexpr float kMost = 448.f;              // of e4m3
+constexpr float kLeastCode = 0.001953125f;  // 2^-9
+constexpr float kLeastScale = 1.17549435e-38f;      // 2^-126
+
+struct Part {
+    void* param;
+    const void* grad;
+    float* master;
+    void *m, *v;
+    float *m_scale, *v_scale;
+    int64_t n;
+    int64_t end_chunk;                      // chunks of this tensor and the ones in front of it
+};
+
+struct Table {
+    Part part[kTable];
+    int32_t n_parts, n_chunks;
+};
+
+// What the step's number sets, for all workgroups.
+struct Coefs {
+    float factor, decay, rate, second;
+    uint32_t key;
+};
+
+struct Constants {
+    float b1, rest1, b2, rest2, eps;
+};
+
+__global__ void adamw_prepare_kernel(int64_t* step, double lr, const float* lr_at, double b1, double b2, double weight_decay,
+                                     const float* norm, float max_norm, Coefs* out) {
+    const int64_t t = *step + 1;
+    if (lr_at) lr = (double)*lr_at;
+    Coefs c;
+    const float quotient = norm ? max_norm / (*norm + 1e-6f) : 1.f;
+    c.factor = quotient > 1.f ? 1.f : quotient;         // NaN, of a norm that is none, stays NaN
+    c.decay = (float)(1.0 - lr * weight_decay);
+    c.rate = (float)(lr / (1.0 - pow(b1, (double)t)));
+    c.second = (float)(1.0 / sqrt(1.0 - pow(b2, (double)t)));
+    c.key = (uint32_t)t * 0x9E3779B9u;
+    *out = c;
+    *step = t;
+}
+
+// 16 bits for the even and 16 for the odd entry of a pair: what multiplications and shifts mix of its number and the step's.
+__device__ __forceinline__ uint32_t dither(uint32_t pair, uint32_t key) {
+    uint32_t x = pair ^ key;
+    x = (x ^ (x >> 16)) * 0x7feb352du;
+    x = (x ^ (x >> 15)) * 0x846ca68bu;
+    return x ^ (x >> 16);
+}
+
+template <int DT>
+__device__ __forceinline__ void load_unit(const void* base, int64_t at, int valid, float (&z)[kUnit]) {
+    const typename Elem<DT>::T* p = (const typename Elem<DT>::T*)base + at;
+    if (valid == kUnit) {
+        mrl::load_floats<DT>(p, z);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kUnit; ++i) z[i] = i < valid ? Elem<DT>::load(p + i) : 0.f;
+    }
+}
+
+template <int DT>
+__device__ __forceinline__ void store_unit(void* base, int64_t at, int valid, const float (&z)[kUnit]) {
+    constexpr int kVec = Elem<DT>::kVec;
+    typename Elem<DT>::T* p = (typename Elem<DT>::T*)base + at;
+    if (valid == kUnit) {
+#pragma unroll
+        for (int q = 0; q < kUnit / kVec; ++q) {
+            float t[kVec];
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) t[i] = z[q * kVec + i];
+            mrl::Vec<DT>::store(p + q * kVec, Elem<DT>::pack(t));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kUnit; ++i)
+            if (i < valid) Elem<DT>::store(p + i, z[i]);
+    }
+}
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef u32x2 u32x2_anywhere __attribute__((aligned(1)));
+
+__device__ __forceinline__ u32x2 load_codes(const void* base, int64_t at, int valid) {
+    const uint8_t* p = (const uint8_t*)base + at;
+    if (valid == kUnit) return *(const u32x2_anywhere*)p;
+    u32x2 r = {0u, 0u};
+#pragma unroll
+    for (int i = 0; i < kUnit; ++i)
+        if (i < valid) r[i >> 2] |= (uint32_t)p[i] << (8 * (i & 3));
+    return r;
+}
+
+__device__ __forceinline__ void store_codes(void* base, int64_t at, int valid, u32x2 c) {
+    uint8_t* p = (uint8_t*)base + at;
+    if (valid == kUnit) {
+        *(u32x2_anywhere*)p = c;
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < kUnit; ++i)
+        if (i < valid) p[i] = (uint8_t)(c[i >> 2] >> (8 * (i & 3)));
+}
+
+__device__ __forceinline__ void values_of(u32x2 c, float scale, float (&z)[kUnit]) {
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        const mrl_vocab::floatx2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[w], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[w], true);
+        z[4 * w] = mrl::mul_rn(lo[0], scale);
+        z[4 * w + 1] = mrl::mul_rn(lo[1], scale);
+        z[4 * w + 2] = mrl::mul_rn(hi[0], scale);
+        z[4 * w + 3] = mrl::mul_rn(hi[1], scale);
+    }
+}
+
+// The largest |z| of the 16 lanes of a block, by its bits: an infinity's lie above all numbers', NaN's above those.
+__device__ __forceinline__ float block_scale(const float (&z)[kUnit]) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < kUnit; ++i) most = max(most, __float_as_uint(fabsf(z[i])));
+    most = max(most, mrl::lane_partner_bits<0>(most));
+    most = max(most, mrl::lane_partner_bits<1>(most));
+    most = max(most, mrl::lane_partner_bits<2>(most));
+    most = max(most, mrl::lane_partner_bits<3>(most));
+    const float s = mrl::mul_rn(__uint_as_float(most), 1.f / kMost);
+    return s < kLeastScale ? kLeastScale : s;
+}
+
+// floor(|x| / step + u) steps of x's binade, x = z / scale: what the conversion instruction does with the dither in the upper bits.
+template <bool kRoot>
+__device__ __forceinline__ u32x2 codes_of(const float (&z)[kUnit], float scale, const uint32_t (&bits)[kUnit / 2]) {
+    const float inv = 1.f / scale;
+    u32x2 c = {0u, 0u};
+    float x[kUnit];
+#pragma unroll
+    for (int i = 0; i < kUnit; ++i) {
+        float t = mrl::mul_rn(z[i], inv);
+        t = t > kMost ? kMost : t;          // NaN stays
+        if (kRoot) t = z[i] > 0.f && t < kLeastCode ? kLeastCode : t;
+        else t = t < -kMost ? -kMost : t;
+        x[i] = t;
+    }
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        int r = 0;
+        r = __builtin_amdgcn_cvt_sr_fp8_f32(x[4 * w], (int)(bits[2 * w] << 16), r, 0);
+        r = __builtin_amdgcn_cvt_sr_fp8_f32(x[4 * w + 1], (int)(bits[2 * w] & 0xffff0000u), r, 1);
+        r = __builtin_amdgcn_cvt_sr_fp8_f32(x[4 * w + 2], (int)(bits[2 * w + 1] << 16), r, 2);
+        r = __builtin_amdgcn_cvt_sr_fp8_f32(x[4 * w + 3], (int)(bits[2 * w + 1] & 0xffff0000u), r, 3);
+        c[w] = (uint32_t)r;
+    }
+    return c;
+}
+
+template <int PT, int GT, bool kMaster, bool kSmall>
+__global__ __launch_bounds__(kBlock) void adamw_kernel(Table t, const Coefs* __restrict__ coefs, Constants k) {
+    __shared__ int32_t ends[64];
+    if (threadIdx.x < 64) ends[threadIdx.x] = (int)threadIdx.x < t.n_parts ? (int32_t)t.part[threadIdx.x].end_chunk : 0x7fffffff;
+    __syncthreads();
+    const Coefs c = *coefs;
+    for (int chunk = blockIdx.x; chunk < t.n_chunks; chunk += gridDim.x) {
+        // as many tensors end at or in front of it
+        const int part = __builtin_amdgcn_readfirstlane(__popcll(__ballot(ends[threadIdx.x & 63] <= chunk)));
+        const Part& p = t.part[part];
+        const int64_t at = (chunk - (part == 0 ? 0 : t.part[part - 1].end_chunk)) * kChunk + threadIdx.x * kUnit;
+        const int64_t left = p.n - at;
+        const int valid = left >= kUnit ? kUnit : left > 0 ? (int)left : 0;
+        float g[kUnit], w[kUnit], m[kUnit], v[kUnit];
+        load_unit<GT>(p.grad, at, valid, g);
+        if (kMaster) load_unit<MRL_F32>(p.master, at, valid, w);
+        else load_unit<PT>(p.param, at, valid, w);
+        const int64_t block = valid > 0 ? at / 128 : 0;
+        if (kSmall) {
+            values_of(load_codes(p.m, at, valid), p.m_scale[block], m);
+            values_of(load_codes(p.v, at, valid), p.v_scale[block], v);
+#pragma unroll
+            for (int i = 0; i < kUnit; ++i) v[i] = mrl::mul_rn(v[i], v[i]);
+        } else {
+            load_unit<MRL_F32>(p.m, at, valid, m);
+            load_unit<MRL_F32>(p.v, at, valid, v);
+        }
+        float root[kUnit];
+#pragma unroll
+        for (int i = 0; i < kUnit; ++i) {
+            g[i] = mrl::mul_rn(g[i], c.factor);
+            m[i] = mrl::add_rn(mrl::mul_rn(m[i], k.b1), mrl::mul_rn(g[i], k.rest1));
+            v[i] = mrl::add_rn(mrl::mul_rn(v[i], k.b2), mrl::mul_rn(mrl::mul_rn(g[i], g[i]), k.rest2));
+            root[i] = sqrtf(v[i]);
+            w[i] = w[i] * c.decay - m[i] / (root[i] * c.second + k.eps) * c.rate;
+        }
+        if (kMaster) store_unit<MRL_F32>(p.master, at, valid, w);
+        store_unit<PT>(p.param, at, valid, w);
+        if (kSmall) {
+            uint32_t bits[kUnit / 2];
+#pragma unroll
+            for (int i = 0; i < kUnit / 2; ++i) bits[i] = dither((uint32_t)(at / 2) + i, c.key);
+            const float ms = block_scale(m), vs = block_scale(root);
+            store_codes(p.m, at, valid, codes_of<false>(m, ms, bits));
+            store_codes(p.v, at, valid, codes_of<true>(root, vs, bits));
+            if (valid > 0 && (threadIdx.x & 15) == 0) {
+                p.m_scale[block] = ms;
+                p.v_scale[block] = vs;
+            }
+        } else {
+            store_unit<MRL_F32>(p.m, at, valid, m);
+            store_unit<MRL_F32>(p.v, at, valid, v);
+        }
+    }
+}
+
+// The launches of a list for the tensors of a kind that are not empty: launch(table) for each at most kTable of them.
+template <typename F>
+void for_tables(const mrl_adamw_tensor* list, int64_t n, int dtype, int grad_dtype, bool master, F launch) {
+    Table t;
+    t.n_parts = 0;
+    int64_t chunks = 0;
+    for (int64_t i = 0; i < n; ++i) {
+        const mrl_adamw_tensor& p = list[i];
+        if (p.n == 0 || p.dtype != dtype || p.grad_dtype != grad_dtype || (p.master != nullptr) != master) continue;
+        chunks += (p.n + kChunk - 1) / kChunk;
+        t.part[t.n_parts++] = {p.param, p.grad, (float*)p.master, p.exp_avg, p.exp_avg_sq, p.exp_avg_scale, p.exp_avg_sq_scale, p.n, chunks};
+        t.n_chunks = (int32_t)chunks;
+        if (t.n_parts == kTable) {
+            launch(t);
+            t.n_parts = 0;
+            chunks = 0;
+        }
+    }
+    if (t.n_parts > 0) launch(t);
+}
+
+int check_tensor(const char* fn, long long i, const mrl_adamw_tensor& p, int bits) {
+    const size_t es = mrl::float_dtype_bytes(p.dtype), gs = mrl::float_dtype_bytes(p.grad_dtype), ms = bits == 8 ? 1 : 4;
+    MRL_REQUIRE(es != 0, MRL_ERR_UNSUPPORTED, "%s: tensor %lld: dtype %d (want F32, BF16 or F16)", fn, i, p.dtype);
+    MRL_REQUIRE(gs != 0 && (p.grad_dtype == p.dtype || p.grad_dtype == MRL_F32), MRL_ERR_UNSUPPORTED,
+                "%s: tensor %lld: gradient dtype %d (want the parameter's or F32)", fn, i, p.grad_dtype);
+    MRL_REQUIRE(p.n >= 0, MRL_ERR_INVALID_ARG, "%s: tensor %lld: n=%lld", fn, i, (long long)p.n);
+    MRL_REQUIRE(p.n <= (1LL << 33), MRL_ERR_UNSUPPORTED, "%s: tensor %lld: n=%lld (at most 2^33)", fn, i, (long long)p.n);
+    MRL_REQUIRE(!p.master || p.dtype != MRL_F32, MRL_ERR_INVALID_ARG, "%s: tensor %lld: main weights beside an F32 parameter", fn, i);
+    MRL_REQUIRE(p.n == 0 || (p.param && p.grad && p.exp_avg && p.exp_avg_sq && (bits == 32 || (p.exp_avg_scale && p.exp_avg_sq_scale))),
+                MRL_ERR_INVALID_ARG, "%s: tensor %lld: NULL pointer", fn, i);
+    MRL_REQUIRE(mrl::aligned(p.param, es) && mrl::aligned(p.grad, gs) && mrl::aligned(p.master, 4) && mrl::aligned(p.exp_avg, ms) &&
+                    mrl::aligned(p.exp_avg_sq, ms) && mrl::aligned(p.exp_avg_scale, 4) && mrl::aligned(p.exp_avg_sq_scale, 4),
+                MRL_ERR_MISALIGNED, "%s: tensor %lld: misaligned", fn, i);
+    return MRL_OK;
+}
+
+// What is written meets nothing else that is read or written: a parameter given twice would take two steps.
+int check_overlap(const char* fn, const mrl_adamw_tensor* list, int64_t n, int bits, const int64_t* step, const float* norm,
+                  const float* lr, const float* workspace) {
+    struct Range {
+        uintptr_t begin, end;
+        int32_t tensor;
+        bool written;
+    };
+    const std::unique_ptr<Range[]> all(new (std::nothrow) Range[n * 7 + 4]);
+    MRL_REQUIRE(all, MRL_ERR_UNSUPPORTED, "%s: no host memory to look %lld tensors over", fn, (long long)n);
+    int64_t count = 0;
+    const auto add = [&](const void* p, int64_t bytes, int64_t i, bool written) {
+        if (p && bytes > 0) all[count++] = {(uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes, (int32_t)i, written};
+    };
+    for (int64_t i = 0; i < n; ++i) {
+        const mrl_adamw_tensor& p = list[i];
+        const int64_t moment = bits == 8 ? p.n : 4 * p.n, scales = bits == 8 ? (p.n + 127) / 128 * 4 : 0;
+        add(p.param, p.n * mrl::float_dtype_bytes(p.dtype), i, true);
+        add(p.grad, p.n * mrl::float_dtype_bytes(p.grad_dtype), i, false);
+        add(p.master, p.n * 4, i, true);
+        add(p.exp_avg, moment, i, true);
+        add(p.exp_avg_sq, moment, i, true);
+        add(p.exp_avg_scale, scales, i, true);
+        add(p.exp_avg_sq_scale, scales, i, true);
+    }
+    add(step, 8, -1, true);
+    add(norm, 4, -1, false);
+    add(lr, 4, -1, false);
+    add(workspace, MRL_ADAMW_WORKSPACE_BYTES, -1, true);
+    std::sort(all.get(), all.get() + count, [](const Range& a, const Range& b) { return a.begin < b.begin; });
+    // the furthest ends so far of everything and of what is written
+    uintptr_t reach = 0, written = 0;
+    for (int64_t q = 0; q < count; ++q) {
+        const Range& r = all[q];
+        MRL_REQUIRE(r.begin >= (r.written ? reach : written), MRL_ERR_INVALID_ARG, "%s: tensor %d shares memory with another that is written",
+                    fn, r.tensor);
+        reach = std::max(reach, r.end);
+        if (r.written) written = std::max(written, r.end);
+    }
+    return MRL_OK;
+}
+
+}  // namespace
+
+extern "C" int mrl_adamw_step(const mrl_adamw_tensor* tensors, int64_t n_tensors, int bits, int64_t* step, double lr,
+                              const float* lr_at, double beta1, double beta2, double eps, double weight_decay, const float* grad_norm,
+                              float max_norm, void* workspace, void* stream) {
+    const char* fn = "mrl_adamw_step";
+    MRL_REQUIRE(n_tensors >= 0 && (n_tensors == 0 || tensors), MRL_ERR_INVALID_ARG, "%s: n_tensors=%lld", fn, (long long)n_tensors);
+    MRL_REQUIRE(n_tensors <= MRL_GRAD_TENSORS, MRL_ERR_UNSUPPORTED, "%s: %lld tensors (at most %d)", fn, (long long)n_tensors, MRL_GRAD_TENSORS);
+    MRL_REQUIRE(bits == 32 || bits == 8, MRL_ERR_UNSUPPORTED, "%s: bits=%d (want 32 or 8)", fn, bits);
+    const auto number = [](double x) { return x >= 0.0 && x <= 3.0e38; };
+    MRL_REQUIRE((lr_at || number(lr)) && number(weight_decay) && number(eps) && eps > 0.0 && (float)eps > 0.f, MRL_ERR_INVALID_ARG,
+                "%s: lr=%g eps=%g weight_decay=%g", fn, lr, eps, weight_decay);
+    MRL_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, MRL_ERR_INVALID_ARG, "%s: betas %g and %g (want [0, 1))", fn,
+                beta1, beta2);
+    MRL_REQUIRE(!grad_norm || max_norm >= 0.f, MRL_ERR_INVALID_ARG, "%s: max_norm=%g", fn, (double)max_norm);
+    MRL_REQUIRE(step && workspace, MRL_ERR_INVALID_ARG, "%s: NULL pointer", fn);
+    MRL_REQUIRE(mrl::aligned(step, 8) && mrl::aligned(lr_at, 4) && mrl::aligned(grad_norm, 4) && mrl::aligned(workspace, 16), MRL_ERR_MISALIGNED,
+                "%s: misaligned buffer", fn);
+    for (int64_t i = 0; i < n_tensors; ++i) {
+        const int rc = check_tensor(fn, (long long)i, tensors[i], bits);
+        if (rc != MRL_OK) return rc;
+    }
+    const int rc = check_overlap(fn, tensors, n_tensors, bits, step, grad_norm, lr_at, (const float*)workspace);
+    if (rc != MRL_OK) return rc;
+    hipStream_t s = mrl::as_stream(stream);
+    Coefs* coefs = (Coefs*)workspace;
+    static_assert(sizeof(Coefs) <= MRL_ADAMW_WORKSPACE_BYTES, "the workspace holds them");
+    hipLaunchKernelGGL(adamw_prepare_kernel, dim3(1), dim3(1), 0, s, step, lr, lr_at, beta1, beta2, weight_decay, grad_norm, max_norm, coefs);
+    const Constants k = {(float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps};
+    const auto launch = [&](const Table& t, auto kernel) {
+        const int64_t groups = t.n_chunks < kMostGroups ? t.n_chunks : kMostGroups;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(kBlock), 0, s, t, coefs, k);
+    };
+#define MRL_KIND(DT, GT, MASTER)                                                                                     \
+    for_tables(tensors, n_tensors, DT, GT, MASTER, [&](const Table& t) {                                             \
+        bits == 8 ? launch(t, adamw_kernel<DT, GT, MASTER, true>) : launch(t, adamw_kernel<DT, GT, MASTER, false>);  \
+    })
+    MRL_KIND(MRL_F32, MRL_F32, false);
+    MRL_KIND(MRL_BF16, MRL_BF16, false);
+    MRL_KIND(MRL_BF16, MRL_BF16, true);
+    MRL_KIND(MRL_BF16, MRL_F32, false);
+    MRL_KIND(MRL_BF16, MRL_F32, true);
+    MRL_KIND(MRL_F16, MRL_F16, false);
+    MRL_KIND(MRL_F16, MRL_F16, true);
+    MRL_KIND(MRL_F16, MRL_F32, false);
+    MRL_KIND(MRL_F16, MRL_F32, true);
+#undef MRL_KIND
+    return mrl::check_launch(fn);
+}

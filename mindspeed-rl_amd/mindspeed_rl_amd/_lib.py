@@ -26,6 +26,7 @@ _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _int = ctypes.c_int
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 
 class RaggedColumn(ctypes.Structure):
     """struct mrl_ragged_column"""
@@ -120,6 +121,12 @@ SIGNATURES = {
     "mrl_embedding_bwd": [_vp, _int, _i64, _i64, _vp, _int, _i64, _i64, _f32, _vp, _int, _int, _vp, _i64, _vp],
     "mrl_grad_norm": [_vp, _i64, _vp, _vp, _vp],
     "mrl_grad_clip": [_vp, _i64, _f32, _vp, _vp, _vp],
+    "mrl_add_norm_fwd": [_vp, _int, _i64, _vp, _int, _i64, _i64, _i64, _vp, _int, _f32, _vp, _vp, _vp, _vp],
+    "mrl_norm_fp8_fwd": [_vp, _int, _i64, _vp, _int, _i64, _i64, _i64, _vp, _int, _f32, _i64, _vp, _vp, _vp, _vp],
+    "mrl_add_norm_bwd_workspace_bytes": [_i64, _i64],
+    "mrl_add_norm_bwd": [_vp, _i64, _vp, _i64, _vp, _int, _int, _i64, _i64, _vp, _int, _vp, _vp, _vp, _vp, _vp, _i64, _vp],
+    "mrl_rotary": [_vp, _vp, _int, _vp, _int, _i64, _i64, _i64, _i64, _vp, _i64, _int, _f32, _int, _vp],
+    "mrl_adamw_step": [_vp, _i64, _int, _vp, _f64, _vp, _f64, _f64, _f64, _f64, _vp, _f32, _vp, _vp],
     "mrl_copy_bytes": [_vp, _vp, _i64, _vp],
     "mrl_bandwidth_probe": [_int, _vp, _vp, _i64, _i64, _vp],
 }
@@ -127,7 +134,8 @@ _RESTYPES = {"mrl_last_error": ctypes.c_char_p, "mrl_fused_workspace_bytes": cty
              "mrl_lmhead_workspace_bytes": ctypes.c_int64, "mrl_lmhead_static_max_tokens": ctypes.c_int64,
              "mrl_set_wide_spin_limit": ctypes.c_int64, "mrl_gae_whiten_workspace_bytes": ctypes.c_int64,
              "mrl_value_loss_workspace_bytes": ctypes.c_int64, "mrl_lmhead_bwd_workspace_bytes": ctypes.c_int64,
-             "mrl_norm_bwd_workspace_bytes": ctypes.c_int64, "mrl_embedding_bwd_workspace_bytes": ctypes.c_int64}
+             "mrl_norm_bwd_workspace_bytes": ctypes.c_int64, "mrl_add_norm_bwd_workspace_bytes": ctypes.c_int64,
+             "mrl_embedding_bwd_workspace_bytes": ctypes.c_int64}
 
 _lib = None
 _entry = {}             # name -> bound function, looked up once

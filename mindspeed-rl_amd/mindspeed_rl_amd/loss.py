@@ -579,8 +579,9 @@ class MultimodalLogProbComputer(LogProbComputer):
 
 
 def _refuse_norm_of_logits(kwargs):
-    if kwargs.get("final_norm_weight") is not None:
-        raise ValueError("final_norm_weight= needs lm_head_weight=: logits are not normalised")
+    for name in ("final_norm_weight", "final_norm_residual"):
+        if kwargs.get(name) is not None:
+            raise ValueError("%s= needs lm_head_weight=: logits are not normalised" % name)
 
 
 # ------------------------------------------------------------------------------------ loss objects
@@ -619,7 +620,8 @@ class BaseLossFunc(ABC):
         logits exist for one chunk of rows at a time, and ``backward()`` reaches the hidden states
         and the weight.  Forward-only calls take the same keyword through ``compute_log_probs``.  With
         ``final_norm_weight=`` the hidden states are those in front of the model's last norm
-        (:func:`norms.final_norm`), and ``backward()`` reaches its weight and bias as well."""
+        (:func:`norms.final_norm`), and ``backward()`` reaches its weight and bias as well, with ``final_norm_residual=``
+        also the residual stream."""
         from .lmhead import fused_lmhead_policy_loss
         if type(self.logprob_computer) is not StandardLogProbComputer:
             raise NotImplementedError("lm_head_weight= needs the standard log-prob strategy")

@@ -20,6 +20,12 @@ def _workspace_bytes(n_rows, hidden):
     return _lib.load().mrl_norm_bwd_workspace_bytes(n_rows, hidden)
 
 
+@functools.lru_cache(maxsize=256)
+def _add_workspace_bytes(n_rows, hidden):
+    """mrl_add_norm_bwd_workspace_bytes: a function of its arguments alone."""
+    return _lib.load().mrl_add_norm_bwd_workspace_bytes(n_rows, hidden)
+
+
 def _forward(x, weight, bias, eps, layer, keep):
     """y, and what the backward takes if `keep`: the rows, their stride, the weight, [mean and] rstd of the rows."""
     dev, hidden = x.device, x.shape[-1]
@@ -118,19 +124,150 @@ def rms_norm(x, weight, eps=1e-6):
     return _norm(x, weight, None, eps, False)
 
 
+def _added(x, residual, weight, eps):
+    """What :func:`add_rms_norm` and :func:`rms_norm_fp8` ask of their arguments."""
+    if x.dtype not in _FLOATS:
+        raise TypeError("x must be float32, bfloat16 or float16, not %s" % x.dtype)
+    if weight.dtype is not x.dtype and weight.dtype is not torch.float32:
+        raise TypeError("weight must have the type of x (%s) or float32, not %s" % (x.dtype, weight.dtype))
+    if x.dim() < 1 or x.shape[-1] < 1 or weight.dim() != 1 or weight.shape[0] != x.shape[-1]:
+        raise ValueError("weight must have the shape of x's last dimension: x %s, weight %s"
+                         % (tuple(x.shape), tuple(weight.shape)))
+    if residual is not None:
+        if residual.dtype is not x.dtype and residual.dtype is not torch.float32:
+            raise TypeError("residual must have the type of x (%s) or float32, not %s" % (x.dtype, residual.dtype))
+        if residual.shape != x.shape:
+            raise ValueError("residual must have the shape of x: %s and %s" % (tuple(residual.shape), tuple(x.shape)))
+    eps = float(eps)
+    if not 0.0 < eps < float("inf"):
+        raise ValueError("eps must be positive and finite, not %r" % eps)
+    _lib.require_device(x, residual, weight)
+    return eps
+
+
+def _add_forward(x, residual, weight, eps, keep):
+    """y, h and, if `keep`, rstd of the rows; the weight as the kernels read it."""
+    dev, hidden = x.device, x.shape[-1]
+    flat, x_stride = _flat_rows(x)
+    res, r_stride = _flat_rows(residual)
+    n_rows, w = flat.shape[0], weight.contiguous()
+    y, h = torch.empty(x.shape, dtype=x.dtype, device=dev), torch.empty(x.shape, dtype=residual.dtype, device=dev)
+    rstd = torch.empty(n_rows, dtype=torch.float32, device=dev) if keep else None
+    _lib.call("mrl_add_norm_fwd", flat.data_ptr(), _lib.dtype_code(x), x_stride, res.data_ptr(), _lib.dtype_code(h), r_stride,
+              n_rows, hidden, w.data_ptr(), _lib.dtype_code(w), eps, h.data_ptr(), y.data_ptr(), _lib.ptr(rstd), _lib.stream(dev))
+    return y, h, w, rstd
+
+
+def _add_backward(ctx, dy, dh):
+    h, w, rstd = ctx.saved_tensors
+    shape, dtype = ctx.meta
+    dev, hidden, n_rows = h.device, shape[-1], rstd.shape[0]
+    need_x, need_r, need_w = ctx.needs_input_grad[:3]
+    if dy is None:                          # nothing came back through the norm
+        dw = torch.zeros_like(w) if need_w else None
+        if dh is None:
+            return None, None, dw, None
+        return dh.to(dtype) if need_x else None, dh if need_r else None, dw, None
+    dy, dy_stride = _flat_rows(dy)
+    dh_stride = hidden
+    if dh is not None:
+        dh, dh_stride = _flat_rows(dh)
+    dx = torch.empty(shape, dtype=dtype, device=dev) if need_x else None
+    dr = torch.empty(shape, dtype=h.dtype, device=dev) if need_r and not (need_x and h.dtype is dtype) else None
+    dw = workspace = None
+    ws_bytes = 0
+    if need_w:
+        dw = torch.empty_like(w)
+        ws_bytes = _add_workspace_bytes(n_rows, hidden)
+        workspace = w.new_empty(ws_bytes, dtype=torch.uint8)
+    _lib.call("mrl_add_norm_bwd", dy.data_ptr(), dy_stride, _lib.ptr(dh), dh_stride, h.data_ptr(), _lib.dtype_code(h), _lib.dtype_code(dy),
+              n_rows, hidden, w.data_ptr(), _lib.dtype_code(w), rstd.data_ptr(), _lib.ptr(dx), _lib.ptr(dr), _lib.ptr(dw),
+              _lib.ptr(workspace), ws_bytes, _lib.stream(dev))
+    return dx, dr if dr is not None or not need_r else dx, dw, None
+
+
+_add_backward_once = once_differentiable(_add_backward)
+
+
+class _AddNorm(torch.autograd.Function):
+    """(x[..., H], residual[..., H], weight[H]) -> y, h; h itself and rstd of the rows are kept for the backward."""
+
+    @staticmethod
+    def forward(ctx, x, residual, weight, eps):
+        y, h, w, rstd = _add_forward(x, residual, weight, eps, True)
+        ctx.save_for_backward(h, w, rstd)
+        ctx.meta = (x.shape, x.dtype)
+        ctx.set_materialize_grads(False)
+        return y, h
+
+    @staticmethod
+    def backward(ctx, dy, dh):
+        return _add_backward_once(ctx, dy, dh) if torch.is_grad_enabled() else _add_backward(ctx, dy, dh)
+
+
+def add_rms_norm(x, residual, weight, eps=1e-6):
+    """``(y, h)``: the residual stream behind a layer, ``h = x + residual``, and its RMS norm ``y = h * (mean(h^2) + eps)^(-1/2) *
+    weight`` for the next one, in one pass.  ``x`` ``[..., H]`` is fp32, bf16 or fp16, ``residual`` of the same shape and of the type of
+    ``x`` or fp32 (rows of any stride), ``weight`` ``[H]`` of the type of ``x`` or fp32; ``h`` has the residual's type and ``y`` that of ``x``.
+    The norm is that of ``h`` as it is returned, so the call gives what ``rms_norm(x + residual, weight)`` gives but for the order
+    of the sums.  Differentiable (once) with respect to all three, from gradients of either output or both; the same limits
+    as :func:`layer_norm`'s, and fewer than 2^24 rows."""
+    eps = _added(x, residual, weight, eps)
+    if torch.is_grad_enabled() and (x.requires_grad or residual.requires_grad or weight.requires_grad) or _transformed():
+        return _AddNorm.apply(x, residual, weight, eps)
+    return _add_forward(x, residual, weight, eps, False)[:2]
+
+
+def rms_norm_fp8(x, weight, eps=1e-6, residual=None, block=None):
+    """``(q, scale)``: the RMS norm of ``x`` in 8 bits, for a product that takes OCP e4m3 operands: ``q`` (``torch.float8_e4m3fn``, the shape of
+    ``x``) times ``scale`` (fp32) is the norm.  ``block=None``: a scale for each row, ``[..., 1]``; ``block=128``: one for each 128 entries, ``[..., H /
+    128]`` (``H`` a multiple of 128).  ``scale`` is the largest magnitude over 448, at least 2^-126, and ``q`` is rounded to the nearest, ties to
+    even.  With ``residual`` the norm is that of ``h = x + residual`` as in :func:`add_rms_norm`, and ``(q, scale, h)`` is returned.
+    A pass without gradients: with inputs that require one it is refused."""
+    eps = _added(x, residual, weight, eps)
+    if block is not None and block != 128:
+        raise ValueError("block must be None (a scale for each row) or 128, not %r" % (block,))
+    hidden = x.shape[-1]
+    if block and hidden % block:
+        raise ValueError("rows of %d entries are not whole blocks of %d" % (hidden, block))
+    if (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad))
+            or _transformed()):
+        raise RuntimeError("rms_norm_fp8 has no gradient: call it under torch.no_grad() or with detached tensors")
+    dev = x.device
+    flat, x_stride = _flat_rows(x)
+    n_rows, w = flat.shape[0], weight.contiguous()
+    res, r_stride, h = None, hidden, None
+    if residual is not None:
+        res, r_stride = _flat_rows(residual)
+        h = torch.empty(x.shape, dtype=residual.dtype, device=dev)
+    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=dev)
+    scale = torch.empty((*x.shape[:-1], hidden // block if block else 1), dtype=torch.float32, device=dev)
+    _lib.call("mrl_norm_fp8_fwd", flat.data_ptr(), _lib.dtype_code(x), x_stride, _lib.ptr(res), _lib.dtype_code(x if res is None else res),
+              r_stride, n_rows, hidden, w.data_ptr(), _lib.dtype_code(w), eps, block or 0, _lib.ptr(h), q.data_ptr(), scale.data_ptr(),
+              _lib.stream(dev))
+    return (q, scale) if h is None else (q, scale, h)
+
+
 def final_norm(hidden, kwargs):
     """The hidden states that the lm_head takes: ``hidden`` itself, or normalised if the caller of a loss object says
-    how (``final_norm_weight=``; ``final_norm_type=`` "rms" (default) or "layer", ``final_norm_bias=``, ``final_norm_eps=``)."""
+    how (``final_norm_weight=``; ``final_norm_type=`` "rms" (default) or "layer", ``final_norm_bias=``, ``final_norm_eps=``;
+    ``final_norm_residual=``: the residual stream that the RMS norm adds the last layer's output ``hidden`` to)."""
     weight = kwargs.get("final_norm_weight")
     kind, bias = kwargs.get("final_norm_type", "rms"), kwargs.get("final_norm_bias")
+    residual = kwargs.get("final_norm_residual")
     if kind not in ("rms", "layer"):
         raise ValueError("final_norm_type must be 'rms' or 'layer', not %r" % (kind,))
     if weight is None:
         if bias is not None:
             raise ValueError("final_norm_bias= needs final_norm_weight=")
+        if residual is not None:
+            raise ValueError("final_norm_residual= needs final_norm_weight=")
         return hidden
     if kind == "rms":
         if bias is not None:
             raise ValueError("final_norm_bias= needs final_norm_type='layer'")
-        return rms_norm(hidden, weight, kwargs.get("final_norm_eps", 1e-6))
+        eps = kwargs.get("final_norm_eps", 1e-6)
+        return rms_norm(hidden, weight, eps) if residual is None else add_rms_norm(hidden, residual, weight, eps)[0]
+    if residual is not None:
+        raise ValueError("final_norm_residual= needs final_norm_type='rms'")
     return layer_norm(hidden, weight, bias, kwargs.get("final_norm_eps", 1e-5))

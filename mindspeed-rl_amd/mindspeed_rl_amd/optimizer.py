@@ -1,0 +1,143 @@
+"""The update's last step: AdamW over all parameters at once, clipped by the norm of the gradients on the way, without a wait for
+the device; moments in 32 or in 8 bits.
+
+The reference takes its optimizer from the training framework below it.  Here it works on what :func:`global_grad_norm` has seen:
+the clipped gradients are never written.
+"""
+import array
+
+import torch
+from torch.autograd.graph import increment_version
+
+from . import _lib
+
+_BLOCK = 128                # entries that share a scale
+_E4M3 = torch.float8_e4m3fn
+_CODES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+
+
+def _blocks(n):
+    return -(-n // _BLOCK)
+
+
+def adamw_state(params, bits=32, master=True):
+    """What :func:`adamw_` keeps for ``params`` from one step to the next, as its keyword arguments: ``exp_avg``, ``exp_avg_sq`` (zeros), ``step`` (an
+    int64 scalar on the device, 0), with ``bits=8`` ``exp_avg_scale`` and ``exp_avg_sq_scale``, and with ``master`` fp32 copies of the bf16 and
+    fp16 parameters (None for those of fp32).  Plain lists of tensors, which ``torch.save`` takes."""
+    params = list(params)
+    if bits not in (8, 32):
+        raise ValueError("bits must be 32 or 8, not %r" % (bits,))
+    if not params:
+        raise ValueError("no parameters")
+    _check_params(params)
+    dev = _lib.require_device(*params)
+    state = {"exp_avg": [], "exp_avg_sq": [], "step": torch.zeros((), dtype=torch.int64, device=dev)}
+    dtype = torch.float32 if bits == 32 else _E4M3
+    for name in ("exp_avg", "exp_avg_sq"):
+        state[name] = [torch.zeros(p.shape, dtype=dtype, device=dev) for p in params]
+        if bits == 8:
+            state[name + "_scale"] = [torch.full((_blocks(p.numel()),), 2.0 ** -126, device=dev) for p in params]
+    if master:
+        state["master"] = [None if p.dtype is torch.float32 else p.detach().float() for p in params]
+    return state
+
+
+def _check_params(params):
+    for p in params:
+        if not isinstance(p, torch.Tensor):
+            raise TypeError("parameters must be tensors, not %s" % type(p).__name__)
+        if p.dtype not in _CODES or p.layout is not torch.strided:
+            raise TypeError("parameters must be dense float32, bfloat16 or float16 tensors, not %s of %s" % (p.layout, p.dtype))
+        if not p.is_contiguous():
+            raise ValueError("parameters must be contiguous: a tensor of shape %s has strides %s" % (tuple(p.shape), p.stride()))
+
+
+def _check_held(name, held, p, dtype):
+    if not isinstance(held, torch.Tensor) or held.dtype is not dtype or held.shape != p.shape or not held.is_contiguous():
+        raise ValueError("%s must hold contiguous tensors of %s with the parameters' shapes" % (name, dtype))
+
+
+def adamw_(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, master=None,
+           exp_avg_scale=None, exp_avg_sq_scale=None, grad_norm=None, max_norm=None):
+    """One step of AdamW (decoupled weight decay) for every tensor of ``params``, in place:
+
+        ``m = b1 m + (1 - b1) g``, ``v = b2 v + (1 - b2) g^2``,
+        ``p = p (1 - lr weight_decay) - m / (sqrt(v) / sqrt(1 - b2^t) + eps) * lr / (1 - b1^t)``, ``t`` the number of this step
+
+    ``params``: contiguous fp32, bf16 or fp16 tensors (leaves that require gradients are meant), ``grads``: for each a gradient of the
+    same shape and of the parameter's type or fp32, or None, which leaves its parameter alone.  The others are those of :func:`adamw_state`:
+    ``adamw_(params, grads, **state, lr=...)``; parameters with another ``lr`` or ``weight_decay`` take a call and a state of their own.
+    ``master``: fp32 weights that the step is taken on; the parameter is their rounded value.  ``exp_avg_scale`` and ``exp_avg_sq_scale``
+    belong to moments in 8 bits (``torch.float8_e4m3fn``: of ``m`` and ``sqrt(v)`` over their scales, blocks of 128 entries, rounded
+    up or down by a hash of the step and the place, so that the same call gives the same bits).
+
+    ``grad_norm`` (the fp32 scalar of :func:`global_grad_norm`) and ``max_norm``: gradients are multiplied by ``min(1, max_norm / (grad_norm + 1e-6))``
+    first, as :func:`clip_grad_norm_` would have it.  ``lr`` may be an fp32 scalar on the device.  ``step`` is counted up on the device, and a
+    captured call can be replayed.  Gradients have to be finite.  Nothing that is written may share memory with anything else of the call."""
+    lists = [list(params), list(grads), list(exp_avg), list(exp_avg_sq)]
+    n = len(lists[0])
+    small = exp_avg_scale is not None or exp_avg_sq_scale is not None
+    if small and (exp_avg_scale is None or exp_avg_sq_scale is None):
+        raise ValueError("exp_avg_scale and exp_avg_sq_scale belong together")
+    lists += [list(x) if x is not None else [None] * n for x in (master, exp_avg_scale, exp_avg_sq_scale)]
+    if any(len(x) != n for x in lists):
+        raise ValueError("lists of one length are wanted: %s" % ([len(x) for x in lists],))
+    lr_at = None
+    if isinstance(lr, torch.Tensor):
+        if lr.dtype is not torch.float32 or lr.numel() != 1:
+            raise TypeError("lr must be a number or one float32 on the device, not %s %s" % (lr.dtype, tuple(lr.shape)))
+        lr_at, lr_value = lr.data_ptr(), 0.0
+    else:
+        lr_value = float(lr)
+    b1, b2 = map(float, betas)
+    eps, weight_decay = float(eps), float(weight_decay)
+    if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
+        raise ValueError("betas must lie in [0, 1): %r" % (betas,))
+    if not (0.0 <= lr_value < float("inf") and 1e-30 <= eps < float("inf") and 0.0 <= weight_decay < float("inf")):
+        raise ValueError("lr and weight_decay must not be negative, and eps at least 1e-30: %r, %r, %r" % (lr, weight_decay, eps))
+    if not isinstance(step, torch.Tensor) or step.dtype is not torch.int64 or step.numel() != 1:
+        raise TypeError("step must be one int64 on the device")
+    if (grad_norm is None) != (max_norm is None):
+        raise ValueError("grad_norm and max_norm belong together")
+    if grad_norm is not None:
+        max_norm = float(max_norm)
+        if not isinstance(grad_norm, torch.Tensor) or grad_norm.dtype is not torch.float32 or grad_norm.numel() != 1:
+            raise TypeError("grad_norm must be one float32 on the device")
+        if not max_norm >= 0.0:
+            raise ValueError("max_norm must not be negative: %r" % max_norm)
+    moments = _E4M3 if small else torch.float32
+    words, tensors, written, kept = [], [], [step], []
+    for p, g, m, v, w, ms, vs in zip(*lists):
+        _check_params((p,))
+        if g is None:
+            continue
+        if not isinstance(g, torch.Tensor) or g.layout is not torch.strided or g.shape != p.shape or (
+                g.dtype is not p.dtype and g.dtype is not torch.float32):
+            raise ValueError("a gradient must have the shape of its parameter, and its type or float32: %s %s"
+                             % (tuple(p.shape), p.dtype))
+        _check_held("exp_avg", m, p, moments)
+        _check_held("exp_avg_sq", v, p, moments)
+        if w is not None:
+            if p.dtype is torch.float32:
+                raise ValueError("a float32 parameter is its own main weight: its entry of master must be None")
+            _check_held("master", w, p, torch.float32)
+        if small:
+            for s in (ms, vs):
+                if not isinstance(s, torch.Tensor) or s.dtype is not torch.float32 or s.shape != (_blocks(p.numel()),) or not s.is_contiguous():
+                    raise ValueError("scales must be contiguous float32, one for each %d entries" % _BLOCK)
+        held = [x for x in (w, m, v, ms, vs) if x is not None]
+        if any(x.requires_grad for x in held):
+            raise ValueError("what the step keeps is part of a graph: give detached tensors")
+        tensors += (p, g, *held)
+        written += (p, *held)
+        if not g.is_contiguous():
+            g = g.detach().contiguous()
+            kept.append(g)
+        words += (p.data_ptr(), g.data_ptr(), _lib.ptr(w) or 0, m.data_ptr(), v.data_ptr(), _lib.ptr(ms) or 0, _lib.ptr(vs) or 0, p.numel(),
+                  _CODES[p.dtype] | _CODES[g.dtype] << 32)
+    dev = _lib.require_device(step, grad_norm, lr if lr_at is not None else None, *tensors)
+    table = array.array("q", words)
+    coefs = torch.empty(8, dtype=torch.float32, device=dev)
+    _lib.call("mrl_adamw_step", table.buffer_info()[0], len(words) // 9, 8 if small else 32, step.data_ptr(), lr_value, lr_at, b1, b2, eps,
+              weight_decay, _lib.ptr(grad_norm), max_norm or 0.0, coefs.data_ptr(), _lib.stream(dev))
+    increment_version(written)              # autograd looks whether what it kept has been written to
