@@ -8,12 +8,11 @@
 // gives what an addition and a norm behind it give.  Sums are held in fp32.
 #include "lane_ops.h"
 #include "mrl_internal.h"
+#include "norm_rows.h"
 #include "vector_access.h"
 #include "vocab_common.h"
 
 namespace {
-
-using mrl_vocab::Elem;
 
 constexpr int kBlock = 256;
 constexpr int kColumnSlabs = 256;           // most partial sums of a column
@@ -164,14 +163,333 @@ __global__ __launch_bounds__(kBlock) void add_norm_columns_kernel(BwdArgs a, int
     a.part[(int64_t)blockIdx.y * a.hidden + j] = dw;
 }
 
-template <int WDT>
-__global__ __launch_bounds__(kBlock) void add_norm_part_sum_kernel(const float* __restrict__ part, int n_parts, int64_t hidden,
-                                                                   typename Elem<WDT>::T* __restrict__ dweight) {
-    const int64_t j = (int64_t)blockIdx.x * kBlock + threadIdx.x;
-    if (j >= hidden) return;
-    float s = 0.f;
-    for (int g = 0; g < n_parts; ++g) s += part[(int64_t)g * hidden + j];
-    Elem<WDT>::store(dweight + j, s);
+// ------------------------------------------------------------------------------------ rows in registers
+// kN entries as they were loaded: one vector of 16 bytes, or two of a wider type than the rows'.
+template <int DT, int kN>
+struct Raw {
+    static constexpr int kVec = Elem<DT>::kVec, kParts = kN / kVec;
+    using T = typename Elem<DT>::T;
+    u32x4 v[kParts];
+    template <bool kStream>
+    __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+        for (int i = 0; i < kParts; ++i) v[i] = kStream ? mrl::Vec<DT>::load_nt(p + i * kVec) : mrl::Vec<DT>::load(p + i * kVec);
+    }
+    template <bool kStream>
+    __device__ __forceinline__ void store(T* p) const {
+#pragma unroll
+        for (int i = 0; i < kParts; ++i) {
+            if (kStream) mrl::Vec<DT>::store_nt(p + i * kVec, v[i]);
+            else mrl::Vec<DT>::store(p + i * kVec, v[i]);
+        }
+    }
+    __device__ __forceinline__ void unpack(float (&z)[kN]) const {
+#pragma unroll
+        for (int i = 0; i < kParts; ++i) {
+            float t[kVec];
+            Elem<DT>::unpack(v[i], t);
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) z[i * kVec + j] = t[j];
+        }
+    }
+    __device__ __forceinline__ void pack(const float (&z)[kN]) {
+#pragma unroll
+        for (int i = 0; i < kParts; ++i) {
+            float t[kVec];
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) t[j] = z[i * kVec + j];
+            v[i] = Elem<DT>::pack(t);
+        }
+    }
+};
+
+template <int kN>
+__device__ __forceinline__ void store_codes(uint8_t* p, const float (&z)[kN]) {
+    typedef uint32_t Words __attribute__((ext_vector_type(kN / 4)));
+    typedef Words WordsAnywhere __attribute__((aligned(1)));
+    Words c;
+#pragma unroll
+    for (int w = 0; w < kN / 4; ++w) {
+        int t = __builtin_amdgcn_cvt_pk_fp8_f32(z[4 * w], z[4 * w + 1], 0, false);
+        c[w] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(z[4 * w + 2], z[4 * w + 3], t, true);
+    }
+    *(WordsAnywhere*)p = c;
+}
+
+__device__ __forceinline__ uint32_t lanes_most(uint32_t x) {    // over 16 lanes
+    x = max(x, mrl::lane_partner_bits<0>(x));
+    x = max(x, mrl::lane_partner_bits<1>(x));
+    x = max(x, mrl::lane_partner_bits<2>(x));
+    return max(x, mrl::lane_partner_bits<3>(x));
+}
+
+// Over a team, in all of its lanes, as team_sum2.
+__device__ __forceinline__ uint32_t team_most(uint32_t x, int lanes, uint32_t* lds) {
+    x = lanes_most(x);
+    if (lanes == 16) return x;
+    x = max(x, (uint32_t)__shfl_xor((int)x, 16, 64));
+    x = max(x, (uint32_t)__shfl_xor((int)x, 32, 64));
+    if (lanes == 64) return x;
+    lds[threadIdx.x >> 6] = x;
+    __syncthreads();
+    const int waves = lanes >> 6, first = (threadIdx.x >> 6) / waves * waves, w = threadIdx.x & 15;
+    return lanes_most(w < waves ? lds[first + w] : 0u);
+}
+
+// A team a row, kVecs vectors a lane, each row read once.  The last vector of a row that is not whole vectors overlaps the one in
+// front of it; what a lane holds twice over is left out of its sums and written twice with the same bits.
+template <int DT, int RT, int WDT, int kVecs, bool kRes, bool kFp8, bool kStream>
+__global__ __launch_bounds__(1024) void add_norm_fwd_rows_kernel(FwdArgs a, int lanes) {
+    using T = typename Elem<DT>::T;
+    using R = typename Elem<RT>::T;
+    constexpr int kVec = Elem<DT>::kVec;
+    __shared__ float2 lds[16];
+    __shared__ uint32_t most_lds[16];
+    const int tl = threadIdx.x & (lanes - 1);
+    const int64_t wanted = (int64_t)blockIdx.x * (blockDim.x / lanes) + threadIdx.x / lanes;
+    const bool live = wanted < a.n_rows;
+    const int64_t row = live ? wanted : a.n_rows - 1;
+    const Columns<kVecs, kVec> col(tl, lanes, a.hidden);
+    Raw<DT, kVec> x[kVecs];
+    Raw<RT, kVec> h[kVecs];
+    Raw<WDT, kVec> w[kVecs];
+#pragma unroll
+    for (int q = 0; q < kVecs; ++q) x[q].template load<kStream>((const T*)a.x + row * a.x_stride + col.at(q));
+    if (kRes) {
+#pragma unroll
+        for (int q = 0; q < kVecs; ++q) h[q].template load<kStream>((const R*)a.residual + row * a.residual_stride + col.at(q));
+    }
+#pragma unroll
+    for (int q = 0; q < kVecs; ++q) w[q].template load<false>((const typename Elem<WDT>::T*)a.weight + col.at(q));
+    const auto value = [&](int q, float (&z)[kVec]) {
+        if (kRes) h[q].unpack(z);
+        else x[q].unpack(z);
+    };
+    float ss = 0.f;
+#pragma unroll
+    for (int q = 0; q < kVecs; ++q) {
+        float z[kVec];
+        if (kRes) {
+            float t[kVec];
+            x[q].unpack(z);
+            h[q].unpack(t);
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) z[i] += t[i];
+            h[q].pack(z);
+        }
+        value(q, z);
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) ss += col.own(q, i) ? z[i] * z[i] : 0.f;
+    }
+    const float r = 1.f / sqrtf(team_sum2(ss, 0.f, lanes, lds).x * (1.f / (float)a.hidden) + a.eps);
+    float inv = 1.f;
+    if (kFp8 && !a.block) {
+        uint32_t most = 0;
+#pragma unroll
+        for (int q = 0; q < kVecs; ++q) {
+            float z[kVec], wf[kVec];
+            value(q, z);
+            w[q].unpack(wf);
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) most = max(most, __float_as_uint(fabsf(z[i] * r * wf[i])));
+        }
+        const float s = scale_of(team_most(most, lanes, most_lds));
+        inv = 1.f / s;
+        if (live && tl == 0) a.scale[row] = s;
+    }
+    if (!live) return;
+#pragma unroll
+    for (int q = 0; q < kVecs; ++q) {
+        const int64_t at = row * a.hidden + col.at(q);
+        if (kRes) h[q].template store<kStream>((R*)a.h + at);
+        float z[kVec], wf[kVec];
+        value(q, z);
+        w[q].unpack(wf);
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) z[i] = z[i] * r * wf[i];
+        if (!kFp8) {
+            Raw<DT, kVec> y;
+            y.pack(z);
+            y.template store<kStream>((T*)a.y + at);
+            continue;
+        }
+        if (a.block) {                      // of whole blocks: 16 lanes, or 32 of fp32, a block
+            uint32_t most = 0;
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) most = max(most, __float_as_uint(fabsf(z[i])));
+            most = lanes_most(most);
+            if (kVec == 4) most = max(most, (uint32_t)__shfl_xor((int)most, 16, 64));
+            const float s = scale_of(most);
+            inv = 1.f / s;
+            if (q == kVecs - 1 && col.skip) continue;       // lanes behind the row
+            if ((tl & (128 / kVec - 1)) == 0) a.scale[at / 128] = s;
+        }
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) z[i] *= inv;
+        store_codes<kVec>((uint8_t*)a.y + at, z);
+    }
+    if (a.rstd && tl == 0) a.rstd[row] = r;
+}
+
+// The backward in one pass: workgroups stay and take rows in turn, a team a row, and hold the sums over their rows of the lane's
+// columns in registers; the workgroup's sums go to part[group][hidden].
+constexpr int kBwdBlock = 512;              // threads of a workgroup that holds several teams
+constexpr int kBwdGroups = 512;             // most workgroups: two on each of 256 CUs
+constexpr int64_t kBwdManyVecs = 4 << 20;   // 64 MiB of rows
+
+template <int DT, int RT, int WDT, int kVecs, int kBlockMost, bool kDh, bool kStream>
+__global__ __launch_bounds__(kBlockMost) void add_norm_bwd_rows_kernel(BwdArgs a, int lanes, void* __restrict__ dweight) {
+    using T = typename Elem<DT>::T;
+    using R = typename Elem<RT>::T;
+    constexpr int kVec = Elem<DT>::kVec;
+    constexpr bool kOne = kBlockMost > kBwdBlock;       // the team is the workgroup
+    constexpr bool kAhead = kVecs == 1;                 // the next row is requested before this one is summed
+    extern __shared__ float columns[];                  // [kVecs * kVec][lanes] sums on their way between teams
+    __shared__ float2 lds[2][16];
+    const int teams = kOne ? 1 : blockDim.x / lanes, team = kOne ? 0 : threadIdx.x / lanes;
+    const int tl = threadIdx.x - team * lanes, hidden = a.hidden;
+    const Columns<kVecs, kVec> col(tl, lanes, hidden);
+    const float inv = 1.f / (float)hidden;
+    float dw[kVecs][kVec] = {};
+    Raw<WDT, kVec> w[kVecs];
+#pragma unroll
+    for (int q = 0; q < kVecs; ++q) w[q].template load<false>((const typename Elem<WDT>::T*)a.weight + col.at(q));
+    const int64_t step = (int64_t)gridDim.x * teams;
+    Raw<RT, kVec> hn[kVecs], un[kVecs];
+    Raw<DT, kVec> gn[kVecs];
+    float rn;
+    const auto request = [&](int64_t wanted) {
+        const int64_t row = wanted < a.n_rows ? wanted : a.n_rows - 1;
+        rn = a.rstd[row];
+#pragma unroll
+        for (int q = 0; q < kVecs; ++q) {
+            hn[q].template load<kStream>((const R*)a.h + row * hidden + col.at(q));
+            gn[q].template load<kStream>((const T*)a.dy + row * a.dy_stride + col.at(q));
+        }
+        if (kDh) {
+#pragma unroll
+            for (int q = 0; q < kVecs; ++q) un[q].template load<kStream>((const R*)a.dh + row * a.dh_stride + col.at(q));
+        }
+    };
+    if (kAhead) request((int64_t)blockIdx.x * teams + team);
+    int turn = 0;
+    for (int64_t base = (int64_t)blockIdx.x * teams; base < a.n_rows; base += step, turn ^= 1) {
+        // teams behind the last row do that row again, without its share of the columns' sums
+        const bool counts = kOne || base + team < a.n_rows;
+        const int64_t row = counts ? base + team : a.n_rows - 1;
+        if (!kAhead) request(row);
+        Raw<RT, kVec> h[kVecs], u[kVecs];
+        Raw<DT, kVec> g[kVecs];
+#pragma unroll
+        for (int q = 0; q < kVecs; ++q) {
+            h[q] = hn[q];
+            g[q] = gn[q];
+            if (kDh) u[q] = un[q];
+        }
+        const float r = rn;
+        if (kAhead) request(base + team + step);
+        float sgn = 0.f;
+#pragma unroll
+        for (int q = 0; q < kVecs; ++q) {
+            float z[kVec], gf[kVec], wf[kVec];
+            h[q].unpack(z);
+            g[q].unpack(gf);
+            w[q].unpack(wf);
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) {
+                const float own = col.own(q, i) ? gf[i] : 0.f, n = z[i] * r;
+                dw[q][i] += (counts ? own : 0.f) * n;
+                sgn += own * wf[i] * n;
+            }
+        }
+        const float c = team_sum2(sgn, 0.f, lanes, lds[turn]).x * inv;
+#pragma unroll
+        for (int q = 0; q < kVecs; ++q) {
+            float z[kVec], gf[kVec], wf[kVec], uf[kVec] = {};
+            h[q].unpack(z);
+            g[q].unpack(gf);
+            w[q].unpack(wf);
+            if (kDh) u[q].unpack(uf);
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) z[i] = r * (gf[i] * wf[i] - z[i] * r * c) + uf[i];
+            const int64_t at = row * hidden + col.at(q);
+            if (a.dx) {
+                Raw<DT, kVec> d;
+                d.pack(z);
+                d.template store<kStream>((T*)a.dx + at);
+            }
+            if (a.dresidual) {
+                Raw<RT, kVec> d;
+                d.pack(z);
+                d.template store<kStream>((R*)a.dresidual + at);
+            }
+        }
+    }
+    if (!a.part && !dweight) return;
+    // the workgroup's sums: teams of a wavefront by lane exchange, then one after the other through LDS
+    const bool paired = !kOne && lanes < 64;
+    const int turns = paired ? blockDim.x >> 6 : teams, mine = paired ? threadIdx.x >> 6 : team;
+    const bool holds = !paired || (threadIdx.x & 63) < 16;
+    if (paired) {
+#pragma unroll
+        for (int q = 0; q < kVecs; ++q)
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) {
+                dw[q][i] += __shfl_xor(dw[q][i], 16, 64);
+                dw[q][i] += __shfl_xor(dw[q][i], 32, 64);
+            }
+    }
+    float* out = a.part ? a.part + (int64_t)blockIdx.x * hidden : nullptr;
+    typename Elem<WDT>::T* vec = (typename Elem<WDT>::T*)dweight;       // the sums themselves, of the only workgroup
+    for (int t = 0; t < turns; ++t) {
+        if (t == mine && holds) {
+#pragma unroll
+            for (int q = 0; q < kVecs; ++q)
+#pragma unroll
+                for (int i = 0; i < kVec; ++i) {
+                    float* at = columns + (q * kVec + i) * lanes + tl;          // a lane's place is the same for every team
+                    const float s = dw[q][i] + (!kOne && t > 0 ? *at : 0.f);
+                    if (t < turns - 1) *at = s;
+                    else if (col.own(q, i) && out) out[col.at(q) + i] = s;
+                    else if (col.own(q, i)) Elem<WDT>::store(vec + col.at(q) + i, s);
+                }
+        }
+        if (!kOne) __syncthreads();
+    }
+}
+
+constexpr int kMaxVecs = 4;
+
+// 16 lanes (not where 32 share a block's scale), then whole wavefronts.
+Team fwd_team_of(int dtype, int64_t hidden, int block) {
+    const int64_t nv = vectors_of(dtype, hidden);
+    if (nv == 0) return {0, 0};
+    if (nv <= 64 && !(block && dtype == MRL_F32)) return team_that_fits(nv, 16, (int)((nv + 15) / 16));
+    for (int lanes = 64; lanes <= 1024; lanes *= 2)
+        if (nv <= (int64_t)lanes * kMaxVecs) return team_that_fits(nv, lanes, (int)((nv + lanes - 1) / lanes));
+    return {0, 0};
+}
+
+Team bwd_team_of(int dtype, int64_t n_rows, int64_t hidden) {
+    const int64_t nv = vectors_of(dtype, hidden);
+    if (nv == 0) return {0, 0};
+    if (nv <= 32) return team_that_fits(nv, 16, (int)((nv + 15) / 16));
+    const bool two = nv > 256 || (nv > 128 && n_rows * nv >= kBwdManyVecs);
+    for (int vecs = two ? 2 : 1; vecs <= 2; vecs *= 2) {
+        const int64_t waves = (nv + 64 * vecs - 1) / (64 * vecs);
+        if (waves <= 16) return team_that_fits(nv, waves * 64, vecs);
+    }
+    return {0, 0};
+}
+
+// Threads and number of the backward's workgroups.
+int bwd_block(const Team& team) { return team.lanes > kBwdBlock ? team.lanes : kBwdBlock / team.lanes * team.lanes; }
+
+int bwd_groups(const Team& team, int64_t n_rows) {
+    const int teams = bwd_block(team) / team.lanes;
+    const int64_t turns = (n_rows + teams - 1) / teams, fit = team.lanes > kBwdBlock ? kBwdGroups / 2 : kBwdGroups;
+    const int64_t each = (turns + fit - 1) / fit;       // and no more workgroups than take as long
+    return (int)((turns + each - 1) / each);
 }
 
 int64_t slab_rows_of(int64_t n_rows) {
@@ -179,25 +497,88 @@ int64_t slab_rows_of(int64_t n_rows) {
     return rows < 16 ? 16 : rows;
 }
 
+// launch(weight's type) for the rows' type or fp32.
+template <int DT, typename F>
+void with_weight(int wide, F launch) {
+    if constexpr (DT == MRL_F32) launch(Int<MRL_F32>());
+    else if (wide) launch(Int<MRL_F32>());
+    else launch(Int<DT>());
+}
+
+template <typename F>
+void with_flag(bool flag, F launch) {
+    if (flag) launch(Int<1>());
+    else launch(Int<0>());
+}
+
 template <int DT, int RT>
 void launch_fwd(const FwdArgs& a, hipStream_t stream) {
-    hipLaunchKernelGGL((add_norm_fwd_kernel<DT, RT>), dim3((unsigned)a.n_rows), dim3(kBlock), 0, stream, a);
+    const Team team = fwd_team_of(DT, a.hidden, a.block);
+    if (team.lanes == 0) {
+        hipLaunchKernelGGL((add_norm_fwd_kernel<DT, RT>), dim3((unsigned)a.n_rows), dim3(kBlock), 0, stream, a);
+        return;
+    }
+    const int block = team.lanes > 256 ? team.lanes : 256, teams = block / team.lanes;
+    const bool lines = team.lanes >= 64 && a.hidden * (int64_t)sizeof(typename Elem<DT>::T) % 128 == 0;
+    const auto launch = [&](auto wdt, auto vecs, auto res, auto fp8, auto nt) {
+        hipLaunchKernelGGL((add_norm_fwd_rows_kernel<DT, RT, decltype(wdt)::value, decltype(vecs)::value, decltype(res)::value != 0,
+                                                     decltype(fp8)::value != 0, decltype(nt)::value != 0>),
+                           dim3((unsigned)((a.n_rows + teams - 1) / teams)), dim3(block), 0, stream, a, team.lanes);
+    };
+    with_weight<DT>(a.wide_weight, [&](auto wdt) {
+        with_vecs(team.vecs, [&](auto vecs) {
+            with_flag(lines, [&](auto nt) {
+                if (!a.scale) launch(wdt, vecs, Int<1>(), Int<0>(), nt);
+                else if (a.residual) launch(wdt, vecs, Int<1>(), Int<1>(), nt);
+                else if constexpr (DT == RT) launch(wdt, vecs, Int<0>(), Int<1>(), nt);
+            });
+        });
+    });
 }
 
 template <int DT, int RT>
 void launch_bwd(const BwdArgs& a, hipStream_t stream) {
+    const Team team = bwd_team_of(DT, a.n_rows, a.hidden);
+    const auto sum_parts = [&](int n_parts) {
+        with_weight<DT>(a.wide_weight, [&](auto wdt) {
+            constexpr int WDT = decltype(wdt)::value;
+            hipLaunchKernelGGL((norm_part_sum_kernel<WDT>), dim3((unsigned)((a.hidden + 31) / 32)), dim3(1024), 0, stream, a.part,
+                               (int64_t)a.hidden, n_parts, (int64_t)a.hidden, (typename Elem<WDT>::T*)a.dweight, (typename Elem<WDT>::T*)nullptr);
+        });
+    };
+    if (team.lanes > 0 && a.n_rows > 0 && (a.dx || a.dresidual)) {
+        const int groups = bwd_groups(team, a.n_rows), block = bwd_block(team);
+        const bool lines = team.lanes >= 64 && a.hidden * (int64_t)sizeof(typename Elem<DT>::T) % 128 == 0;
+        BwdArgs b = a;
+        if (!a.dweight || groups == 1) b.part = nullptr;
+        const size_t lds = a.dweight && block > team.lanes ? (size_t)team.lanes * team.vecs * Elem<DT>::kVec * 4 : 0;
+        const auto launch = [&](auto wdt, auto vecs, auto most, auto dh, auto nt) {
+            hipLaunchKernelGGL((add_norm_bwd_rows_kernel<DT, RT, decltype(wdt)::value, decltype(vecs)::value, decltype(most)::value,
+                                                         decltype(dh)::value != 0, decltype(nt)::value != 0>),
+                               dim3((unsigned)groups), dim3(block), lds, stream, b, team.lanes, groups > 1 ? nullptr : a.dweight);
+        };
+        with_weight<DT>(a.wide_weight, [&](auto wdt) {
+            with_flag(a.dh != nullptr, [&](auto dh) {
+                with_flag(lines, [&](auto nt) {
+                    if (team.vecs == 2 && team.lanes > kBwdBlock) launch(wdt, Int<2>(), Int<1024>(), dh, nt);
+                    else if (team.vecs == 2) launch(wdt, Int<2>(), Int<kBwdBlock>(), dh, nt);
+                    else if (team.lanes > kBwdBlock) launch(wdt, Int<1>(), Int<1024>(), dh, nt);
+                    else launch(wdt, Int<1>(), Int<kBwdBlock>(), dh, nt);
+                });
+            });
+        });
+        if (a.dweight && groups > 1) sum_parts(groups);
+        return;
+    }
     if ((a.dx || a.dresidual) && a.n_rows > 0)
         hipLaunchKernelGGL((add_norm_bwd_kernel<DT, RT>), dim3((unsigned)a.n_rows), dim3(kBlock), 0, stream, a);
     if (!a.dweight) return;
     const int64_t slab = slab_rows_of(a.n_rows);
     const int n_slabs = (int)((a.n_rows + slab - 1) / slab);
-    const unsigned groups = (unsigned)((a.hidden + kBlock - 1) / kBlock);
-    if (n_slabs > 0) hipLaunchKernelGGL((add_norm_columns_kernel<DT, RT>), dim3(groups, (unsigned)n_slabs), dim3(kBlock), 0, stream, a, slab);
-    if (a.wide_weight)
-        hipLaunchKernelGGL((add_norm_part_sum_kernel<MRL_F32>), dim3(groups), dim3(kBlock), 0, stream, a.part, n_slabs, a.hidden, (float*)a.dweight);
-    else
-        hipLaunchKernelGGL((add_norm_part_sum_kernel<DT>), dim3(groups), dim3(kBlock), 0, stream, a.part, n_slabs, a.hidden,
-                           (typename Elem<DT>::T*)a.dweight);
+    if (n_slabs > 0)
+        hipLaunchKernelGGL((add_norm_columns_kernel<DT, RT>), dim3((unsigned)((a.hidden + kBlock - 1) / kBlock), (unsigned)n_slabs), dim3(kBlock), 0,
+                           stream, a, slab);
+    sum_parts(n_slabs);
 }
 
 // The instance for the types of the rows and of the residual stream: the rows' type or fp32.
@@ -271,13 +652,15 @@ extern "C" int mrl_norm_fp8_fwd(const void* x, int dtype, int64_t x_stride, cons
     const int rc = check_fwd(fn, dtype, residual_dtype, weight_dtype, a, hidden);
     if (rc != MRL_OK || n_rows == 0) return rc;
     MRL_REQUIRE(scale, MRL_ERR_INVALID_ARG, "%s: NULL scale", fn);
-    dispatch(dtype, residual_dtype, a, mrl::as_stream(stream));
+    dispatch(dtype, residual ? residual_dtype : dtype, a, mrl::as_stream(stream));
     return mrl::check_launch(fn);
 }
 
 extern "C" int64_t mrl_add_norm_bwd_workspace_bytes(int64_t n_rows, int64_t hidden) {
     if (n_rows <= 0 || hidden <= 0 || n_rows > 0x7fffffffLL || !mrl::launch_fits(n_rows, kBlock) || hidden > MRL_NORM_MAX_HIDDEN) return 0;
-    return (n_rows < kColumnSlabs ? n_rows : kColumnSlabs) * hidden * 4;
+    // a sum of a column for each workgroup of the one pass or each slab of rows: neither are more than the rows
+    static_assert(kColumnSlabs <= kBwdGroups, "a place for every slab");
+    return (n_rows < kBwdGroups ? n_rows : kBwdGroups) * hidden * 4;
 }
 
 extern "C" int mrl_add_norm_bwd(const void* dy, int64_t dy_stride, const void* dh, int64_t dh_stride, const void* h,
