@@ -26,11 +26,16 @@ namespace {
 
 using mrl_vocab::Elem;
 
-constexpr int kBlock = 256;
-constexpr int kUnit = 8;                    // entries of a lane: 16 lanes a block of 128
+// A lane takes four entries, so that what a wavefront reads or writes of an fp32 tensor at a time lies together, and a workgroup
+// one chunk, after which it ends: the memory serves small workgroups that come and go best.  All of it goes past the caches.
+// us, 719 M bf16 parameters with fp32 gradients, main weights and moments (21.6 GB) / 449 M with bf16 gradients and moments in 8
+// bits (7.2 GB): 3 550 / 1 230; eight entries a lane 4 226 / 1 344, 64, 256, 512 and 1 024 threads 3 615, 3 715, 3 869, 3 860 /
+// 1 228, 1 221, 1 257, 1 330; through the caches (256 threads) 4 096 / 1 350, loads alone past them 4 060 / 1 291, stores alone 3 960 / 1 262.
+constexpr int kBlock = 128;
+constexpr int kUnit = 4;                    // entries of a lane: 32 lanes a block of 128
 constexpr int kChunk = kBlock * kUnit;      // entries of a workgroup
 constexpr int kTable = 54;                  // tensors of a launch: 4 KB of arguments
-constexpr int64_t kMostGroups = (1LL << 24) - 1;    // of a launch, which holds fewer than 2^32 threads
+constexpr int64_t kMostGroups = (1LL << 25) - 1;    // of a launch, which holds fewer than 2^32 threads
 constexpr float kMost = 448.f;              // of e4m3
 constexpr float kLeastCode = 0.001953125f;  // 2^-9
 constexpr float kLeastScale = 1.17549435e-38f;      // 2^-126
@@ -83,72 +88,73 @@ __device__ __forceinline__ uint32_t dither(uint32_t pair, uint32_t key) {
     return x ^ (x >> 16);
 }
 
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef u32x2 u32x2_anywhere __attribute__((aligned(2)));
+typedef uint32_t u32_anywhere __attribute__((aligned(1)));
+
+// A lane's entries from `at` on, of which `valid` are the tensor's; zeros behind them.
 template <int DT>
 __device__ __forceinline__ void load_unit(const void* base, int64_t at, int valid, float (&z)[kUnit]) {
     const typename Elem<DT>::T* p = (const typename Elem<DT>::T*)base + at;
-    if (valid == kUnit) {
-        mrl::load_floats<DT>(p, z);
-    } else {
+    if (valid < kUnit) {
 #pragma unroll
         for (int i = 0; i < kUnit; ++i) z[i] = i < valid ? Elem<DT>::load(p + i) : 0.f;
+    } else if constexpr (DT == MRL_F32) {
+        Elem<DT>::unpack(mrl::Vec<DT>::load_nt(p), z);
+    } else {
+        const u32x2 v = __builtin_nontemporal_load((const u32x2_anywhere*)p);
+        float t[8];
+        Elem<DT>::unpack(mrl::make_u32x4(v.x, v.y, 0u, 0u), t);
+#pragma unroll
+        for (int i = 0; i < kUnit; ++i) z[i] = t[i];
     }
 }
 
 template <int DT>
 __device__ __forceinline__ void store_unit(void* base, int64_t at, int valid, const float (&z)[kUnit]) {
-    constexpr int kVec = Elem<DT>::kVec;
     typename Elem<DT>::T* p = (typename Elem<DT>::T*)base + at;
-    if (valid == kUnit) {
-#pragma unroll
-        for (int q = 0; q < kUnit / kVec; ++q) {
-            float t[kVec];
-#pragma unroll
-            for (int i = 0; i < kVec; ++i) t[i] = z[q * kVec + i];
-            mrl::Vec<DT>::store(p + q * kVec, Elem<DT>::pack(t));
-        }
-    } else {
+    if (valid < kUnit) {
 #pragma unroll
         for (int i = 0; i < kUnit; ++i)
             if (i < valid) Elem<DT>::store(p + i, z[i]);
+    } else if constexpr (DT == MRL_F32) {
+        mrl::Vec<DT>::store_nt(p, Elem<DT>::pack(z));
+    } else {
+        const u32x2 v = {Elem<DT>::pack2(z[0], z[1]), Elem<DT>::pack2(z[2], z[3])};
+        __builtin_nontemporal_store(v, (u32x2_anywhere*)p);
     }
 }
 
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-typedef u32x2 u32x2_anywhere __attribute__((aligned(1)));
-
-__device__ __forceinline__ u32x2 load_codes(const void* base, int64_t at, int valid) {
+__device__ __forceinline__ uint32_t load_codes(const void* base, int64_t at, int valid) {
     const uint8_t* p = (const uint8_t*)base + at;
-    if (valid == kUnit) return *(const u32x2_anywhere*)p;
-    u32x2 r = {0u, 0u};
+    if (valid == kUnit) return __builtin_nontemporal_load((const u32_anywhere*)p);
+    uint32_t c = 0;
 #pragma unroll
     for (int i = 0; i < kUnit; ++i)
-        if (i < valid) r[i >> 2] |= (uint32_t)p[i] << (8 * (i & 3));
-    return r;
+        if (i < valid) c |= (uint32_t)p[i] << (8 * i);
+    return c;
 }
 
-__device__ __forceinline__ void store_codes(void* base, int64_t at, int valid, u32x2 c) {
+__device__ __forceinline__ void store_codes(void* base, int64_t at, int valid, uint32_t c) {
     uint8_t* p = (uint8_t*)base + at;
     if (valid == kUnit) {
-        *(u32x2_anywhere*)p = c;
+        __builtin_nontemporal_store(c, (u32_anywhere*)p);
         return;
     }
 #pragma unroll
     for (int i = 0; i < kUnit; ++i)
-        if (i < valid) p[i] = (uint8_t)(c[i >> 2] >> (8 * (i & 3)));
+        if (i < valid) p[i] = (uint8_t)(c >> (8 * i));
 }
 
-__device__ __forceinline__ void values_of(u32x2 c, float scale, float (&z)[kUnit]) {
-#pragma unroll
-    for (int w = 0; w < 2; ++w) {
-        const mrl_vocab::floatx2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[w], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[w], true);
-        z[4 * w] = mrl::mul_rn(lo[0], scale);
-        z[4 * w + 1] = mrl::mul_rn(lo[1], scale);
-        z[4 * w + 2] = mrl::mul_rn(hi[0], scale);
-        z[4 * w + 3] = mrl::mul_rn(hi[1], scale);
-    }
+__device__ __forceinline__ void values_of(uint32_t c, float scale, float (&z)[kUnit]) {
+    const mrl_vocab::floatx2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, true);
+    z[0] = mrl::mul_rn(lo[0], scale);
+    z[1] = mrl::mul_rn(lo[1], scale);
+    z[2] = mrl::mul_rn(hi[0], scale);
+    z[3] = mrl::mul_rn(hi[1], scale);
 }
 
-// The largest |z| of the 16 lanes of a block, by its bits: an infinity's lie above all numbers', NaN's above those.
+// The scale of the 32 lanes of a block, from the largest |z|, by its bits: an infinity's lie above all numbers', NaN's above those.
 __device__ __forceinline__ float block_scale(const float (&z)[kUnit]) {
     uint32_t most = 0;
 #pragma unroll
@@ -157,15 +163,15 @@ __device__ __forceinline__ float block_scale(const float (&z)[kUnit]) {
     most = max(most, mrl::lane_partner_bits<1>(most));
     most = max(most, mrl::lane_partner_bits<2>(most));
     most = max(most, mrl::lane_partner_bits<3>(most));
+    most = max(most, (uint32_t)__shfl_xor((int)most, 16, 64));
     const float s = mrl::mul_rn(__uint_as_float(most), 1.f / kMost);
     return s < kLeastScale ? kLeastScale : s;
 }
 
 // floor(|x| / step + u) steps of x's binade, x = z / scale: what the conversion instruction does with the dither in the upper bits.
 template <bool kRoot>
-__device__ __forceinline__ u32x2 codes_of(const float (&z)[kUnit], float scale, const uint32_t (&bits)[kUnit / 2]) {
+__device__ __forceinline__ uint32_t codes_of(const float (&z)[kUnit], float scale, const uint32_t (&bits)[kUnit / 2]) {
     const float inv = 1.f / scale;
-    u32x2 c = {0u, 0u};
     float x[kUnit];
 #pragma unroll
     for (int i = 0; i < kUnit; ++i) {
@@ -175,16 +181,12 @@ __device__ __forceinline__ u32x2 codes_of(const float (&z)[kUnit], float scale, 
         else t = t < -kMost ? -kMost : t;
         x[i] = t;
     }
-#pragma unroll
-    for (int w = 0; w < 2; ++w) {
-        int r = 0;
-        r = __builtin_amdgcn_cvt_sr_fp8_f32(x[4 * w], (int)(bits[2 * w] << 16), r, 0);
-        r = __builtin_amdgcn_cvt_sr_fp8_f32(x[4 * w + 1], (int)(bits[2 * w] & 0xffff0000u), r, 1);
-        r = __builtin_amdgcn_cvt_sr_fp8_f32(x[4 * w + 2], (int)(bits[2 * w + 1] << 16), r, 2);
-        r = __builtin_amdgcn_cvt_sr_fp8_f32(x[4 * w + 3], (int)(bits[2 * w + 1] & 0xffff0000u), r, 3);
-        c[w] = (uint32_t)r;
-    }
-    return c;
+    int c = 0;
+    c = __builtin_amdgcn_cvt_sr_fp8_f32(x[0], (int)(bits[0] << 16), c, 0);
+    c = __builtin_amdgcn_cvt_sr_fp8_f32(x[1], (int)(bits[0] & 0xffff0000u), c, 1);
+    c = __builtin_amdgcn_cvt_sr_fp8_f32(x[2], (int)(bits[1] << 16), c, 2);
+    c = __builtin_amdgcn_cvt_sr_fp8_f32(x[3], (int)(bits[1] & 0xffff0000u), c, 3);
+    return (uint32_t)c;
 }
 
 template <int PT, int GT, bool kMaster, bool kSmall>
@@ -200,14 +202,17 @@ __global__ __launch_bounds__(kBlock) void adamw_kernel(Table t, const Coefs* __r
         const int64_t at = (chunk - (part == 0 ? 0 : t.part[part - 1].end_chunk)) * kChunk + threadIdx.x * kUnit;
         const int64_t left = p.n - at;
         const int valid = left >= kUnit ? kUnit : left > 0 ? (int)left : 0;
+        // everything is on its way before any of it is waited for
         float g[kUnit], w[kUnit], m[kUnit], v[kUnit];
         load_unit<GT>(p.grad, at, valid, g);
         if (kMaster) load_unit<MRL_F32>(p.master, at, valid, w);
         else load_unit<PT>(p.param, at, valid, w);
         const int64_t block = valid > 0 ? at / 128 : 0;
         if (kSmall) {
-            values_of(load_codes(p.m, at, valid), p.m_scale[block], m);
-            values_of(load_codes(p.v, at, valid), p.v_scale[block], v);
+            const uint32_t mc = load_codes(p.m, at, valid), vc = load_codes(p.v, at, valid);
+            const float ms = p.m_scale[block], vs = p.v_scale[block];
+            values_of(mc, ms, m);
+            values_of(vc, vs, v);
 #pragma unroll
             for (int i = 0; i < kUnit; ++i) v[i] = mrl::mul_rn(v[i], v[i]);
         } else {
@@ -232,7 +237,7 @@ __global__ __launch_bounds__(kBlock) void adamw_kernel(Table t, const Coefs* __r
             const float ms = block_scale(m), vs = block_scale(root);
             store_codes(p.m, at, valid, codes_of<false>(m, ms, bits));
             store_codes(p.v, at, valid, codes_of<true>(root, vs, bits));
-            if (valid > 0 && (threadIdx.x & 15) == 0) {
+            if (valid > 0 && (threadIdx.x & 31) == 0) {
                 p.m_scale[block] = ms;
                 p.v_scale[block] = vs;
             }

@@ -126,18 +126,18 @@ def rms_norm(x, weight, eps=1e-6):
 
 def _added(x, residual, weight, eps):
     """What :func:`add_rms_norm` and :func:`rms_norm_fp8` ask of their arguments."""
-    if x.dtype not in _FLOATS:
-        raise TypeError("x must be float32, bfloat16 or float16, not %s" % x.dtype)
-    if weight.dtype is not x.dtype and weight.dtype is not torch.float32:
-        raise TypeError("weight must have the type of x (%s) or float32, not %s" % (x.dtype, weight.dtype))
-    if x.dim() < 1 or x.shape[-1] < 1 or weight.dim() != 1 or weight.shape[0] != x.shape[-1]:
-        raise ValueError("weight must have the shape of x's last dimension: x %s, weight %s"
-                         % (tuple(x.shape), tuple(weight.shape)))
+    dtype, shape = x.dtype, x.shape
+    if dtype not in _FLOATS:
+        raise TypeError("x must be float32, bfloat16 or float16, not %s" % dtype)
+    if weight.dtype is not dtype and weight.dtype is not torch.float32:
+        raise TypeError("weight must have the type of x (%s) or float32, not %s" % (dtype, weight.dtype))
+    if len(shape) < 1 or shape[-1] < 1 or weight.dim() != 1 or weight.shape[0] != shape[-1]:
+        raise ValueError("weight must have the shape of x's last dimension: x %s, weight %s" % (tuple(shape), tuple(weight.shape)))
     if residual is not None:
-        if residual.dtype is not x.dtype and residual.dtype is not torch.float32:
-            raise TypeError("residual must have the type of x (%s) or float32, not %s" % (x.dtype, residual.dtype))
-        if residual.shape != x.shape:
-            raise ValueError("residual must have the shape of x: %s and %s" % (tuple(residual.shape), tuple(x.shape)))
+        if residual.dtype is not dtype and residual.dtype is not torch.float32:
+            raise TypeError("residual must have the type of x (%s) or float32, not %s" % (dtype, residual.dtype))
+        if residual.shape != shape:
+            raise ValueError("residual must have the shape of x: %s and %s" % (tuple(residual.shape), tuple(shape)))
     eps = float(eps)
     if not 0.0 < eps < float("inf"):
         raise ValueError("eps must be positive and finite, not %r" % eps)
@@ -145,14 +145,20 @@ def _added(x, residual, weight, eps):
     return eps
 
 
+def _rows(x, hidden):
+    """The rows of ``x``, how many, their stride, and memory for as many dense ones."""
+    if x.is_contiguous():
+        return x, x.numel() // hidden, hidden, torch.empty_like(x)
+    flat, stride = _flat_rows(x)
+    return flat, flat.shape[0], stride, torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
 def _add_forward(x, residual, weight, eps, keep):
     """y, h and, if `keep`, rstd of the rows; the weight as the kernels read it."""
-    dev, hidden = x.device, x.shape[-1]
-    flat, x_stride = _flat_rows(x)
-    res, r_stride = _flat_rows(residual)
-    n_rows, w = flat.shape[0], weight.contiguous()
-    y, h = torch.empty(x.shape, dtype=x.dtype, device=dev), torch.empty(x.shape, dtype=residual.dtype, device=dev)
-    rstd = torch.empty(n_rows, dtype=torch.float32, device=dev) if keep else None
+    dev, hidden, w = x.device, x.shape[-1], weight.contiguous()
+    flat, n_rows, x_stride, y = _rows(x, hidden)
+    res, _, r_stride, h = _rows(residual, hidden)
+    rstd = w.new_empty(n_rows, dtype=torch.float32) if keep else None
     _lib.call("mrl_add_norm_fwd", flat.data_ptr(), _lib.dtype_code(x), x_stride, res.data_ptr(), _lib.dtype_code(h), r_stride,
               n_rows, hidden, w.data_ptr(), _lib.dtype_code(w), eps, h.data_ptr(), y.data_ptr(), _lib.ptr(rstd), _lib.stream(dev))
     return y, h, w, rstd
@@ -168,12 +174,13 @@ def _add_backward(ctx, dy, dh):
         if dh is None:
             return None, None, dw, None
         return dh.to(dtype) if need_x else None, dh if need_r else None, dw, None
-    dy, dy_stride = _flat_rows(dy)
-    dh_stride = hidden
-    if dh is not None:
+    dy_stride = dh_stride = hidden
+    if not dy.is_contiguous():
+        dy, dy_stride = _flat_rows(dy)
+    if dh is not None and not dh.is_contiguous():
         dh, dh_stride = _flat_rows(dh)
     dx = torch.empty(shape, dtype=dtype, device=dev) if need_x else None
-    dr = torch.empty(shape, dtype=h.dtype, device=dev) if need_r and not (need_x and h.dtype is dtype) else None
+    dr = torch.empty_like(h) if need_r and not (need_x and h.dtype is dtype) else None
     dw = workspace = None
     ws_bytes = 0
     if need_w:
@@ -233,13 +240,13 @@ def rms_norm_fp8(x, weight, eps=1e-6, residual=None, block=None):
     if (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad))
             or _transformed()):
         raise RuntimeError("rms_norm_fp8 has no gradient: call it under torch.no_grad() or with detached tensors")
-    dev = x.device
-    flat, x_stride = _flat_rows(x)
-    n_rows, w = flat.shape[0], weight.contiguous()
+    dev, w, x_stride = x.device, weight.contiguous(), hidden
+    flat, n_rows = x, x.numel() // hidden
+    if not x.is_contiguous():
+        flat, x_stride = _flat_rows(x)
     res, r_stride, h = None, hidden, None
     if residual is not None:
-        res, r_stride = _flat_rows(residual)
-        h = torch.empty(x.shape, dtype=residual.dtype, device=dev)
+        res, _, r_stride, h = _rows(residual, hidden)
     q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=dev)
     scale = torch.empty((*x.shape[:-1], hidden // block if block else 1), dtype=torch.float32, device=dev)
     _lib.call("mrl_norm_fp8_fwd", flat.data_ptr(), _lib.dtype_code(x), x_stride, _lib.ptr(res), _lib.dtype_code(x if res is None else res),

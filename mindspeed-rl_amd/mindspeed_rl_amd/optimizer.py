@@ -5,6 +5,8 @@ The reference takes its optimizer from the training framework below it.  Here it
 the clipped gradients are never written.
 """
 import array
+import itertools
+import operator
 
 import torch
 from torch.autograd.graph import increment_version
@@ -14,6 +16,11 @@ from . import _lib
 _BLOCK = 128                # entries that share a scale
 _E4M3 = torch.float8_e4m3fn
 _CODES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+
+
+# what every tensor of a list is asked: the host's time is what a short list takes
+_DATA_PTR, _NUMEL, _CONTIGUOUS, _GET_DEVICE = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous, torch.Tensor.get_device
+_DTYPE, _SHAPE, _REQUIRES_GRAD = map(operator.attrgetter, ("dtype", "shape", "requires_grad"))
 
 
 def _blocks(n):
@@ -52,9 +59,21 @@ def _check_params(params):
             raise ValueError("parameters must be contiguous: a tensor of shape %s has strides %s" % (tuple(p.shape), p.stride()))
 
 
-def _check_held(name, held, p, dtype):
-    if not isinstance(held, torch.Tensor) or held.dtype is not dtype or held.shape != p.shape or not held.is_contiguous():
+def _check_held(name, held, shapes, dtype):
+    """What the step keeps: tensors of `dtype` and the parameters' shapes, as they lie in memory."""
+    if set(map(type, held)) - {torch.Tensor, torch.nn.Parameter} or set(map(_DTYPE, held)) - {dtype} or [*map(_SHAPE, held)] != shapes or (
+            False in map(_CONTIGUOUS, held)):
         raise ValueError("%s must hold contiguous tensors of %s with the parameters' shapes" % (name, dtype))
+    if True in map(_REQUIRES_GRAD, held):
+        raise ValueError("what the step keeps is part of a graph: give detached tensors")
+
+
+def _check_grads(params, grads):
+    for p, g in zip(params, grads):
+        if not isinstance(g, torch.Tensor) or g.layout is not torch.strided or g.shape != p.shape or (
+                g.dtype is not p.dtype and g.dtype is not torch.float32):
+            raise ValueError("a gradient must have the shape of its parameter, and its type or float32: %s %s"
+                             % (tuple(p.shape), p.dtype))
 
 
 def adamw_(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, master=None,
@@ -74,13 +93,13 @@ def adamw_(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999), eps
     ``grad_norm`` (the fp32 scalar of :func:`global_grad_norm`) and ``max_norm``: gradients are multiplied by ``min(1, max_norm / (grad_norm + 1e-6))``
     first, as :func:`clip_grad_norm_` would have it.  ``lr`` may be an fp32 scalar on the device.  ``step`` is counted up on the device, and a
     captured call can be replayed.  Gradients have to be finite.  Nothing that is written may share memory with anything else of the call."""
-    lists = [list(params), list(grads), list(exp_avg), list(exp_avg_sq)]
-    n = len(lists[0])
+    params, grads, exp_avg, exp_avg_sq = list(params), list(grads), list(exp_avg), list(exp_avg_sq)
     small = exp_avg_scale is not None or exp_avg_sq_scale is not None
     if small and (exp_avg_scale is None or exp_avg_sq_scale is None):
         raise ValueError("exp_avg_scale and exp_avg_sq_scale belong together")
-    lists += [list(x) if x is not None else [None] * n for x in (master, exp_avg_scale, exp_avg_sq_scale)]
-    if any(len(x) != n for x in lists):
+    lists = [params, grads, exp_avg, exp_avg_sq]
+    lists += [list(x) for x in (master, exp_avg_scale, exp_avg_sq_scale) if x is not None]
+    if len(set(map(len, lists))) != 1:
         raise ValueError("lists of one length are wanted: %s" % ([len(x) for x in lists],))
     lr_at = None
     if isinstance(lr, torch.Tensor):
@@ -105,39 +124,45 @@ def adamw_(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999), eps
             raise TypeError("grad_norm must be one float32 on the device")
         if not max_norm >= 0.0:
             raise ValueError("max_norm must not be negative: %r" % max_norm)
-    moments = _E4M3 if small else torch.float32
-    words, tensors, written, kept = [], [], [step], []
-    for p, g, m, v, w, ms, vs in zip(*lists):
-        _check_params((p,))
-        if g is None:
-            continue
-        if not isinstance(g, torch.Tensor) or g.layout is not torch.strided or g.shape != p.shape or (
-                g.dtype is not p.dtype and g.dtype is not torch.float32):
-            raise ValueError("a gradient must have the shape of its parameter, and its type or float32: %s %s"
-                             % (tuple(p.shape), p.dtype))
-        _check_held("exp_avg", m, p, moments)
-        _check_held("exp_avg_sq", v, p, moments)
-        if w is not None:
-            if p.dtype is torch.float32:
-                raise ValueError("a float32 parameter is its own main weight: its entry of master must be None")
-            _check_held("master", w, p, torch.float32)
-        if small:
-            for s in (ms, vs):
-                if not isinstance(s, torch.Tensor) or s.dtype is not torch.float32 or s.shape != (_blocks(p.numel()),) or not s.is_contiguous():
-                    raise ValueError("scales must be contiguous float32, one for each %d entries" % _BLOCK)
-        held = [x for x in (w, m, v, ms, vs) if x is not None]
-        if any(x.requires_grad for x in held):
-            raise ValueError("what the step keeps is part of a graph: give detached tensors")
-        tensors += (p, g, *held)
-        written += (p, *held)
-        if not g.is_contiguous():
-            g = g.detach().contiguous()
-            kept.append(g)
-        words += (p.data_ptr(), g.data_ptr(), _lib.ptr(w) or 0, m.data_ptr(), v.data_ptr(), _lib.ptr(ms) or 0, _lib.ptr(vs) or 0, p.numel(),
-                  _CODES[p.dtype] | _CODES[g.dtype] << 32)
-    dev = _lib.require_device(step, grad_norm, lr if lr_at is not None else None, *tensors)
-    table = array.array("q", words)
+    _check_params(params)
+    if any(g is None for g in grads):
+        kept = [k for k, g in enumerate(grads) if g is not None]
+        lists = [[x[k] for k in kept] for x in lists]
+        params, grads = lists[:2]
+    held = lists[2:4]
+    shapes = [*map(_SHAPE, params)]
+    _check_grads(params, grads)
+    for name, x in zip(("exp_avg", "exp_avg_sq"), held):
+        _check_held(name, x, shapes, _E4M3 if small else torch.float32)
+    sizes = [*map(_NUMEL, params)]
+    columns = [[*map(_DATA_PTR, params)], None, itertools.repeat(0), *([*map(_DATA_PTR, x)] for x in held)]
+    if master is not None:
+        main = lists[4]
+        if any(w is not None and p.dtype is torch.float32 for w, p in zip(main, params)):
+            raise ValueError("a float32 parameter is its own main weight: its entry of master must be None")
+        there = [k for k, w in enumerate(main) if w is not None]
+        only = [main[k] for k in there]
+        _check_held("master", only, [shapes[k] for k in there], torch.float32)
+        columns[2] = [0 if w is None else w.data_ptr() for w in main]
+        held = [*held, only]
+    if small:
+        counts = [torch.Size((_blocks(n),)) for n in sizes]
+        for name, x in zip(("exp_avg_scale", "exp_avg_sq_scale"), lists[-2:]):
+            _check_held(name, x, counts, torch.float32)
+            columns.append([*map(_DATA_PTR, x)])
+        held = [*held, *lists[-2:]]
+    else:
+        columns += [itertools.repeat(0)] * 2
+    codes = [_CODES[p.dtype] | _CODES[g.dtype] << 32 for p, g in zip(params, grads)]
+    written = [step, *params, *itertools.chain.from_iterable(held)]
+    devices = set(map(_GET_DEVICE, itertools.chain(written, grads)))
+    if len(devices) != 1 or -1 in devices:
+        _lib.require_device(*written, *grads)       # raises
+    dev = _lib.require_device(step, grad_norm, lr if lr_at is not None else None)
+    dense = grads if False not in map(_CONTIGUOUS, grads) else [g.detach().contiguous() for g in grads]
+    columns[1] = [*map(_DATA_PTR, dense)]
+    table = array.array("q", itertools.chain.from_iterable(zip(*columns, sizes, codes)))
     coefs = torch.empty(8, dtype=torch.float32, device=dev)
-    _lib.call("mrl_adamw_step", table.buffer_info()[0], len(words) // 9, 8 if small else 32, step.data_ptr(), lr_value, lr_at, b1, b2, eps,
+    _lib.call("mrl_adamw_step", table.buffer_info()[0], len(sizes), 8 if small else 32, step.data_ptr(), lr_value, lr_at, b1, b2, eps,
               weight_decay, _lib.ptr(grad_norm), max_norm or 0.0, coefs.data_ptr(), _lib.stream(dev))
     increment_version(written)              # autograd looks whether what it kept has been written to

@@ -1,6 +1,7 @@
 """Rotary positions of queries and keys: the position ids that :func:`preprocess_packed_seqs` hands out (or a batch's, or those of
 single tokens) turn pairs of entries of every head.  The reference leaves them to the model below it.
 """
+import array
 import ctypes
 import math
 
@@ -23,19 +24,22 @@ def _turn(xs, positions, inv_freq, interleaved, start, scale, back):
     """The turned tensors of `xs`, dense."""
     # copies live until the launch: the next one may not take their memory
     xs = [x.contiguous() if x.stride(-1) != 1 and x.shape[-1] > 1 else x for x in xs]
-    sides, outs = [], []
+    words, outs = [], []
     for x in xs:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        outer, inner, head = x.stride()[:-1] if x.dim() == 4 else (0, *x.stride()[:-1])
-        dim = x.shape[-1]
-        sides.append(RotarySide(x.data_ptr(), out.data_ptr(), x.shape[-2], dim, start if start >= 0 else dim + start, outer, inner, head))
+        shape, dev = x.shape, x.device
+        out = torch.empty(shape, dtype=x.dtype, device=dev)
+        *lead, heads, dim = shape
+        *apart, head, _ = x.stride()
+        if len(apart) == 1:
+            lead, apart = (1, *lead), (0, *apart)
+        words += (x.data_ptr(), out.data_ptr(), heads, dim, start if start >= 0 else dim + start, *apart, head)
         outs.append(out)
-    x = xs[0]
-    n_outer, n_inner = x.shape[:2] if x.dim() == 4 else (1, x.shape[0])
-    pos_outer, pos_inner = positions.stride() if x.dim() == 4 else (0, positions.stride(0))
-    _lib.call("mrl_rotary", ctypes.addressof(sides[0]), ctypes.addressof(sides[1]) if len(sides) > 1 else None, _lib.dtype_code(x),
-              positions.data_ptr(), _lib.dtype_code(positions), pos_outer, pos_inner, n_outer, n_inner, inv_freq.data_ptr(),
-              2 * inv_freq.shape[0], interleaved, scale, back, _lib.stream(x.device))
+    pos = positions.stride()
+    sides = array.array("q", words)         # struct mrl_rotary_side, one or two
+    at = sides.buffer_info()[0]
+    _lib.call("mrl_rotary", at, at + 64 if len(xs) > 1 else None, _lib.dtype_code(out), positions.data_ptr(), _lib.dtype_code(positions),
+              pos[0] if len(pos) > 1 else 0, pos[-1], *lead, inv_freq.data_ptr(), 2 * inv_freq.shape[0], interleaved, scale, back,
+              _lib.stream(dev))
     return outs
 
 
@@ -79,41 +83,41 @@ def rotary(q, k, position_ids, inv_freq, interleaved=False, start=0, scale=1.0):
     bits.  ``part`` entries of a head from ``start`` on (from its end, if negative) are turned, entries ``i`` and ``i + part / 2`` of them
     or, with ``interleaved``, ``2 i`` and ``2 i + 1``; the others are copied.  Results are dense; entries are turned in fp32 and rounded once.
     Differentiable (once) with respect to ``q`` and ``k``."""
-    for name, x in (("q", q), ("k", k)):
-        if x is None and name == "k":
-            continue
-        if x.dtype not in _FLOATS or x.dtype is not q.dtype:
-            raise TypeError("%s must be float32, bfloat16 or float16, and of one type with q: %s" % (name, x.dtype))
-        if x.dim() not in (3, 4) or x.dim() != q.dim() or x.shape[:-2] != q.shape[:-2] or x.shape[-2] < 1:
-            raise ValueError("%s must be [tokens, heads, dim] or [batch, tokens, heads, dim], of one batch with q: %s and %s"
-                             % (name, tuple(x.shape), tuple(q.shape)))
-    if inv_freq.dim() != 1 or inv_freq.shape[0] < 1 or inv_freq.dtype not in (torch.float64, torch.float32):
-        raise TypeError("inv_freq must be float64 or float32 of one dimension, not %s %s" % (inv_freq.dtype, tuple(inv_freq.shape)))
-    part = 2 * inv_freq.shape[0]
+    dtype, lead = q.dtype, q.shape[:-2]
+    part = 2 * inv_freq.numel()
     start, scale = int(start), float(scale)
-    for name, x in (("q", q), ("k", k)):
-        if x is not None:
-            begin = start if start >= 0 else x.shape[-1] + start
-            if begin < 0 or begin + part > x.shape[-1]:
-                raise ValueError("%s: %d entries from %d on are not in a head of %d" % (name, part, start, x.shape[-1]))
+    if inv_freq.dim() != 1 or part < 2 or inv_freq.dtype not in (torch.float64, torch.float32):
+        raise TypeError("inv_freq must be float64 or float32 of one dimension, not %s %s" % (inv_freq.dtype, tuple(inv_freq.shape)))
+    for name, x in (("q", q), ("k", k)) if k is not None else (("q", q),):
+        shape = x.shape
+        if dtype not in _FLOATS or x.dtype is not dtype:
+            raise TypeError("%s must be float32, bfloat16 or float16, and of one type with q: %s" % (name, x.dtype))
+        if len(shape) not in (3, 4) or shape[:-2] != lead or shape[-2] < 1:
+            raise ValueError("%s must be [tokens, heads, dim] or [batch, tokens, heads, dim], of one batch with q: %s and %s"
+                             % (name, tuple(shape), tuple(q.shape)))
+        begin = start if start >= 0 else shape[-1] + start
+        if begin < 0 or begin + part > shape[-1]:
+            raise ValueError("%s: %d entries from %d on are not in a head of %d" % (name, part, start, shape[-1]))
     if not math.isfinite(scale):
         raise ValueError("scale must be finite, not %r" % scale)
     if position_ids.dtype not in (torch.int64, torch.int32):
         raise TypeError("position_ids must be int64 or int32, not %s" % position_ids.dtype)
-    lead = q.shape[:-2]
-    if position_ids.dim() == 2 and q.dim() == 3 and position_ids.shape[0] == 1:
-        position_ids = position_ids[0]
-    if position_ids.dim() not in (1, len(lead)) or position_ids.shape[-1] != lead[-1] or (
-            position_ids.dim() == 2 and position_ids.shape[0] not in (1, lead[0])):
-        raise ValueError("position_ids must be [tokens] or [batch, tokens] of q: %s and %s" % (tuple(position_ids.shape), tuple(q.shape)))
+    if position_ids.shape != lead:
+        if position_ids.dim() == 2 and len(lead) == 1 and position_ids.shape[0] == 1:
+            position_ids = position_ids[0]
+        if position_ids.dim() not in (1, len(lead)) or position_ids.shape[-1] != lead[-1] or (
+                position_ids.dim() == 2 and position_ids.shape[0] not in (1, lead[0])):
+            raise ValueError("position_ids must be [tokens] or [batch, tokens] of q: %s and %s" % (tuple(position_ids.shape), tuple(q.shape)))
+        position_ids = position_ids.expand(lead)
     _lib.require_device(q, k, position_ids, inv_freq)
     if inv_freq.requires_grad:
         raise ValueError("inv_freq is not differentiable here: detach it")
-    positions = position_ids.expand(lead)
-    inv_freq = inv_freq.to(torch.float64).contiguous()
+    if inv_freq.dtype is not torch.float64 or not inv_freq.is_contiguous():
+        inv_freq = inv_freq.to(torch.float64).contiguous()
+    interleaved = bool(interleaved)
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)) or _transformed():
-        return _Rotary.apply(q, k, positions, inv_freq, bool(interleaved), start, scale)
-    outs = _turn([q] if k is None else [q, k], positions, inv_freq, bool(interleaved), start, scale, False)
+        return _Rotary.apply(q, k, position_ids, inv_freq, interleaved, start, scale)
+    outs = _turn([q] if k is None else [q, k], position_ids, inv_freq, interleaved, start, scale, False)
     return (outs[0], outs[1] if k is not None else None)
 
 
