@@ -247,8 +247,8 @@ def rms_norm_fp8(x, weight, eps=1e-6, residual=None, block=None):
     res, r_stride, h = None, hidden, None
     if residual is not None:
         res, _, r_stride, h = _rows(residual, hidden)
-    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=dev)
-    scale = torch.empty((*x.shape[:-1], hidden // block if block else 1), dtype=torch.float32, device=dev)
+    q = x.new_empty(x.shape, dtype=torch.float8_e4m3fn)
+    scale = x.new_empty((*x.shape[:-1], hidden // block if block else 1), dtype=torch.float32)
     _lib.call("mrl_norm_fp8_fwd", flat.data_ptr(), _lib.dtype_code(x), x_stride, _lib.ptr(res), _lib.dtype_code(x if res is None else res),
               r_stride, n_rows, hidden, w.data_ptr(), _lib.dtype_code(w), eps, block or 0, _lib.ptr(h), q.data_ptr(), scale.data_ptr(),
               _lib.stream(dev))

@@ -20,7 +20,11 @@ _CODES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _li
 
 # what every tensor of a list is asked: the host's time is what a short list takes
 _DATA_PTR, _NUMEL, _CONTIGUOUS, _GET_DEVICE = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous, torch.Tensor.get_device
-_DTYPE, _SHAPE, _REQUIRES_GRAD = map(operator.attrgetter, ("dtype", "shape", "requires_grad"))
+_DTYPE, _SHAPE, _LAYOUT, _REQUIRES_GRAD = map(operator.attrgetter, ("dtype", "shape", "layout", "requires_grad"))
+
+
+def _is_tensor(t):
+    return isinstance(t, torch.Tensor)
 
 
 def _blocks(n):
@@ -50,30 +54,34 @@ def adamw_state(params, bits=32, master=True):
 
 
 def _check_params(params):
-    for p in params:
-        if not isinstance(p, torch.Tensor):
-            raise TypeError("parameters must be tensors, not %s" % type(p).__name__)
-        if p.dtype not in _CODES or p.layout is not torch.strided:
-            raise TypeError("parameters must be dense float32, bfloat16 or float16 tensors, not %s of %s" % (p.layout, p.dtype))
-        if not p.is_contiguous():
-            raise ValueError("parameters must be contiguous: a tensor of shape %s has strides %s" % (tuple(p.shape), p.stride()))
+    """Their shapes and types."""
+    if not all(map(_is_tensor, params)):
+        raise TypeError("parameters must be tensors, not %s" % [type(p).__name__ for p in params if not _is_tensor(p)][0])
+    dtypes = [*map(_DTYPE, params)]
+    if not _CODES.keys() >= set(dtypes) or {*map(_LAYOUT, params)} - {torch.strided}:
+        raise TypeError("parameters must be dense float32, bfloat16 or float16 tensors")
+    shapes = [*map(_SHAPE, params)]
+    if False in map(_CONTIGUOUS, params):
+        raise ValueError("parameters must be contiguous: of the shapes %s not all are" % [tuple(s) for s in shapes])
+    return shapes, dtypes
 
 
 def _check_held(name, held, shapes, dtype):
     """What the step keeps: tensors of `dtype` and the parameters' shapes, as they lie in memory."""
-    if set(map(type, held)) - {torch.Tensor, torch.nn.Parameter} or set(map(_DTYPE, held)) - {dtype} or [*map(_SHAPE, held)] != shapes or (
-            False in map(_CONTIGUOUS, held)):
+    if not all(map(_is_tensor, held)) or {*map(_DTYPE, held)} - {dtype} or [*map(_SHAPE, held)] != shapes or False in map(_CONTIGUOUS, held):
         raise ValueError("%s must hold contiguous tensors of %s with the parameters' shapes" % (name, dtype))
     if True in map(_REQUIRES_GRAD, held):
         raise ValueError("what the step keeps is part of a graph: give detached tensors")
 
 
-def _check_grads(params, grads):
-    for p, g in zip(params, grads):
-        if not isinstance(g, torch.Tensor) or g.layout is not torch.strided or g.shape != p.shape or (
-                g.dtype is not p.dtype and g.dtype is not torch.float32):
-            raise ValueError("a gradient must have the shape of its parameter, and its type or float32: %s %s"
-                             % (tuple(p.shape), p.dtype))
+def _check_grads(grads, shapes, dtypes):
+    """Their types."""
+    if not all(map(_is_tensor, grads)) or {*map(_LAYOUT, grads)} - {torch.strided}:
+        raise ValueError("gradients must be dense tensors")
+    types = [*map(_DTYPE, grads)]
+    if [*map(_SHAPE, grads)] != shapes or (types != dtypes and any(g is not p and g is not torch.float32 for g, p in zip(types, dtypes))):
+        raise ValueError("a gradient must have the shape of its parameter, and its type or float32")
+    return types
 
 
 def adamw_(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, master=None,
@@ -124,21 +132,21 @@ def adamw_(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999), eps
             raise TypeError("grad_norm must be one float32 on the device")
         if not max_norm >= 0.0:
             raise ValueError("max_norm must not be negative: %r" % max_norm)
-    _check_params(params)
+    shapes, dtypes = _check_params(params)
     if any(g is None for g in grads):
         kept = [k for k, g in enumerate(grads) if g is not None]
         lists = [[x[k] for k in kept] for x in lists]
         params, grads = lists[:2]
+        shapes, dtypes = [shapes[k] for k in kept], [dtypes[k] for k in kept]
     held = lists[2:4]
-    shapes = [*map(_SHAPE, params)]
-    _check_grads(params, grads)
+    types = _check_grads(grads, shapes, dtypes)
     for name, x in zip(("exp_avg", "exp_avg_sq"), held):
         _check_held(name, x, shapes, _E4M3 if small else torch.float32)
     sizes = [*map(_NUMEL, params)]
     columns = [[*map(_DATA_PTR, params)], None, itertools.repeat(0), *([*map(_DATA_PTR, x)] for x in held)]
     if master is not None:
         main = lists[4]
-        if any(w is not None and p.dtype is torch.float32 for w, p in zip(main, params)):
+        if any(w is not None and p is torch.float32 for w, p in zip(main, dtypes)):
             raise ValueError("a float32 parameter is its own main weight: its entry of master must be None")
         there = [k for k, w in enumerate(main) if w is not None]
         only = [main[k] for k in there]
@@ -153,7 +161,7 @@ def adamw_(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999), eps
         held = [*held, *lists[-2:]]
     else:
         columns += [itertools.repeat(0)] * 2
-    codes = [_CODES[p.dtype] | _CODES[g.dtype] << 32 for p, g in zip(params, grads)]
+    codes = [_CODES[p] | _CODES[g] << 32 for p, g in zip(dtypes, types)]
     written = [step, *params, *itertools.chain.from_iterable(held)]
     devices = set(map(_GET_DEVICE, itertools.chain(written, grads)))
     if len(devices) != 1 or -1 in devices:

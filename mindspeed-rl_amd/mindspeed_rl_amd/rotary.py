@@ -26,8 +26,8 @@ def _turn(xs, positions, inv_freq, interleaved, start, scale, back):
     xs = [x.contiguous() if x.stride(-1) != 1 and x.shape[-1] > 1 else x for x in xs]
     words, outs = [], []
     for x in xs:
-        shape, dev = x.shape, x.device
-        out = torch.empty(shape, dtype=x.dtype, device=dev)
+        shape = x.shape
+        out = x.new_empty(shape)
         *lead, heads, dim = shape
         *apart, head, _ = x.stride()
         if len(apart) == 1:
@@ -39,7 +39,7 @@ def _turn(xs, positions, inv_freq, interleaved, start, scale, back):
     at = sides.buffer_info()[0]
     _lib.call("mrl_rotary", at, at + 64 if len(xs) > 1 else None, _lib.dtype_code(out), positions.data_ptr(), _lib.dtype_code(positions),
               pos[0] if len(pos) > 1 else 0, pos[-1], *lead, inv_freq.data_ptr(), 2 * inv_freq.shape[0], interleaved, scale, back,
-              _lib.stream(dev))
+              _lib.stream(out.device))
     return outs
 
 
