@@ -6,6 +6,11 @@
 //
 // What is normalised is h as it is stored: the next layer's residual, this norm and its backward see one value, and the call
 // gives what an addition and a norm behind it give.  Sums are held in fp32.
+//
+// Both passes are bound by memory: the forward reads two tensors and writes two, the backward reads three and writes one (two, where the
+// stream is wider than the rows).  32 768 x 4 096 bf16: forward 171 us (6.3 TB/s), backward with the weight's gradient 177 (6.1), to e4m3 by
+// rows 153, by blocks 158 (6.0); 32 768 x 3 584 bf16 beside an fp32 stream 227 (6.2) and 310 (6.1), to e4m3 209.  (Here and below: calls that
+// follow each other in a replayed graph.)
 #include "lane_ops.h"
 #include "mrl_internal.h"
 #include "norm_rows.h"
@@ -164,40 +169,57 @@ __global__ __launch_bounds__(kBlock) void add_norm_columns_kernel(BwdArgs a, int
 }
 
 // ------------------------------------------------------------------------------------ rows in registers
-// kN entries as they were loaded: one vector of 16 bytes, or two of a wider type than the rows'.
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef u32x2 u32x2_anywhere __attribute__((aligned(2)));
+
+// kN entries as they were loaded: a vector of 16 bytes, half of one beside a wider stream, or two of an fp32 weight.
 template <int DT, int kN>
 struct Raw {
     static constexpr int kVec = Elem<DT>::kVec, kParts = kN / kVec;
+    static constexpr bool kHalf = kN < kVec;
     using T = typename Elem<DT>::T;
-    u32x4 v[kParts];
+    u32x4 v[kHalf ? 1 : kParts];
     template <bool kStream>
     __device__ __forceinline__ void load(const T* p) {
+        if constexpr (kHalf) {
+            const u32x2_anywhere* from = (const u32x2_anywhere*)p;
+            const u32x2 t = kStream ? __builtin_nontemporal_load(from) : *from;
+            v[0] = mrl::make_u32x4(t.x, t.y, 0u, 0u);
+        } else {
 #pragma unroll
-        for (int i = 0; i < kParts; ++i) v[i] = kStream ? mrl::Vec<DT>::load_nt(p + i * kVec) : mrl::Vec<DT>::load(p + i * kVec);
+            for (int i = 0; i < kParts; ++i) v[i] = kStream ? mrl::Vec<DT>::load_nt(p + i * kVec) : mrl::Vec<DT>::load(p + i * kVec);
+        }
     }
     template <bool kStream>
     __device__ __forceinline__ void store(T* p) const {
+        if constexpr (kHalf) {
+            u32x2_anywhere* to = (u32x2_anywhere*)p;
+            const u32x2 t = {v[0].x, v[0].y};
+            if (kStream) __builtin_nontemporal_store(t, to);
+            else *to = t;
+        } else {
 #pragma unroll
-        for (int i = 0; i < kParts; ++i) {
-            if (kStream) mrl::Vec<DT>::store_nt(p + i * kVec, v[i]);
-            else mrl::Vec<DT>::store(p + i * kVec, v[i]);
+            for (int i = 0; i < kParts; ++i) {
+                if (kStream) mrl::Vec<DT>::store_nt(p + i * kVec, v[i]);
+                else mrl::Vec<DT>::store(p + i * kVec, v[i]);
+            }
         }
     }
     __device__ __forceinline__ void unpack(float (&z)[kN]) const {
 #pragma unroll
-        for (int i = 0; i < kParts; ++i) {
+        for (int i = 0; i < (kHalf ? 1 : kParts); ++i) {
             float t[kVec];
             Elem<DT>::unpack(v[i], t);
 #pragma unroll
-            for (int j = 0; j < kVec; ++j) z[i * kVec + j] = t[j];
+            for (int j = 0; j < (kHalf ? kN : kVec); ++j) z[i * kVec + j] = t[j];
         }
     }
     __device__ __forceinline__ void pack(const float (&z)[kN]) {
 #pragma unroll
-        for (int i = 0; i < kParts; ++i) {
-            float t[kVec];
+        for (int i = 0; i < (kHalf ? 1 : kParts); ++i) {
+            float t[kVec] = {};
 #pragma unroll
-            for (int j = 0; j < kVec; ++j) t[j] = z[i * kVec + j];
+            for (int j = 0; j < (kHalf ? kN : kVec); ++j) t[j] = z[i * kVec + j];
             v[i] = Elem<DT>::pack(t);
         }
     }
@@ -236,17 +258,17 @@ __device__ __forceinline__ uint32_t team_most(uint32_t x, int lanes, uint32_t* l
     return lanes_most(w < waves ? lds[first + w] : 0u);
 }
 
-// A team a row, kVecs vectors a lane, each row read once.  The last vector of a row that is not whole vectors overlaps the one in
+// A team a row, kVecs vectors of the stream's type a lane, each row read once.  The last vector of a row that is not whole vectors overlaps the one in
 // front of it; what a lane holds twice over is left out of its sums and written twice with the same bits.
 template <int DT, int RT, int WDT, int kVecs, bool kRes, bool kFp8, bool kStream>
 __global__ __launch_bounds__(1024) void add_norm_fwd_rows_kernel(FwdArgs a, int lanes) {
     using T = typename Elem<DT>::T;
     using R = typename Elem<RT>::T;
-    constexpr int kVec = Elem<DT>::kVec;
+    constexpr int kVec = Elem<RT>::kVec;
     __shared__ float2 lds[16];
     __shared__ uint32_t most_lds[16];
-    const int tl = threadIdx.x & (lanes - 1);
-    const int64_t wanted = (int64_t)blockIdx.x * (blockDim.x / lanes) + threadIdx.x / lanes;
+    const int team = threadIdx.x / lanes, tl = threadIdx.x - team * lanes;
+    const int64_t wanted = (int64_t)blockIdx.x * (blockDim.x / lanes) + team;
     const bool live = wanted < a.n_rows;
     const int64_t row = live ? wanted : a.n_rows - 1;
     const Columns<kVecs, kVec> col(tl, lanes, a.hidden);
@@ -341,9 +363,9 @@ template <int DT, int RT, int WDT, int kVecs, int kBlockMost, bool kDh, bool kSt
 __global__ __launch_bounds__(kBlockMost) void add_norm_bwd_rows_kernel(BwdArgs a, int lanes, void* __restrict__ dweight) {
     using T = typename Elem<DT>::T;
     using R = typename Elem<RT>::T;
-    constexpr int kVec = Elem<DT>::kVec;
+    constexpr int kVec = Elem<RT>::kVec;
     constexpr bool kOne = kBlockMost > kBwdBlock;       // the team is the workgroup
-    constexpr bool kAhead = kVecs == 1;                 // the next row is requested before this one is summed
+    constexpr bool kAhead = kVecs == 1 || (kVecs == 2 && !kOne);   // the next row is requested before this one is summed
     extern __shared__ float columns[];                  // [kVecs * kVec][lanes] sums on their way between teams
     __shared__ float2 lds[2][16];
     const int teams = kOne ? 1 : blockDim.x / lanes, team = kOne ? 0 : threadIdx.x / lanes;
@@ -458,26 +480,36 @@ __global__ __launch_bounds__(kBlockMost) void add_norm_bwd_rows_kernel(BwdArgs a
     }
 }
 
-constexpr int kMaxVecs = 4;
-
-// 16 lanes (not where 32 share a block's scale), then whole wavefronts.
-Team fwd_team_of(int dtype, int64_t hidden, int block) {
-    const int64_t nv = vectors_of(dtype, hidden);
-    if (nv == 0) return {0, 0};
-    if (nv <= 64 && !(block && dtype == MRL_F32)) return team_that_fits(nv, 16, (int)((nv + 15) / 16));
-    for (int lanes = 64; lanes <= 1024; lanes *= 2)
-        if (nv <= (int64_t)lanes * kMaxVecs) return team_that_fits(nv, lanes, (int)((nv + lanes - 1) / lanes));
+// 16 lanes (not where 32 share a block's scale), then as many wavefronts as `vecs` vectors a lane make, or more vectors where
+// 16 of them are not enough.
+Team team_of_waves(int64_t nv, int vecs) {
+    for (; vecs <= 4; ++vecs) {
+        const int64_t lanes = (nv + 64 * vecs - 1) / (64 * vecs) * 64;
+        if (lanes <= 1024) return team_that_fits(nv, lanes, (int)((nv + lanes - 1) / lanes));
+    }
     return {0, 0};
 }
 
-Team bwd_team_of(int dtype, int64_t n_rows, int64_t hidden) {
-    const int64_t nv = vectors_of(dtype, hidden);
+// Two vectors of each of x and the residual are on a lane's way, or four of x alone (us, one / two / four: 32 768 x 4 096 bf16
+// 173 / 171 / 176, to e4m3 by blocks 155 / 158 / 158, without a residual 117 / 84 / 70).
+Team fwd_team_of(int rtype, int64_t hidden, int block, bool residual) {
+    const int64_t nv = vectors_of(rtype, hidden);
+    if (nv == 0) return {0, 0};
+    if (nv <= 64 && !(block && rtype == MRL_F32)) return team_that_fits(nv, 16, (int)((nv + 15) / 16));
+    return team_of_waves(nv, residual ? 2 : 4);
+}
+
+// One vector a lane, the next row requested ahead.  Two (ahead as well) for much data whose rows are 4 or 8 KB: teams of one would be
+// workgroups of 512 threads then, which take longer (us, one / two: 65 536 x 2 048 bf16 191 / 177, 32 768 x 4 096 191 / 178, 1 536 133 /
+// 142, 32 768 x 3 584 156 / 160, 5 120 228 / 244).  Rows that 1 024 lanes do not hold so: two or, of fp32, four a lane, not ahead.
+Team bwd_team_of(int rtype, int64_t n_rows, int64_t hidden) {
+    const int64_t nv = vectors_of(rtype, hidden);
     if (nv == 0) return {0, 0};
     if (nv <= 32) return team_that_fits(nv, 16, (int)((nv + 15) / 16));
-    const bool two = nv > 256 || (nv > 128 && n_rows * nv >= kBwdManyVecs);
-    for (int vecs = two ? 2 : 1; vecs <= 2; vecs *= 2) {
-        const int64_t waves = (nv + 64 * vecs - 1) / (64 * vecs);
-        if (waves <= 16) return team_that_fits(nv, waves * 64, vecs);
+    if ((nv == 256 || nv == 512) && n_rows * nv >= kBwdManyVecs) return team_that_fits(nv, nv / 2, 2);
+    for (int vecs = 1; vecs <= (rtype == MRL_F32 ? 4 : 2); vecs *= 2) {
+        const int64_t lanes = (nv + 64 * vecs - 1) / (64 * vecs) * 64;
+        if (lanes <= 1024) return team_that_fits(nv, lanes, vecs);
     }
     return {0, 0};
 }
@@ -513,12 +545,12 @@ void with_flag(bool flag, F launch) {
 
 template <int DT, int RT>
 void launch_fwd(const FwdArgs& a, hipStream_t stream) {
-    const Team team = fwd_team_of(DT, a.hidden, a.block);
+    const Team team = fwd_team_of(RT, a.hidden, a.block, a.residual != nullptr);
     if (team.lanes == 0) {
         hipLaunchKernelGGL((add_norm_fwd_kernel<DT, RT>), dim3((unsigned)a.n_rows), dim3(kBlock), 0, stream, a);
         return;
     }
-    const int block = team.lanes > 256 ? team.lanes : 256, teams = block / team.lanes;
+    const int block = team.lanes > kBlock ? team.lanes : kBlock / team.lanes * team.lanes, teams = block / team.lanes;
     const bool lines = team.lanes >= 64 && a.hidden * (int64_t)sizeof(typename Elem<DT>::T) % 128 == 0;
     const auto launch = [&](auto wdt, auto vecs, auto res, auto fp8, auto nt) {
         hipLaunchKernelGGL((add_norm_fwd_rows_kernel<DT, RT, decltype(wdt)::value, decltype(vecs)::value, decltype(res)::value != 0,
@@ -538,7 +570,7 @@ void launch_fwd(const FwdArgs& a, hipStream_t stream) {
 
 template <int DT, int RT>
 void launch_bwd(const BwdArgs& a, hipStream_t stream) {
-    const Team team = bwd_team_of(DT, a.n_rows, a.hidden);
+    const Team team = bwd_team_of(RT, a.n_rows, a.hidden);
     const auto sum_parts = [&](int n_parts) {
         with_weight<DT>(a.wide_weight, [&](auto wdt) {
             constexpr int WDT = decltype(wdt)::value;
@@ -551,7 +583,7 @@ void launch_bwd(const BwdArgs& a, hipStream_t stream) {
         const bool lines = team.lanes >= 64 && a.hidden * (int64_t)sizeof(typename Elem<DT>::T) % 128 == 0;
         BwdArgs b = a;
         if (!a.dweight || groups == 1) b.part = nullptr;
-        const size_t lds = a.dweight && block > team.lanes ? (size_t)team.lanes * team.vecs * Elem<DT>::kVec * 4 : 0;
+        const size_t lds = a.dweight && block > team.lanes ? (size_t)team.lanes * team.vecs * Elem<RT>::kVec * 4 : 0;
         const auto launch = [&](auto wdt, auto vecs, auto most, auto dh, auto nt) {
             hipLaunchKernelGGL((add_norm_bwd_rows_kernel<DT, RT, decltype(wdt)::value, decltype(vecs)::value, decltype(most)::value,
                                                          decltype(dh)::value != 0, decltype(nt)::value != 0>),
@@ -560,6 +592,9 @@ void launch_bwd(const BwdArgs& a, hipStream_t stream) {
         with_weight<DT>(a.wide_weight, [&](auto wdt) {
             with_flag(a.dh != nullptr, [&](auto dh) {
                 with_flag(lines, [&](auto nt) {
+                    if constexpr (RT == MRL_F32) {
+                        if (team.vecs == 4) return launch(wdt, Int<4>(), Int<1024>(), dh, nt);
+                    }
                     if (team.vecs == 2 && team.lanes > kBwdBlock) launch(wdt, Int<2>(), Int<1024>(), dh, nt);
                     else if (team.vecs == 2) launch(wdt, Int<2>(), Int<kBwdBlock>(), dh, nt);
                     else if (team.lanes > kBwdBlock) launch(wdt, Int<1>(), Int<1024>(), dh, nt);

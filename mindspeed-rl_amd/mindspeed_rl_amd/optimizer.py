@@ -23,8 +23,11 @@ _DATA_PTR, _NUMEL, _CONTIGUOUS, _GET_DEVICE = torch.Tensor.data_ptr, torch.Tenso
 _DTYPE, _SHAPE, _LAYOUT, _REQUIRES_GRAD = map(operator.attrgetter, ("dtype", "shape", "layout", "requires_grad"))
 
 
-def _is_tensor(t):
-    return isinstance(t, torch.Tensor)
+_USUAL = {torch.Tensor, torch.nn.Parameter}
+
+
+def _are_tensors(ts):
+    return _USUAL.issuperset(map(type, ts)) or all(isinstance(t, torch.Tensor) for t in ts)
 
 
 def _blocks(n):
@@ -55,8 +58,8 @@ def adamw_state(params, bits=32, master=True):
 
 def _check_params(params):
     """Their shapes and types."""
-    if not all(map(_is_tensor, params)):
-        raise TypeError("parameters must be tensors, not %s" % [type(p).__name__ for p in params if not _is_tensor(p)][0])
+    if not _are_tensors(params):
+        raise TypeError("parameters must be tensors, not %s" % sorted({type(p).__name__ for p in params}))
     dtypes = [*map(_DTYPE, params)]
     if not _CODES.keys() >= set(dtypes) or {*map(_LAYOUT, params)} - {torch.strided}:
         raise TypeError("parameters must be dense float32, bfloat16 or float16 tensors")
@@ -68,7 +71,7 @@ def _check_params(params):
 
 def _check_held(name, held, shapes, dtype):
     """What the step keeps: tensors of `dtype` and the parameters' shapes, as they lie in memory."""
-    if not all(map(_is_tensor, held)) or {*map(_DTYPE, held)} - {dtype} or [*map(_SHAPE, held)] != shapes or False in map(_CONTIGUOUS, held):
+    if not _are_tensors(held) or {*map(_DTYPE, held)} - {dtype} or [*map(_SHAPE, held)] != shapes or False in map(_CONTIGUOUS, held):
         raise ValueError("%s must hold contiguous tensors of %s with the parameters' shapes" % (name, dtype))
     if True in map(_REQUIRES_GRAD, held):
         raise ValueError("what the step keeps is part of a graph: give detached tensors")
@@ -76,7 +79,7 @@ def _check_held(name, held, shapes, dtype):
 
 def _check_grads(grads, shapes, dtypes):
     """Their types."""
-    if not all(map(_is_tensor, grads)) or {*map(_LAYOUT, grads)} - {torch.strided}:
+    if not _are_tensors(grads) or {*map(_LAYOUT, grads)} - {torch.strided}:
         raise ValueError("gradients must be dense tensors")
     types = [*map(_DTYPE, grads)]
     if [*map(_SHAPE, grads)] != shapes or (types != dtypes and any(g is not p and g is not torch.float32 for g, p in zip(types, dtypes))):
