@@ -27,15 +27,15 @@ namespace {
 using mrl_vocab::Elem;
 
 // A lane takes four entries, so that what a wavefront reads or writes of an fp32 tensor at a time lies together, and a workgroup
-// one chunk, after which it ends: the memory serves small workgroups that come and go best.  All of it goes past the caches.
-// us, 719 M bf16 parameters with fp32 gradients, main weights and moments (21.6 GB) / 449 M with bf16 gradients and moments in 8
-// bits (7.2 GB): 3 550 / 1 230; eight entries a lane 4 226 / 1 344, 64, 256, 512 and 1 024 threads 3 615, 3 715, 3 869, 3 860 /
-// 1 228, 1 221, 1 257, 1 330; through the caches (256 threads) 4 096 / 1 350, loads alone past them 4 060 / 1 291, stores alone 3 960 / 1 262.
-constexpr int kBlock = 128;
+// one chunk, after which it ends: the memory serves small workgroups that come and go best.  All of it goes past the caches.  us,
+// 719 M bf16 parameters with fp32 gradients, main weights and moments (21.6 GB, 6.1 TB/s) by 64, 128, 256 threads 3 655, 3 560, 3 813;
+// 449 M with bf16 gradients and moments in 8 bits (7.2 GB, 6.2 TB/s) 1 187, 1 173, 1 171, 42 M of fp32 that lie off the lines 157, 136, 126;
+// eight entries a lane 4 226 (1 344), through the caches 4 001 (1 300).
 constexpr int kUnit = 4;                    // entries of a lane: 32 lanes a block of 128
-constexpr int kChunk = kBlock * kUnit;      // entries of a workgroup
+constexpr int block_of(bool small) { return small ? 256 : 128; }
+constexpr int chunk_of(bool small) { return block_of(small) * kUnit; }     // entries of a workgroup
 constexpr int kTable = 54;                  // tensors of a launch: 4 KB of arguments
-constexpr int64_t kMostGroups = (1LL << 25) - 1;    // of a launch, which holds fewer than 2^32 threads
+constexpr int64_t kMostGroups = (1LL << 24) - 1;    // of a launch, which holds fewer than 2^32 threads
 constexpr float kMost = 448.f;              // of e4m3
 constexpr float kLeastCode = 0.001953125f;  // 2^-9
 constexpr float kLeastScale = 1.17549435e-38f;      // 2^-126
@@ -92,42 +92,61 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef u32x2 u32x2_anywhere __attribute__((aligned(2)));
 typedef uint32_t u32_anywhere __attribute__((aligned(1)));
 
-// A lane's entries from `at` on, of which `valid` are the tensor's; zeros behind them.
+// A lane's entries as they lie in memory.  kWhole: all of them are the tensor's, and a load is one instruction that nothing waits for
+// before the values are asked for; else `valid` of them are, zeros stand behind them, and they are loaded one by one.
 template <int DT>
-__device__ __forceinline__ void load_unit(const void* base, int64_t at, int valid, float (&z)[kUnit]) {
-    const typename Elem<DT>::T* p = (const typename Elem<DT>::T*)base + at;
-    if (valid < kUnit) {
+struct Unit {
+    using T = typename Elem<DT>::T;
+    u32x4 v;
+    template <bool kWhole>
+    __device__ __forceinline__ void load(const void* base, int64_t at, int valid) {
+        const T* p = (const T*)base + at;
+        if constexpr (!kWhole) {
+            float z[kUnit];
 #pragma unroll
-        for (int i = 0; i < kUnit; ++i) z[i] = i < valid ? Elem<DT>::load(p + i) : 0.f;
-    } else if constexpr (DT == MRL_F32) {
-        Elem<DT>::unpack(mrl::Vec<DT>::load_nt(p), z);
-    } else {
-        const u32x2 v = __builtin_nontemporal_load((const u32x2_anywhere*)p);
-        float t[8];
-        Elem<DT>::unpack(mrl::make_u32x4(v.x, v.y, 0u, 0u), t);
+            for (int i = 0; i < kUnit; ++i) z[i] = i < valid ? Elem<DT>::load(p + i) : 0.f;
+            put(z);
+        } else if constexpr (DT == MRL_F32) {
+            v = mrl::Vec<DT>::load_nt(p);
+        } else {
+            const u32x2 t = __builtin_nontemporal_load((const u32x2_anywhere*)p);
+            v = mrl::make_u32x4(t.x, t.y, 0u, 0u);
+        }
+    }
+    template <bool kWhole>
+    __device__ __forceinline__ void store(void* base, int64_t at, int valid) const {
+        T* p = (T*)base + at;
+        if constexpr (!kWhole) {
+            float z[kUnit];
+            get(z);
+#pragma unroll
+            for (int i = 0; i < kUnit; ++i)
+                if (i < valid) Elem<DT>::store(p + i, z[i]);
+        } else if constexpr (DT == MRL_F32) {
+            mrl::Vec<DT>::store_nt(p, v);
+        } else {
+            const u32x2 t = {v.x, v.y};
+            __builtin_nontemporal_store(t, (u32x2_anywhere*)p);
+        }
+    }
+    __device__ __forceinline__ void get(float (&z)[kUnit]) const {
+        float t[Elem<DT>::kVec];
+        Elem<DT>::unpack(v, t);
 #pragma unroll
         for (int i = 0; i < kUnit; ++i) z[i] = t[i];
     }
-}
-
-template <int DT>
-__device__ __forceinline__ void store_unit(void* base, int64_t at, int valid, const float (&z)[kUnit]) {
-    typename Elem<DT>::T* p = (typename Elem<DT>::T*)base + at;
-    if (valid < kUnit) {
+    __device__ __forceinline__ void put(const float (&z)[kUnit]) {
+        float t[Elem<DT>::kVec] = {};
 #pragma unroll
-        for (int i = 0; i < kUnit; ++i)
-            if (i < valid) Elem<DT>::store(p + i, z[i]);
-    } else if constexpr (DT == MRL_F32) {
-        mrl::Vec<DT>::store_nt(p, Elem<DT>::pack(z));
-    } else {
-        const u32x2 v = {Elem<DT>::pack2(z[0], z[1]), Elem<DT>::pack2(z[2], z[3])};
-        __builtin_nontemporal_store(v, (u32x2_anywhere*)p);
+        for (int i = 0; i < kUnit; ++i) t[i] = z[i];
+        v = Elem<DT>::pack(t);
     }
-}
+};
 
+template <bool kWhole>
 __device__ __forceinline__ uint32_t load_codes(const void* base, int64_t at, int valid) {
     const uint8_t* p = (const uint8_t*)base + at;
-    if (valid == kUnit) return __builtin_nontemporal_load((const u32_anywhere*)p);
+    if (kWhole) return __builtin_nontemporal_load((const u32_anywhere*)p);
     uint32_t c = 0;
 #pragma unroll
     for (int i = 0; i < kUnit; ++i)
@@ -135,9 +154,10 @@ __device__ __forceinline__ uint32_t load_codes(const void* base, int64_t at, int
     return c;
 }
 
+template <bool kWhole>
 __device__ __forceinline__ void store_codes(void* base, int64_t at, int valid, uint32_t c) {
     uint8_t* p = (uint8_t*)base + at;
-    if (valid == kUnit) {
+    if (kWhole) {
         __builtin_nontemporal_store(c, (u32_anywhere*)p);
         return;
     }
@@ -189,8 +209,80 @@ __device__ __forceinline__ uint32_t codes_of(const float (&z)[kUnit], float scal
     return (uint32_t)c;
 }
 
+// A lane's share of a chunk: entries from `at` on.
+template <int PT, int GT, bool kMaster, bool kSmall, bool kWhole>
+__device__ __forceinline__ void step_unit(const Part& p, int64_t at, const Coefs& c, const Constants& k) {
+    const int64_t left = p.n - at;
+    const int valid = kWhole || left >= kUnit ? kUnit : left > 0 ? (int)left : 0;
+    constexpr int kWT = kMaster ? MRL_F32 : PT;
+    void* const weights = kMaster ? (void*)p.master : p.param;
+    Unit<GT> gu;
+    Unit<kWT> wu;
+    Unit<MRL_F32> mu, vu;
+    uint32_t mc, vc;
+    float ms, vs;
+    const int64_t block = kWhole || valid > 0 ? at / 128 : 0;
+    gu.template load<kWhole>(p.grad, at, valid);
+    wu.template load<kWhole>(weights, at, valid);
+    if (kSmall) {
+        mc = load_codes<kWhole>(p.m, at, valid);
+        vc = load_codes<kWhole>(p.v, at, valid);
+        ms = p.m_scale[block];
+        vs = p.v_scale[block];
+    } else {
+        mu.template load<kWhole>(p.m, at, valid);
+        vu.template load<kWhole>(p.v, at, valid);
+    }
+    float g[kUnit], w[kUnit], m[kUnit], v[kUnit], root[kUnit];
+    gu.get(g);
+    wu.get(w);
+    if (kSmall) {
+        values_of(mc, ms, m);
+        values_of(vc, vs, v);
+#pragma unroll
+        for (int i = 0; i < kUnit; ++i) v[i] = mrl::mul_rn(v[i], v[i]);
+    } else {
+        mu.get(m);
+        vu.get(v);
+    }
+#pragma unroll
+    for (int i = 0; i < kUnit; ++i) {
+        g[i] = mrl::mul_rn(g[i], c.factor);
+        m[i] = mrl::add_rn(mrl::mul_rn(m[i], k.b1), mrl::mul_rn(g[i], k.rest1));
+        v[i] = mrl::add_rn(mrl::mul_rn(v[i], k.b2), mrl::mul_rn(mrl::mul_rn(g[i], g[i]), k.rest2));
+        root[i] = sqrtf(v[i]);
+        w[i] = w[i] * c.decay - m[i] / (root[i] * c.second + k.eps) * c.rate;
+    }
+    wu.put(w);
+    wu.template store<kWhole>(weights, at, valid);
+    if (kMaster) {
+        Unit<PT> pu;
+        pu.put(w);
+        pu.template store<kWhole>(p.param, at, valid);
+    }
+    if (kSmall) {
+        uint32_t bits[kUnit / 2];
+#pragma unroll
+        for (int i = 0; i < kUnit / 2; ++i) bits[i] = dither((uint32_t)(at / 2) + i, c.key);
+        ms = block_scale(m);
+        vs = block_scale(root);
+        store_codes<kWhole>(p.m, at, valid, codes_of<false>(m, ms, bits));
+        store_codes<kWhole>(p.v, at, valid, codes_of<true>(root, vs, bits));
+        if (valid > 0 && (threadIdx.x & 31) == 0) {
+            p.m_scale[block] = ms;
+            p.v_scale[block] = vs;
+        }
+    } else {
+        mu.put(m);
+        vu.put(v);
+        mu.template store<kWhole>(p.m, at, valid);
+        vu.template store<kWhole>(p.v, at, valid);
+    }
+}
+
 template <int PT, int GT, bool kMaster, bool kSmall>
-__global__ __launch_bounds__(kBlock) void adamw_kernel(Table t, const Coefs* __restrict__ coefs, Constants k) {
+__global__ __launch_bounds__(block_of(kSmall)) void adamw_kernel(Table t, const Coefs* __restrict__ coefs, Constants k) {
+    constexpr int kChunk = chunk_of(kSmall);
     __shared__ int32_t ends[64];
     if (threadIdx.x < 64) ends[threadIdx.x] = (int)threadIdx.x < t.n_parts ? (int32_t)t.part[threadIdx.x].end_chunk : 0x7fffffff;
     __syncthreads();
@@ -199,65 +291,23 @@ __global__ __launch_bounds__(kBlock) void adamw_kernel(Table t, const Coefs* __r
         // as many tensors end at or in front of it
         const int part = __builtin_amdgcn_readfirstlane(__popcll(__ballot(ends[threadIdx.x & 63] <= chunk)));
         const Part& p = t.part[part];
-        const int64_t at = (chunk - (part == 0 ? 0 : t.part[part - 1].end_chunk)) * kChunk + threadIdx.x * kUnit;
-        const int64_t left = p.n - at;
-        const int valid = left >= kUnit ? kUnit : left > 0 ? (int)left : 0;
-        // everything is on its way before any of it is waited for
-        float g[kUnit], w[kUnit], m[kUnit], v[kUnit];
-        load_unit<GT>(p.grad, at, valid, g);
-        if (kMaster) load_unit<MRL_F32>(p.master, at, valid, w);
-        else load_unit<PT>(p.param, at, valid, w);
-        const int64_t block = valid > 0 ? at / 128 : 0;
-        if (kSmall) {
-            const uint32_t mc = load_codes(p.m, at, valid), vc = load_codes(p.v, at, valid);
-            const float ms = p.m_scale[block], vs = p.v_scale[block];
-            values_of(mc, ms, m);
-            values_of(vc, vs, v);
-#pragma unroll
-            for (int i = 0; i < kUnit; ++i) v[i] = mrl::mul_rn(v[i], v[i]);
-        } else {
-            load_unit<MRL_F32>(p.m, at, valid, m);
-            load_unit<MRL_F32>(p.v, at, valid, v);
-        }
-        float root[kUnit];
-#pragma unroll
-        for (int i = 0; i < kUnit; ++i) {
-            g[i] = mrl::mul_rn(g[i], c.factor);
-            m[i] = mrl::add_rn(mrl::mul_rn(m[i], k.b1), mrl::mul_rn(g[i], k.rest1));
-            v[i] = mrl::add_rn(mrl::mul_rn(v[i], k.b2), mrl::mul_rn(mrl::mul_rn(g[i], g[i]), k.rest2));
-            root[i] = sqrtf(v[i]);
-            w[i] = w[i] * c.decay - m[i] / (root[i] * c.second + k.eps) * c.rate;
-        }
-        if (kMaster) store_unit<MRL_F32>(p.master, at, valid, w);
-        store_unit<PT>(p.param, at, valid, w);
-        if (kSmall) {
-            uint32_t bits[kUnit / 2];
-#pragma unroll
-            for (int i = 0; i < kUnit / 2; ++i) bits[i] = dither((uint32_t)(at / 2) + i, c.key);
-            const float ms = block_scale(m), vs = block_scale(root);
-            store_codes(p.m, at, valid, codes_of<false>(m, ms, bits));
-            store_codes(p.v, at, valid, codes_of<true>(root, vs, bits));
-            if (valid > 0 && (threadIdx.x & 31) == 0) {
-                p.m_scale[block] = ms;
-                p.v_scale[block] = vs;
-            }
-        } else {
-            store_unit<MRL_F32>(p.m, at, valid, m);
-            store_unit<MRL_F32>(p.v, at, valid, v);
-        }
+        const int64_t first = (chunk - (part == 0 ? 0 : t.part[part - 1].end_chunk)) * kChunk, at = first + threadIdx.x * kUnit;
+        // every wavefront of it decides alike
+        if (first + kChunk <= p.n) step_unit<PT, GT, kMaster, kSmall, true>(p, at, c, k);
+        else step_unit<PT, GT, kMaster, kSmall, false>(p, at, c, k);
     }
 }
 
 // The launches of a list for the tensors of a kind that are not empty: launch(table) for each at most kTable of them.
 template <typename F>
-void for_tables(const mrl_adamw_tensor* list, int64_t n, int dtype, int grad_dtype, bool master, F launch) {
+void for_tables(const mrl_adamw_tensor* list, int64_t n, int chunk, int dtype, int grad_dtype, bool master, F launch) {
     Table t;
     t.n_parts = 0;
     int64_t chunks = 0;
     for (int64_t i = 0; i < n; ++i) {
         const mrl_adamw_tensor& p = list[i];
         if (p.n == 0 || p.dtype != dtype || p.grad_dtype != grad_dtype || (p.master != nullptr) != master) continue;
-        chunks += (p.n + kChunk - 1) / kChunk;
+        chunks += (p.n + chunk - 1) / chunk;
         t.part[t.n_parts++] = {p.param, p.grad, (float*)p.master, p.exp_avg, p.exp_avg_sq, p.exp_avg_scale, p.exp_avg_sq_scale, p.n, chunks};
         t.n_chunks = (int32_t)chunks;
         if (t.n_parts == kTable) {
@@ -358,10 +408,10 @@ extern "C" int mrl_adamw_step(const mrl_adamw_tensor* tensors, int64_t n_tensors
     const Constants k = {(float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps};
     const auto launch = [&](const Table& t, auto kernel) {
         const int64_t groups = t.n_chunks < kMostGroups ? t.n_chunks : kMostGroups;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(kBlock), 0, s, t, coefs, k);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(block_of(bits == 8)), 0, s, t, coefs, k);
     };
 #define MRL_KIND(DT, GT, MASTER)                                                                                     \
-    for_tables(tensors, n_tensors, DT, GT, MASTER, [&](const Table& t) {                                             \
+    for_tables(tensors, n_tensors, chunk_of(bits == 8), DT, GT, MASTER, [&](const Table& t) {                                             \
         bits == 8 ? launch(t, adamw_kernel<DT, GT, MASTER, true>) : launch(t, adamw_kernel<DT, GT, MASTER, false>);  \
     })
     MRL_KIND(MRL_F32, MRL_F32, false);
