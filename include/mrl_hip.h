@@ -775,7 +775,8 @@ int mrl_grad_clip(const mrl_grad* grads, int64_t n_grads, float max_norm, float*
  * mrl_add_norm_fwd: h = x + residual, rounded to the residual's type (the rows' or F32), and y = h * rstd * weight, rstd = (mean h^2
  * + eps)^(-1/2) per row of `hidden` entries, in fp32, rounded to the rows' type: what an addition and mrl_norm_fwd (subtract_mean = 0)
  * behind it give.  x and residual: row strides in elements, only read; h and y dense, each of its input's type; weight: the rows'
- * type or F32; rstd [n_rows] fp32, nullable, is what the backward takes.  hidden at most MRL_NORM_MAX_HIDDEN, fewer than 2^24 rows.
+ * type or F32; rstd [n_rows] fp32, nullable, is what the backward takes.  hidden at most MRL_NORM_MAX_HIDDEN, fewer than 2^24 rows, and no
+ * more than 2^32 threads hold, 16 to 1 024 for a row.
  * Outputs share no memory with anything else.
  *
  * mrl_norm_fp8_fwd: the same, or (residual and h NULL) the norm of x itself, with y as OCP e4m3 codes q [n_rows, hidden] and

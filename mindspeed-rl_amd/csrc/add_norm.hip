@@ -529,6 +529,14 @@ int64_t slab_rows_of(int64_t n_rows) {
     return rows < 16 ? 16 : rows;
 }
 
+// Threads of a workgroup of the forward's, and how many of them the rows take.
+int fwd_block(const Team& team) { return team.lanes > kBlock ? team.lanes : team.lanes > 0 ? kBlock / team.lanes * team.lanes : kBlock; }
+
+int64_t fwd_groups(const Team& team, int64_t n_rows) {
+    const int64_t teams = team.lanes > 0 ? fwd_block(team) / team.lanes : 1;
+    return (n_rows + teams - 1) / teams;
+}
+
 // launch(weight's type) for the rows' type or fp32.
 template <int DT, typename F>
 void with_weight(int wide, F launch) {
@@ -546,16 +554,16 @@ void with_flag(bool flag, F launch) {
 template <int DT, int RT>
 void launch_fwd(const FwdArgs& a, hipStream_t stream) {
     const Team team = fwd_team_of(RT, a.hidden, a.block, a.residual != nullptr);
+    const dim3 grid((unsigned)fwd_groups(team, a.n_rows)), block(fwd_block(team));
     if (team.lanes == 0) {
-        hipLaunchKernelGGL((add_norm_fwd_kernel<DT, RT>), dim3((unsigned)a.n_rows), dim3(kBlock), 0, stream, a);
+        hipLaunchKernelGGL((add_norm_fwd_kernel<DT, RT>), grid, block, 0, stream, a);
         return;
     }
-    const int block = team.lanes > kBlock ? team.lanes : kBlock / team.lanes * team.lanes, teams = block / team.lanes;
     const bool lines = team.lanes >= 64 && a.hidden * (int64_t)sizeof(typename Elem<DT>::T) % 128 == 0;
     const auto launch = [&](auto wdt, auto vecs, auto res, auto fp8, auto nt) {
         hipLaunchKernelGGL((add_norm_fwd_rows_kernel<DT, RT, decltype(wdt)::value, decltype(vecs)::value, decltype(res)::value != 0,
                                                      decltype(fp8)::value != 0, decltype(nt)::value != 0>),
-                           dim3((unsigned)((a.n_rows + teams - 1) / teams)), dim3(block), 0, stream, a, team.lanes);
+                           grid, block, 0, stream, a, team.lanes);
     };
     with_weight<DT>(a.wide_weight, [&](auto wdt) {
         with_vecs(team.vecs, [&](auto vecs) {
@@ -649,6 +657,9 @@ int check_sizes(const char* fn, int dtype, int rtype, int wdtype, int64_t n_rows
 int check_fwd(const char* fn, int dtype, int rtype, int wdtype, const FwdArgs& a, int64_t hidden) {
     const int rc = check_sizes(fn, dtype, rtype, wdtype, a.n_rows, hidden);
     if (rc != MRL_OK) return rc;
+    const Team team = fwd_team_of(rtype, hidden, a.block, a.residual != nullptr);
+    MRL_REQUIRE(mrl::launch_fits(fwd_groups(team, a.n_rows), fwd_block(team)), MRL_ERR_UNSUPPORTED,
+                "%s: n_rows=%lld of hidden=%lld (2^32 threads hold fewer, up to 1024 for a row)", fn, (long long)a.n_rows, (long long)hidden);
     MRL_REQUIRE((a.x_stride >= hidden && (!a.residual || a.residual_stride >= hidden)) || a.n_rows <= 1, MRL_ERR_INVALID_ARG,
                 "%s: strides %lld and %lld below hidden=%lld", fn, (long long)a.x_stride, (long long)a.residual_stride, (long long)hidden);
     MRL_REQUIRE(a.eps > 0.f && a.eps <= 3.0e38f, MRL_ERR_INVALID_ARG, "%s: eps=%g (want a positive, finite number)", fn, (double)a.eps);
@@ -684,7 +695,7 @@ extern "C" int mrl_norm_fp8_fwd(const void* x, int dtype, int64_t x_stride, cons
                        weight_dtype == MRL_F32, eps};
     MRL_REQUIRE(block == 0 || block == 128, MRL_ERR_UNSUPPORTED, "%s: block=%lld (want 0, a row, or 128)", fn, (long long)block);
     MRL_REQUIRE(block == 0 || hidden % 128 == 0, MRL_ERR_UNSUPPORTED, "%s: hidden=%lld is not whole blocks of 128", fn, (long long)hidden);
-    const int rc = check_fwd(fn, dtype, residual_dtype, weight_dtype, a, hidden);
+    const int rc = check_fwd(fn, dtype, residual ? residual_dtype : dtype, weight_dtype, a, hidden);
     if (rc != MRL_OK || n_rows == 0) return rc;
     MRL_REQUIRE(scale, MRL_ERR_INVALID_ARG, "%s: NULL scale", fn);
     dispatch(dtype, residual ? residual_dtype : dtype, a, mrl::as_stream(stream));

@@ -176,4 +176,7 @@ def adamw_(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999), eps
     coefs = torch.empty(8, dtype=torch.float32, device=dev)
     _lib.call("mrl_adamw_step", table.buffer_info()[0], len(sizes), 8 if small else 32, step.data_ptr(), lr_value, lr_at, b1, b2, eps,
               weight_decay, _lib.ptr(grad_norm), max_norm or 0.0, coefs.data_ptr(), _lib.stream(dev))
-    increment_version(written)              # autograd looks whether what it kept has been written to
+    try:
+        increment_version(written)          # autograd looks whether what it kept has been written to
+    except RuntimeError:                    # of tensors of inference mode it keeps none
+        increment_version([t for t in written if not t.is_inference()])

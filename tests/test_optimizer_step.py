@@ -78,6 +78,11 @@ def fp32_moments(g, m, v, factor, b1, b2):
     return m * b1 + g * (1 - b1), v * b2 + (g * g) * (1 - b2)
 
 
+def factor_of(norm, limit):
+    """In fp32, by one division (a number over a tensor would be multiplied by the tensor's reciprocal)."""
+    return torch.clamp(torch.full_like(norm, limit) / (norm + 1e-6), max=1.0).item()
+
+
 def make(dev, shapes, dtype, gdtype, seed, bits=32, master=True, scale=1e-2):
     """Parameters, gradients and a state that some steps have been taken on; some gradients are zero, some rows have none."""
     gen = torch.Generator(device=dev).manual_seed(seed)
@@ -234,11 +239,10 @@ def test_clipping_on_the_way(dev, bits):
     params, grads, state = make(dev, SHAPES, BF16, F32, 2, bits)
     norm = mrl.global_grad_norm(grads)
     for limit in (0.3 * norm.item(), 10 * norm.item(), 0.0):
-        factor = torch.clamp(limit / (norm + 1e-6), max=1.0)
         old_params, old = clone(params, state)
         copies = clone(params, state)
         mrl.adamw_(params, grads, **state, grad_norm=norm, max_norm=limit, **HYPER)
-        check(params, grads, state, old_params, old, factor.item())
+        check(params, grads, state, old_params, old, factor_of(norm, limit))
         # the same bits as from clipped gradients
         clipped = [torch.empty_like(g) for g in grads]
         mrl.clip_grad_norm_(grads, limit, out=clipped)
@@ -373,6 +377,23 @@ def test_autograd_sees_the_writes(dev):
         with pytest.raises(_lib.MrlError, match="shares memory"):
             mrl.adamw_(**{"params": [w], "grads": [g], **state, "lr": 1e-2, **kw})
         assert torch.equal(w, kept)
+
+
+@pytest.mark.gpu
+def test_tensors_of_inference_mode_and_empty_lists(dev):
+    """They have no version to count up; a step without a gradient is counted."""
+    params, grads, state = make(dev, [(300,)], F32, F32, 12)
+    twin, twin_state = clone(params, state)
+    with torch.inference_mode():
+        inner, inner_state = clone(params, state)
+        mrl.adamw_(inner, grads, **inner_state, **HYPER)
+    mrl.adamw_(twin, grads, **twin_state, **HYPER)
+    assert torch.equal(inner[0], twin[0]) and inner_state["step"].item() == twin_state["step"].item() == 8
+    mrl.adamw_(twin, [None], **twin_state, **HYPER)
+    assert torch.equal(inner[0], twin[0]) and twin_state["step"].item() == 9
+    step = torch.zeros((), dtype=torch.int64, device=dev)
+    mrl.adamw_([], [], [], [], step, lr=1e-3)
+    assert step.item() == 1
 
 
 @pytest.mark.gpu

@@ -101,7 +101,7 @@ def test_entry_points_refuse_and_launch_nothing():
 
     for rc, kw in [(-2, dict(dtype=_lib.I32)), (-2, dict(wdtype=_lib.BF16)), (-2, dict(rtype=_lib.BF16)), (-1, dict(rows=-1)),
                    (-1, dict(hidden=0)), (-2, dict(hidden=most + 1, xs=most + 1, rs=most + 1)), (-2, dict(rows=1 << 24)),
-                   (-2, dict(rows=1 << 62)), (-1, dict(xs=7)), (-1, dict(rs=7)), (-1, dict(eps=0.0)), (-1, dict(eps=float("nan"))),
+                   (-2, dict(rows=1 << 62)), (-2, dict(rows=1 << 22, hidden=8192, xs=8192, rs=8192)), (-1, dict(xs=7)), (-1, dict(rs=7)), (-1, dict(eps=0.0)), (-1, dict(eps=float("nan"))),
                    (-1, dict(x=None)), (-1, dict(r=None)), (-1, dict(h=None)), (-1, dict(r=None, h=None)), (-1, dict(w=None)),
                    (-1, dict(y=None)), (-3, dict(x=p + 2)), (-3, dict(y=p + 1)), (-3, dict(h=p + 2)), (0, dict(rows=0, x=None))]:
         assert fwd(**kw) == rc, kw
