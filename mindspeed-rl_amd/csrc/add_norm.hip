@@ -9,7 +9,7 @@
 //
 // Both passes are bound by memory: the forward reads two tensors and writes two, the backward reads three and writes one (two, where the
 // stream is wider than the rows).  32 768 x 4 096 bf16: forward 171 us (6.3 TB/s), backward with the weight's gradient 177 (6.1), to e4m3 by
-// rows 153, by blocks 158 (6.0); 32 768 x 3 584 bf16 beside an fp32 stream 227 (6.2) and 310 (6.1), to e4m3 209.  (Here and below: calls that
+// rows 149, by blocks 152 (6.2); 32 768 x 3 584 bf16 beside an fp32 stream 227 (6.2) and 310 (6.1), to e4m3 205.  (Here and below: calls that
 // follow each other in a replayed graph.)
 #include "lane_ops.h"
 #include "mrl_internal.h"
@@ -225,7 +225,7 @@ struct Raw {
     }
 };
 
-template <int kN>
+template <bool kStream, int kN>
 __device__ __forceinline__ void store_codes(uint8_t* p, const float (&z)[kN]) {
     typedef uint32_t Words __attribute__((ext_vector_type(kN / 4)));
     typedef Words WordsAnywhere __attribute__((aligned(1)));
@@ -235,7 +235,8 @@ __device__ __forceinline__ void store_codes(uint8_t* p, const float (&z)[kN]) {
         int t = __builtin_amdgcn_cvt_pk_fp8_f32(z[4 * w], z[4 * w + 1], 0, false);
         c[w] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(z[4 * w + 2], z[4 * w + 3], t, true);
     }
-    *(WordsAnywhere*)p = c;
+    if (kStream) __builtin_nontemporal_store(c, (WordsAnywhere*)p);
+    else *(WordsAnywhere*)p = c;
 }
 
 __device__ __forceinline__ uint32_t lanes_most(uint32_t x) {    // over 16 lanes
@@ -348,7 +349,7 @@ __global__ __launch_bounds__(1024) void add_norm_fwd_rows_kernel(FwdArgs a, int 
         }
 #pragma unroll
         for (int i = 0; i < kVec; ++i) z[i] *= inv;
-        store_codes<kVec>((uint8_t*)a.y + at, z);
+        store_codes<kStream>((uint8_t*)a.y + at, z);
     }
     if (a.rstd && tl == 0) a.rstd[row] = r;
 }
@@ -491,7 +492,7 @@ Team team_of_waves(int64_t nv, int vecs) {
 }
 
 // Two vectors of each of x and the residual are on a lane's way, or four of x alone (us, one / two / four: 32 768 x 4 096 bf16
-// 173 / 171 / 176, to e4m3 by blocks 155 / 158 / 158, without a residual 117 / 84 / 70).
+// 173 / 171 / 176, to e4m3 by blocks (their codes through the caches) 155 / 158 / 158, without a residual 117 / 84 / 70).
 Team fwd_team_of(int rtype, int64_t hidden, int block, bool residual) {
     const int64_t nv = vectors_of(rtype, hidden);
     if (nv == 0) return {0, 0};

@@ -145,19 +145,16 @@ def _added(x, residual, weight, eps):
     return eps
 
 
-def _rows(x, hidden):
-    """The rows of ``x``, how many, their stride, and memory for as many dense ones."""
-    if x.is_contiguous():
-        return x, x.numel() // hidden, hidden, torch.empty_like(x)
-    flat, stride = _flat_rows(x)
-    return flat, flat.shape[0], stride, torch.empty(x.shape, dtype=x.dtype, device=x.device)
-
-
 def _add_forward(x, residual, weight, eps, keep):
     """y, h and, if `keep`, rstd of the rows; the weight as the kernels read it."""
     dev, hidden, w = x.device, x.shape[-1], weight.contiguous()
-    flat, n_rows, x_stride, y = _rows(x, hidden)
-    res, _, r_stride, h = _rows(residual, hidden)
+    n_rows, flat, res, x_stride, r_stride = x.numel() // hidden, x, residual, hidden, hidden
+    if x.is_contiguous() and residual.is_contiguous():
+        y, h = torch.empty_like(x), torch.empty_like(residual)
+    else:
+        flat, x_stride = _flat_rows(x)
+        res, r_stride = _flat_rows(residual)
+        y, h = x.new_empty(x.shape), residual.new_empty(x.shape)
     rstd = w.new_empty(n_rows, dtype=torch.float32) if keep else None
     _lib.call("mrl_add_norm_fwd", flat.data_ptr(), _lib.dtype_code(x), x_stride, res.data_ptr(), _lib.dtype_code(h), r_stride,
               n_rows, hidden, w.data_ptr(), _lib.dtype_code(w), eps, h.data_ptr(), y.data_ptr(), _lib.ptr(rstd), _lib.stream(dev))
@@ -179,7 +176,8 @@ def _add_backward(ctx, dy, dh):
         dy, dy_stride = _flat_rows(dy)
     if dh is not None and not dh.is_contiguous():
         dh, dh_stride = _flat_rows(dh)
-    dx = torch.empty(shape, dtype=dtype, device=dev) if need_x else None
+    # dy has the type of x, and its shape unless it was spread out
+    dx = (torch.empty_like(dy) if dy.shape == shape and dy_stride == hidden else dy.new_empty(shape)) if need_x else None
     dr = torch.empty_like(h) if need_r and not (need_x and h.dtype is dtype) else None
     dw = workspace = None
     ws_bytes = 0
@@ -246,7 +244,8 @@ def rms_norm_fp8(x, weight, eps=1e-6, residual=None, block=None):
         flat, x_stride = _flat_rows(x)
     res, r_stride, h = None, hidden, None
     if residual is not None:
-        res, _, r_stride, h = _rows(residual, hidden)
+        res, r_stride = (residual, hidden) if residual.is_contiguous() else _flat_rows(residual)
+        h = residual.new_empty(x.shape)
     q = x.new_empty(x.shape, dtype=torch.float8_e4m3fn)
     scale = x.new_empty((*x.shape[:-1], hidden // block if block else 1), dtype=torch.float32)
     _lib.call("mrl_norm_fp8_fwd", flat.data_ptr(), _lib.dtype_code(x), x_stride, _lib.ptr(res), _lib.dtype_code(x if res is None else res),
