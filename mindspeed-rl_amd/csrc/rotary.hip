@@ -13,10 +13,9 @@ namespace {
 
 using mrl_vocab::Elem;
 
-constexpr int kBlock = 256;
-constexpr int kWaves = kBlock / 64;
+constexpr int kBlock = 256, kBlockLog = 8;
 // Units of a lane on their way at a time (us, two / four: 32 768 tokens of 32 bf16 heads of 128, there and back, 188 / 178).
-constexpr int kBatch = 4;
+constexpr int kUnits = 4;
 // Bytes read and written that the memory-side cache holds; more go past the caches (us, through / past: the same 196 / 178, 9 477 tokens
 // of 17 fp16 heads of 192 24.7 / 32.6).
 constexpr int64_t kCached = 256 << 20;
@@ -25,8 +24,8 @@ struct Side {                               // queries or keys
     const void* x;
     void* out;                              // [tokens, heads, dim], dense
     int64_t outer, inner, head;             // strides of x
-    int32_t heads, dim, start;
-    int32_t units, copied;                  // units of a head: pairs, then what is copied, so many entries each
+    int32_t heads, dim, start, units;       // units of a head: turned ones, then copied ones
+    int32_t front, copied;                  // vectors in front of the turned part, and of all that is copied
 };
 
 struct Args {
@@ -34,7 +33,7 @@ struct Args {
     const void* positions;
     int64_t pos_outer, pos_inner;
     const double* inv_freq;
-    int32_t n_tokens, n_inner, part, pos_wide, interleaved, splits;
+    int32_t n_tokens, n_inner, part, turned, pos_wide, interleaved, splits, lanes_log;
     float scale, sign;
 };
 
@@ -111,18 +110,37 @@ __device__ __forceinline__ float2 turn_of(double t, float scale, float sign) {
     return make_float2(q == 1 || q == 2 ? -cq * scale : cq * scale, (q >= 2 ? -sq : sq) * sign * scale);
 }
 
-// A wavefront takes a token, or one of `splits` shares of its units.  A unit is kN pairs, or two vectors of kN entries (one, where
-// the layout has it so) that are copied.  Four units a lane are on their way while the sines and cosines of the token's pairs are
-// formed, once, a pair a lane, and put into LDS.
-template <int DT, int kN, bool kInterleaved, bool kStream>
+// A unit is two vectors of kN entries of a head.  Halves: the same place in both.  Interleaved: a vector of each half of the
+// vectors, so that what the lanes take at a time lies together.  Copied entries the same.  The last vector of a stretch that is not whole
+// vectors ends where the stretch ends and overlaps the one in front of it: what lies in both is written twice with the same bits.
+//
+// A token's units are dealt to a wavefront, four to a lane on their way at a time (kBatch; or to `splits` wavefronts, of few tokens), or, where
+// there are no more than 64, one to each of 2^lanes_log lanes.  While they are on their way the sines and cosines of the token's pairs
+// are formed, once, and put into LDS.
+template <int DT, int kN, bool kInterleaved, bool kStream, int kBatch>
 __global__ __launch_bounds__(kBlock) void rotary_kernel(Args a) {
     using T = typename Elem<DT>::T;
-    extern __shared__ float4 turns[];       // cosines, sines: a wavefront's
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), pairs = a.part / 2;
-    const uint32_t item = blockIdx.x * kWaves + wave, token = item / a.splits;
+    constexpr bool kWave = kBatch > 1, kSide = kInterleaved && kN > 1;     // pairs lie side by side in a vector
+    extern __shared__ float2 turns[];       // (cosine, sine) of a token's pairs, after one another
+    const int pairs = a.part / 2;
+    int lane, lanes, slot, base;
+    uint32_t token;
+    if (kWave) {
+        const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), item = blockIdx.x * (kBlock / 64) + wave;
+        lane = threadIdx.x & 63;
+        lanes = 64;
+        slot = wave;
+        token = item / (uint32_t)a.splits;
+        base = (int)(item - token * a.splits) * 64;
+    } else {
+        lanes = 1 << a.lanes_log;
+        lane = threadIdx.x & (lanes - 1);
+        slot = threadIdx.x >> a.lanes_log;
+        token = (blockIdx.x << (kBlockLog - a.lanes_log)) + slot;
+        base = 0;
+    }
     if (token >= (uint32_t)a.n_tokens) return;          // no barrier follows
-    float* cosines = (float*)turns + wave * 2 * pairs;
-    float* sines = cosines + pairs;
+    float2* turn_at = turns + slot * pairs;
     const uint32_t outer = token / (uint32_t)a.n_inner, inner = token - outer * (uint32_t)a.n_inner;
     // what the angles take is requested in front of the entries: a wait for a load is one for those in front of it
     const int64_t place = outer * a.pos_outer + inner * a.pos_inner;
@@ -132,88 +150,87 @@ __global__ __launch_bounds__(kBlock) void rotary_kernel(Args a) {
     const T* from1 = (const T*)a.side[1].x + ((int64_t)outer * a.side[1].outer + (int64_t)inner * a.side[1].inner);
     T* to0 = (T*)a.side[0].out + (int64_t)token * (a.side[0].heads * a.side[0].dim);
     T* to1 = (T*)a.side[1].out + (int64_t)token * (a.side[1].heads * a.side[1].dim);
-    const int turned = pairs / kN;
     const int first = a.side[0].heads * a.side[0].units, all = first + a.side[1].heads * a.side[1].units;
     const int step = 64 * a.splits;
     Pack<DT, kN> va[kBatch], vb[kBatch];
-    int at[kBatch], two[kBatch], unit[kBatch];
+    int one[kBatch], two[kBatch], pair[kBatch], pair2[kBatch];              // pair < 0: copied
     const auto request = [&](int base) {
 #pragma unroll
         for (int q = 0; q < kBatch; ++q) {
             const int wanted = base + q * step + lane, idx = wanted < all ? wanted : all - 1;
             const bool second = idx >= first;
             const int n = second ? idx - first : idx, units = second ? a.side[1].units : a.side[0].units;
-            const int head = (int)((unsigned)n / (unsigned)units), start = second ? a.side[1].start : a.side[0].start;
-            unit[q] = n - head * units;
-            const bool turn = unit[q] < turned;
-            const int copied = second ? a.side[1].copied : a.side[0].copied;
-            int copy = (unit[q] - turned) * copied;
-            copy += copy >= start ? a.part : 0;
-            const int one = turn ? start + unit[q] * (kInterleaved ? 2 * kN : kN) : copy;
-            two[q] = turn ? (kInterleaved ? kN : pairs) : copied - kN;
-            const T* x = (second ? from1 : from0) + head * (second ? a.side[1].head : a.side[0].head) + one;
-            at[q] = head * (second ? a.side[1].dim : a.side[0].dim) + one;
-            va[q].template load<kStream>(x);
-            vb[q].template load<kStream>(x + two[q]);
+            const int head = (int)((unsigned)n / (unsigned)units), unit = n - head * units;
+            const int dim = second ? a.side[1].dim : a.side[0].dim, start = second ? a.side[1].start : a.side[0].start;
+            const int front = second ? a.side[1].front : a.side[0].front, copied = second ? a.side[1].copied : a.side[0].copied;
+            const bool turn = unit < a.turned;
+            int t1, t2;
+            if (kSide) {
+                t1 = min(unit * kN, a.part - kN);
+                t2 = min((unit + a.turned) * kN, a.part - kN);
+                pair[q] = t1 >> 1;
+                pair2[q] = t2 >> 1;
+            } else {
+                const int at = min(unit * kN, pairs - kN);
+                t1 = kInterleaved ? 2 * at : at;
+                t2 = kInterleaved ? 2 * at + 1 : at + pairs;
+                pair[q] = pair2[q] = at;
+            }
+            const int c1 = unit - a.turned, c2 = min(c1 + (copied + 1) / 2, copied - 1), behind = dim - kN;
+            const auto copy = [&](int c) { return c < front ? min(c * kN, start - kN) : min(start + a.part + (c - front) * kN, behind); };
+            t1 = turn ? start + t1 : copy(c1);
+            t2 = turn ? start + t2 : copy(c2);
+            pair[q] = turn ? pair[q] : -1;
+            const T* x = (second ? from1 : from0) + head * (second ? a.side[1].head : a.side[0].head);
+            one[q] = head * dim + t1;
+            two[q] = head * dim + t2;
+            va[q].template load<kStream>(x + t1);
+            vb[q].template load<kStream>(x + t2);
         }
     };
-    int base = (int)(item - token * a.splits) * 64;
     if (base >= all) return;
     request(base);
-    for (int i = lane; i < pairs; i += 64) {
-        const double f = i < 64 ? frequency : a.inv_freq[i];
-        const float2 cs = turn_of(position * (f * 0.15915494309189533577), a.scale, a.sign);
-        cosines[i] = cs.x;
-        sines[i] = cs.y;
+    for (int i = lane; i < pairs; i += lanes) {
+        const double f = i < lanes ? frequency : a.inv_freq[i];
+        turn_at[i] = turn_of(position * (f * 0.15915494309189533577), a.scale, a.sign);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     while (true) {
 #pragma unroll
         for (int q = 0; q < kBatch; ++q) {
-            const bool turn = unit[q] < turned;
-            const int pair = turn ? unit[q] * kN : 0;
-            float z[2 * kN], y[2 * kN], c[kN], sn[kN], za[kN], zb[kN];
-            if constexpr (kN >= 4) {
+            const bool turn = pair[q] >= 0;
+            const float2* t1 = turn_at + (turn ? pair[q] : 0);
+            const float2* t2 = turn_at + (turn ? pair2[q] : 0);
+            float za[kN], zb[kN], ya[kN], yb[kN];
+            va[q].unpack(za);
+            vb[q].unpack(zb);
+            if constexpr (kSide) {
 #pragma unroll
-                for (int i = 0; i < kN; i += 4) {
-                    *(float4*)(c + i) = *(const float4*)(cosines + pair + i);
-                    *(float4*)(sn + i) = *(const float4*)(sines + pair + i);
+                for (int i = 0; i < kN; i += 2) {
+                    const float2 s = t1[i / 2], u = t2[i / 2];
+                    ya[i] = za[i] * s.x - za[i + 1] * s.y;
+                    ya[i + 1] = za[i + 1] * s.x + za[i] * s.y;
+                    yb[i] = zb[i] * u.x - zb[i + 1] * u.y;
+                    yb[i + 1] = zb[i + 1] * u.x + zb[i] * u.y;
                 }
             } else {
 #pragma unroll
                 for (int i = 0; i < kN; ++i) {
-                    c[i] = cosines[pair + i];
-                    sn[i] = sines[pair + i];
+                    const float2 s = t1[i];
+                    ya[i] = za[i] * s.x - zb[i] * s.y;
+                    yb[i] = zb[i] * s.x + za[i] * s.y;
                 }
             }
-            va[q].unpack(za);
-            vb[q].unpack(zb);
-#pragma unroll
-            for (int i = 0; i < kN; ++i) {
-                z[i] = za[i];
-                z[kN + i] = zb[i];
-            }
-#pragma unroll
-            for (int i = 0; i < kN; ++i) {
-                const int p = kInterleaved ? 2 * i : i, r = kInterleaved ? 2 * i + 1 : kN + i;
-                y[p] = z[p] * c[i] - z[r] * sn[i];
-                y[r] = z[r] * c[i] + z[p] * sn[i];
-            }
-#pragma unroll
-            for (int i = 0; i < kN; ++i) {
-                za[i] = y[i];
-                zb[i] = y[kN + i];
-            }
-            Pack<DT, kN> ya, yb;
-            ya.pack(za);
-            yb.pack(zb);
-            ya.v = turn ? ya.v : va[q].v;   // what is copied keeps its bits
-            yb.v = turn ? yb.v : vb[q].v;
+            Pack<DT, kN> pa, pb;
+            pa.pack(ya);
+            pb.pack(yb);
+            pa.v = turn ? pa.v : va[q].v;   // what is copied keeps its bits
+            pb.v = turn ? pb.v : vb[q].v;
             const int idx = base + q * step + lane;
             if (idx < all) {
-                T* out = (idx >= first ? to1 : to0) + at[q];
-                ya.template store<kStream>(out);
-                yb.template store<kStream>(out + two[q]);
+                T* out = idx >= first ? to1 : to0;
+                pa.template store<kStream>(out + one[q]);
+                pb.template store<kStream>(out + two[q]);
             }
         }
         base += kBatch * step;
@@ -222,42 +239,52 @@ __global__ __launch_bounds__(kBlock) void rotary_kernel(Args a) {
     }
 }
 
-template <int DT, int kN>
+template <int DT, int kN, bool kInterleaved>
 void launch(Args a, hipStream_t stream) {
-    const int turned = a.part / 2 / kN;
-    int64_t units = 0;
+    constexpr bool kSide = kInterleaved && kN > 1;
+    const auto vectors = [](int n) { return (n + kN - 1) / kN; };
+    a.turned = kSide ? (vectors(a.part) + 1) / 2 : vectors(a.part / 2);
+    int64_t units = 0, entries = 0;
     for (Side& s : a.side) {
-        s.copied = s.start % (2 * kN) == 0 && (s.dim - a.part) % (2 * kN) == 0 ? 2 * kN : kN;
-        s.units = s.heads ? turned + (s.dim - a.part) / s.copied : 1;
+        s.front = vectors(s.start);
+        s.copied = s.front + vectors(s.dim - a.part - s.start);
+        s.units = s.heads ? a.turned + (s.copied + 1) / 2 : 1;
         units += (int64_t)s.heads * s.units;
+        entries += (int64_t)a.n_tokens * s.heads * s.dim;
     }
+    const bool past = 2 * entries * (int64_t)sizeof(typename Elem<DT>::T) > kCached;
     a.splits = 1;
-    while (a.n_tokens * a.splits < 2048 && units > a.splits * 64) a.splits *= 2;
-    const unsigned groups = (unsigned)((a.n_tokens * a.splits + kWaves - 1) / kWaves);
-    const size_t lds = kWaves * a.part * sizeof(float);
-    int64_t entries = 0;
-    for (const Side& s : a.side) entries += (int64_t)a.n_tokens * s.heads * s.dim;
-    const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(groups), dim3(kBlock), lds, stream, a); };
-    if (2 * entries * (int64_t)sizeof(typename Elem<DT>::T) <= kCached) {
-        if (a.interleaved) go(rotary_kernel<DT, kN, true, false>);
-        else go(rotary_kernel<DT, kN, false, false>);
-    } else {
-        if (a.interleaved) go(rotary_kernel<DT, kN, true, true>);
-        else go(rotary_kernel<DT, kN, false, true>);
+    if (units <= 64) {
+        while ((1 << a.lanes_log) < units) ++a.lanes_log;
+        const int teams = kBlock >> a.lanes_log;
+        const dim3 grid((unsigned)((a.n_tokens + teams - 1) / teams));
+        const size_t lds = (size_t)teams * (a.part / 2) * sizeof(float2);
+        if (past) hipLaunchKernelGGL((rotary_kernel<DT, kN, kInterleaved, true, 1>), grid, dim3(kBlock), lds, stream, a);
+        else hipLaunchKernelGGL((rotary_kernel<DT, kN, kInterleaved, false, 1>), grid, dim3(kBlock), lds, stream, a);
+        return;
     }
+    while (a.n_tokens * a.splits < 2048 && units > a.splits * 64) a.splits *= 2;
+    const int waves = kBlock / 64;
+    const dim3 grid((unsigned)((a.n_tokens * a.splits + waves - 1) / waves));
+    const size_t lds = (size_t)waves * (a.part / 2) * sizeof(float2);
+    if (past) hipLaunchKernelGGL((rotary_kernel<DT, kN, kInterleaved, true, kUnits>), grid, dim3(kBlock), lds, stream, a);
+    else hipLaunchKernelGGL((rotary_kernel<DT, kN, kInterleaved, false, kUnits>), grid, dim3(kBlock), lds, stream, a);
 }
 
-template <int DT>
-void dispatch(const Args& a, hipStream_t stream) {
-    constexpr int kMost = Elem<DT>::kVec;
-    // whole vectors of the turned halves, of what is copied in front of them and behind
-    int fits = a.part / 2;
-    for (const Side& s : a.side)
-        if (s.heads) fits |= s.start | (s.dim - a.part);
-    if (fits % kMost == 0) return launch<DT, kMost>(a, stream);
-    if (fits % 4 == 0) return launch<DT, 4>(a, stream);
-    if (fits % 2 == 0) return launch<DT, 2>(a, stream);
-    launch<DT, 1>(a, stream);
+// The widest vectors that no stretch of a head is shorter than: a half of the turned part (interleaved: the part), what lies
+// in front of it and behind.
+template <int DT, int kN>
+void launch_widest(const Args& a, hipStream_t stream) {
+    bool fits = (a.interleaved ? a.part : a.part / 2) >= kN;
+    for (const Side& s : a.side) {
+        const int behind = s.dim - a.part - s.start;
+        if (s.heads) fits = fits && (s.start == 0 || s.start >= kN) && (behind == 0 || behind >= kN);
+    }
+    if constexpr (kN > 1) {
+        if (!fits) return launch_widest<DT, kN / 2>(a, stream);
+    }
+    if (a.interleaved) launch<DT, kN, true>(a, stream);
+    else launch<DT, kN, false>(a, stream);
 }
 
 }  // namespace
@@ -289,7 +316,7 @@ extern "C" int mrl_rotary(const mrl_rotary_side* q, const mrl_rotary_side* k, in
         MRL_REQUIRE(a.n_tokens == 0 || (s->x && s->out), MRL_ERR_INVALID_ARG, "%s: NULL pointer", fn);
         MRL_REQUIRE(mrl::aligned(s->x, es) && mrl::aligned(s->out, es), MRL_ERR_MISALIGNED, "%s: misaligned buffer", fn);
         a.side[i] = {s->x, s->out, s->stride_outer, s->stride_inner, s->stride_head, (int32_t)s->heads, (int32_t)s->dim,
-                     (int32_t)s->start, 0, 0};
+                     (int32_t)s->start, 0, 0, 0};
     }
     if (a.n_tokens == 0) return MRL_OK;
     MRL_REQUIRE(positions && inv_freq, MRL_ERR_INVALID_ARG, "%s: NULL pointer", fn);
@@ -305,8 +332,8 @@ extern "C" int mrl_rotary(const mrl_rotary_side* q, const mrl_rotary_side* k, in
     a.scale = scale;
     a.sign = back ? -1.f : 1.f;
     hipStream_t s = mrl::as_stream(stream);
-    if (dtype == MRL_F32) dispatch<MRL_F32>(a, s);
-    else if (dtype == MRL_BF16) dispatch<MRL_BF16>(a, s);
-    else dispatch<MRL_F16>(a, s);
+    if (dtype == MRL_F32) launch_widest<MRL_F32, 4>(a, s);
+    else if (dtype == MRL_BF16) launch_widest<MRL_BF16, 8>(a, s);
+    else launch_widest<MRL_F16, 8>(a, s);
     return mrl::check_launch(fn);
 }
