@@ -6,6 +6,9 @@
 // The angle is formed in 64 bits, in turns, and its whole turns are taken off there: at position 2^20 fp32 would be off by 0.06.
 // What is left of it is at most an eighth of a turn off a quarter; sine and cosine of that are their Taylor series in fp32 (terms to x^9 and
 // x^10: what is cut off is below 3e-9).  Entries are turned in fp32 and rounded once.
+//
+// Bound by memory: 32 768 tokens of 32 bf16 heads of 128 (537 MB) 90 us (6.0 TB/s), either layout; heads that end inside lines 4.8 to
+// 5.3 TB/s (72 bf16 59 us).  65 536 tokens of 2 heads of 64: 10 us.  (Here and below: calls that follow each other in a replayed graph.)
 #include "mrl_internal.h"
 #include "vocab_common.h"
 
@@ -16,8 +19,9 @@ using mrl_vocab::Elem;
 constexpr int kBlock = 256, kBlockLog = 8;
 // Units of a lane on their way at a time (us, two / four: 32 768 tokens of 32 bf16 heads of 128, there and back, 188 / 178).
 constexpr int kUnits = 4;
-// Bytes read and written that the memory-side cache holds; more go past the caches (us, through / past: the same 196 / 178, 9 477 tokens
-// of 17 fp16 heads of 192 24.7 / 32.6).
+// Bytes read and written that the memory-side cache holds; more go past the caches, where all stretches are whole lines (us, through /
+// past: 32 768 tokens of 32 bf16 heads of 128 98.8 / 89.6, of 64 fp32 98.0 / 88.1; of 128 with 64 turned 98.0 / 105.9, of 96 75.9 / 89.7; 9 477 of 17
+// fp16 heads of 192, 62 MB, 24.7 / 32.6).
 constexpr int64_t kCached = 256 << 20;
 
 struct Side {                               // queries or keys
@@ -252,7 +256,9 @@ void launch(Args a, hipStream_t stream) {
         units += (int64_t)s.heads * s.units;
         entries += (int64_t)a.n_tokens * s.heads * s.dim;
     }
-    const bool past = 2 * entries * (int64_t)sizeof(typename Elem<DT>::T) > kCached;
+    constexpr int kLine = 128 / sizeof(typename Elem<DT>::T);
+    bool past = 2 * entries * (int64_t)sizeof(typename Elem<DT>::T) > kCached && a.part % (2 * kLine) == 0;
+    for (const Side& s : a.side) past = past && s.dim % kLine == 0 && s.start % kLine == 0;
     a.splits = 1;
     if (units <= 64) {
         while ((1 << a.lanes_log) < units) ++a.lanes_log;
