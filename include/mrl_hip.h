@@ -821,7 +821,7 @@ int mrl_rotary(const mrl_rotary_side* q, const mrl_rotary_side* k, int dtype, co
                const double* inv_freq, int64_t part, int interleaved, float scale, int back, void* stream);
 
 /* mrl_adamw_step: one step of AdamW for every tensor of a list (at most MRL_GRAD_TENSORS), t = step + 1, which is left in `step`:
- *   g' = g * min(1, max_norm / (grad_norm + 1e-6))  (grad_norm NULL: g);  m = beta1 m + (1 - beta1) g';  v = beta2 v + (1 - beta2) g'^2
+ *   g' = g * min(1, max_norm * (1 / (grad_norm + 1e-6)))  (grad_norm NULL: g);  m = beta1 m + (1 - beta1) g';  v = beta2 v + (1 - beta2) g'^2
  *   p = p (1 - lr weight_decay) - m / (sqrt(v) / sqrt(1 - beta2^t) + eps) * lr / (1 - beta1^t)
  * in fp32.  p is `master` (fp32; param is then p rounded) or, without one, param itself (F32, BF16 or F16); grad has the parameter's type or
  * F32 and is only read.  lr: lr_at[0], a device scalar, where that is given.  Nothing is read back: step, lr_at and grad_norm are device

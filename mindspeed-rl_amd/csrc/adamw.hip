@@ -70,7 +70,9 @@ __global__ void adamw_prepare_kernel(int64_t* step, double lr, const float* lr_a
     const int64_t t = *step + 1;
     if (lr_at) lr = (double)*lr_at;
     Coefs c;
-    const float quotient = norm ? max_norm / (*norm + 1e-6f) : 1.f;
+    // max_norm times the reciprocal, each rounded: the bits that torch gives a number over a tensor, its own clipping's among them.  The
+    // moments' codes go up or down by less than a rounding, and a caller who forms the factor there is to find the same ones.
+    const float quotient = norm ? mrl::mul_rn(1.f / (*norm + 1e-6f), max_norm) : 1.f;
     c.factor = quotient > 1.f ? 1.f : quotient;         // NaN, of a norm that is none, stays NaN
     c.decay = (float)(1.0 - lr * weight_decay);
     c.rate = (float)(lr / (1.0 - pow(b1, (double)t)));

@@ -102,7 +102,8 @@ def adamw_(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999), eps
     up or down by a hash of the step and the place, so that the same call gives the same bits).
 
     ``grad_norm`` (the fp32 scalar of :func:`global_grad_norm`) and ``max_norm``: gradients are multiplied by ``min(1, max_norm / (grad_norm + 1e-6))``
-    first, as :func:`clip_grad_norm_` would have it.  ``lr`` may be an fp32 scalar on the device.  ``step`` is counted up on the device, and a
+    first, as :func:`clip_grad_norm_` would have it (but for the factor's last bit, which is that of torch's clipping: ``max_norm`` times the
+    reciprocal).  ``lr`` may be an fp32 scalar on the device.  ``step`` is counted up on the device, and a
     captured call can be replayed.  Gradients have to be finite.  Nothing that is written may share memory with anything else of the call."""
     params, grads, exp_avg, exp_avg_sq = list(params), list(grads), list(exp_avg), list(exp_avg_sq)
     small = exp_avg_scale is not None or exp_avg_sq_scale is not None

@@ -79,8 +79,8 @@ def fp32_moments(g, m, v, factor, b1, b2):
 
 
 def factor_of(norm, limit):
-    """In fp32, by one division (a number over a tensor would be multiplied by the tensor's reciprocal)."""
-    return torch.clamp(torch.full_like(norm, limit) / (norm + 1e-6), max=1.0).item()
+    """As torch gives it: a number over a tensor is the number times the tensor's reciprocal, two roundings."""
+    return torch.clamp(limit / (norm + 1e-6), max=1.0).item()
 
 
 def make(dev, shapes, dtype, gdtype, seed, bits=32, master=True, scale=1e-2):
@@ -243,13 +243,31 @@ def test_clipping_on_the_way(dev, bits):
         copies = clone(params, state)
         mrl.adamw_(params, grads, **state, grad_norm=norm, max_norm=limit, **HYPER)
         check(params, grads, state, old_params, old, factor_of(norm, limit))
-        # the same bits as from clipped gradients
-        clipped = [torch.empty_like(g) for g in grads]
-        mrl.clip_grad_norm_(grads, limit, out=clipped)
+        # the same bits as from gradients that torch's operations have clipped
+        clipped = [g * torch.clamp(limit / (norm + 1e-6), max=1.0) for g in grads]
         mrl.adamw_(copies[0], clipped, **copies[1], **HYPER)
         assert all(torch.equal(a, b) for a, b in zip(params, copies[0]))
+        assert all(torch.equal(a.float(), b.float()) for a, b in zip(state["exp_avg"], copies[1]["exp_avg"]))
+        # and as clip_grad_norm_ scales them, whose factor is one rounding of the quotient: a step and a half of it apart
+        mrl.clip_grad_norm_(grads, limit, out=clipped)
+        for c, g in zip(clipped, grads):
+            assert ((c - g * factor_of(norm, limit)).abs() <= 5 * U * c.abs() + 2.0 ** -149).all()
     mrl.adamw_(params, grads, **state, grad_norm=torch.full((), float("nan"), device=dev), max_norm=1.0, **HYPER)
     assert all(torch.isnan(p).all() for p in params)
+
+
+@pytest.mark.gpu
+def test_the_factor_has_the_bits_of_torch(dev):
+    """Of many norms and limits: the first moment of a first step is (1 - b1) g factor, rounded operation by operation."""
+    gen = torch.Generator().manual_seed(13)
+    g = torch.linspace(0.5, 2.0, 64, device=dev)
+    for _ in range(100):
+        norm = torch.rand((), generator=gen).mul(10).exp().to(dev)
+        limit = float(torch.rand((), generator=gen, dtype=torch.float64)) * norm.item()
+        p = [torch.zeros_like(g)]
+        state = mrl.adamw_state(p)
+        mrl.adamw_(p, [g], **state, lr=1e-3, grad_norm=norm, max_norm=limit)
+        assert torch.equal(state["exp_avg"][0], g * torch.clamp(limit / (norm + 1e-6), max=1.0) * (1 - 0.9))
 
 
 @pytest.mark.gpu
