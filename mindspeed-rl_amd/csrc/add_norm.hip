@@ -64,7 +64,9 @@ __device__ __forceinline__ float weight_at(const void* w, int wide, int j) {
     return wide ? ((const float*)w)[j] : Elem<DT>::load((const typename Elem<DT>::T*)w + j);
 }
 
-// A workgroup a row.
+// ------------------------------------------------------------------------------------ rows of any width
+// Rows that registers do not hold, or shorter than a vector: a workgroup a row, an entry a thread at a time, read again for every sum
+// (from the caches).  4 096 x 40 960 bf16: forward 628 us (2.1 TB/s), backward 961; 100 000 x 7 74 and 117.
 template <int DT, int RT>
 __global__ __launch_bounds__(kBlock) void add_norm_fwd_kernel(FwdArgs a) {
     using T = typename Elem<DT>::T;
