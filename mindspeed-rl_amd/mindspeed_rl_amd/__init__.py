@@ -18,7 +18,7 @@ from .norms import add_rms_norm, layer_norm, rms_norm, rms_norm_fp8
 from .optimizer import adamw_, adamw_state
 from .packing import (generate_mask, pack_index, postprocess_packed_seqs, preprocess_packed_seqs, response_window,
                       truncate_middle_and_pad, truncate_prompt_and_pad)
-from .rotary import rotary, rotary_frequencies
+from .positions import rotary, rotary_frequencies
 from .seqlen_balancing import (balanced_bin_packing, get_reverse_idx, get_seqlen_balanced_partitions, heapq_partition,
                                heapq_partition_with_max, karmarkar_karp, rearrange_micro_batches,
                                split_batches_with_dynamic_bsz)

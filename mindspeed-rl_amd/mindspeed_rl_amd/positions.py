@@ -22,35 +22,38 @@ class RotarySide(ctypes.Structure):
 
 def _turn(xs, positions, inv_freq, interleaved, start, scale, back):
     """The turned tensors of `xs`, dense."""
-    # copies live until the launch: the next one may not take their memory
-    xs = [x.contiguous() if x.stride(-1) != 1 and x.shape[-1] > 1 else x for x in xs]
-    words, outs = [], []
+    words, outs, kept = [], [], []
     for x in xs:
+        strides = x.stride()
+        if strides[-1] != 1:
+            x = x.contiguous()
+            kept.append(x)                  # until the launch: the next copy may not take its memory
+            strides = x.stride()
         shape = x.shape
         out = x.new_empty(shape)
-        *lead, heads, dim = shape
-        *apart, head, _ = x.stride()
-        if len(apart) == 1:
-            lead, apart = (1, *lead), (0, *apart)
-        words += (x.data_ptr(), out.data_ptr(), heads, dim, start if start >= 0 else dim + start, *apart, head)
         outs.append(out)
+        dim = shape[-1]
+        words += (x.data_ptr(), out.data_ptr(), shape[-2], dim, start if start >= 0 else dim + start)
+        words += strides[:3] if len(shape) == 4 else (0, strides[0], strides[1])
     pos = positions.stride()
+    if len(shape) == 4:
+        n_outer, n_inner, pos_outer, pos_inner = shape[0], shape[1], pos[0], pos[1]
+    else:
+        n_outer, n_inner, pos_outer, pos_inner = 1, shape[0], 0, pos[0]
     sides = array.array("q", words)         # struct mrl_rotary_side, one or two
     at = sides.buffer_info()[0]
-    _lib.call("mrl_rotary", at, at + 64 if len(xs) > 1 else None, _lib.dtype_code(out), positions.data_ptr(), _lib.dtype_code(positions),
-              pos[0] if len(pos) > 1 else 0, pos[-1], *lead, inv_freq.data_ptr(), 2 * inv_freq.shape[0], interleaved, scale, back,
+    _lib.call("mrl_rotary", at, at + 64 if len(outs) > 1 else None, _lib.dtype_code(out), positions.data_ptr(), _lib.dtype_code(positions),
+              pos_outer, pos_inner, n_outer, n_inner, inv_freq.data_ptr(), 2 * inv_freq.shape[0], interleaved, scale, back,
               _lib.stream(out.device))
     return outs
 
 
-def _rotary_backward(ctx, *grads):
+def _rotary_backward(ctx, dq, dk):
     positions, inv_freq = ctx.saved_tensors
-    out = [None, None]
-    at = [i for i, g in enumerate(grads) if g is not None and ctx.needs_input_grad[i]]
-    if at:
-        for i, t in zip(at, _turn([grads[i] for i in at], positions, inv_freq, *ctx.meta, True)):
-            out[i] = t
-    return (*out, None, None, None, None, None)
+    need = ctx.needs_input_grad
+    q, k = need[0] and dq is not None, need[1] and dk is not None
+    outs = iter(_turn([g for g, wanted in ((dq, q), (dk, k)) if wanted], positions, inv_freq, *ctx.meta, True) if q or k else ())
+    return next(outs) if q else None, next(outs) if k else None, None, None, None, None, None
 
 
 _rotary_backward_once = once_differentiable(_rotary_backward)
@@ -69,8 +72,8 @@ class _Rotary(torch.autograd.Function):
         return tuple(_turn([q, k], positions, inv_freq, interleaved, start, scale, False))
 
     @staticmethod
-    def backward(ctx, *grads):
-        return _rotary_backward_once(ctx, *grads) if torch.is_grad_enabled() else _rotary_backward(ctx, *grads)
+    def backward(ctx, dq, dk):
+        return _rotary_backward_once(ctx, dq, dk) if torch.is_grad_enabled() else _rotary_backward(ctx, dq, dk)
 
 
 def rotary(q, k, position_ids, inv_freq, interleaved=False, start=0, scale=1.0):

@@ -7,7 +7,7 @@ import torch
 
 import mindspeed_rl_amd as mrl
 from mindspeed_rl_amd import _lib
-from mindspeed_rl_amd.rotary import RotarySide
+from mindspeed_rl_amd.positions import RotarySide
 
 U = 2.0 ** -24                                      # half a step of fp32
 HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
