@@ -12,6 +12,7 @@ from . import _lib
 from .vocab_ops import _flat_rows, _transformed
 
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+_CODES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 
 
 @functools.lru_cache(maxsize=256)
@@ -156,8 +157,8 @@ def _add_forward(x, residual, weight, eps, keep):
         res, r_stride = _flat_rows(residual)
         y, h = x.new_empty(x.shape), residual.new_empty(x.shape)
     rstd = w.new_empty(n_rows, dtype=torch.float32) if keep else None
-    _lib.call("mrl_add_norm_fwd", flat.data_ptr(), _lib.dtype_code(x), x_stride, res.data_ptr(), _lib.dtype_code(h), r_stride,
-              n_rows, hidden, w.data_ptr(), _lib.dtype_code(w), eps, h.data_ptr(), y.data_ptr(), _lib.ptr(rstd), _lib.stream(dev))
+    _lib.call("mrl_add_norm_fwd", flat.data_ptr(), _CODES[x.dtype], x_stride, res.data_ptr(), _CODES[residual.dtype], r_stride,
+              n_rows, hidden, w.data_ptr(), _CODES[w.dtype], eps, h.data_ptr(), y.data_ptr(), _lib.ptr(rstd), _lib.stream(dev))
     return y, h, w, rstd
 
 
@@ -185,8 +186,8 @@ def _add_backward(ctx, dy, dh):
         dw = torch.empty_like(w)
         ws_bytes = _add_workspace_bytes(n_rows, hidden)
         workspace = w.new_empty(ws_bytes, dtype=torch.uint8)
-    _lib.call("mrl_add_norm_bwd", dy.data_ptr(), dy_stride, _lib.ptr(dh), dh_stride, h.data_ptr(), _lib.dtype_code(h), _lib.dtype_code(dy),
-              n_rows, hidden, w.data_ptr(), _lib.dtype_code(w), rstd.data_ptr(), _lib.ptr(dx), _lib.ptr(dr), _lib.ptr(dw),
+    _lib.call("mrl_add_norm_bwd", dy.data_ptr(), dy_stride, _lib.ptr(dh), dh_stride, h.data_ptr(), _CODES[h.dtype], _CODES[dtype],
+              n_rows, hidden, w.data_ptr(), _CODES[w.dtype], rstd.data_ptr(), _lib.ptr(dx), _lib.ptr(dr), _lib.ptr(dw),
               _lib.ptr(workspace), ws_bytes, _lib.stream(dev))
     return dx, dr if dr is not None or not need_r else dx, dw, None
 
@@ -248,8 +249,8 @@ def rms_norm_fp8(x, weight, eps=1e-6, residual=None, block=None):
         h = residual.new_empty(x.shape)
     q = x.new_empty(x.shape, dtype=torch.float8_e4m3fn)
     scale = x.new_empty((*x.shape[:-1], hidden // block if block else 1), dtype=torch.float32)
-    _lib.call("mrl_norm_fp8_fwd", flat.data_ptr(), _lib.dtype_code(x), x_stride, _lib.ptr(res), _lib.dtype_code(x if res is None else res),
-              r_stride, n_rows, hidden, w.data_ptr(), _lib.dtype_code(w), eps, block or 0, _lib.ptr(h), q.data_ptr(), scale.data_ptr(),
+    _lib.call("mrl_norm_fp8_fwd", flat.data_ptr(), _CODES[x.dtype], x_stride, _lib.ptr(res), _CODES[(x if res is None else res).dtype],
+              r_stride, n_rows, hidden, w.data_ptr(), _CODES[w.dtype], eps, block or 0, _lib.ptr(h), q.data_ptr(), scale.data_ptr(),
               _lib.stream(dev))
     return (q, scale) if h is None else (q, scale, h)
 

@@ -11,7 +11,8 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 from .vocab_ops import _transformed
 
-_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+_CODES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+_INTS = {torch.int64: _lib.I64, torch.int32: _lib.I32}
 
 
 class RotarySide(ctypes.Structure):
@@ -42,7 +43,7 @@ def _turn(xs, positions, inv_freq, interleaved, start, scale, back):
         n_outer, n_inner, pos_outer, pos_inner = 1, shape[0], 0, pos[0]
     sides = array.array("q", words)         # struct mrl_rotary_side, one or two
     at = sides.buffer_info()[0]
-    _lib.call("mrl_rotary", at, at + 64 if len(outs) > 1 else None, _lib.dtype_code(out), positions.data_ptr(), _lib.dtype_code(positions),
+    _lib.call("mrl_rotary", at, at + 64 if len(outs) > 1 else None, _CODES[out.dtype], positions.data_ptr(), _INTS[positions.dtype],
               pos_outer, pos_inner, n_outer, n_inner, inv_freq.data_ptr(), 2 * inv_freq.shape[0], interleaved, scale, back,
               _lib.stream(out.device))
     return outs
@@ -93,7 +94,7 @@ def rotary(q, k, position_ids, inv_freq, interleaved=False, start=0, scale=1.0):
         raise TypeError("inv_freq must be float64 or float32 of one dimension, not %s %s" % (inv_freq.dtype, tuple(inv_freq.shape)))
     for name, x in (("q", q), ("k", k)) if k is not None else (("q", q),):
         shape = x.shape
-        if dtype not in _FLOATS or x.dtype is not dtype:
+        if dtype not in _CODES or x.dtype is not dtype:
             raise TypeError("%s must be float32, bfloat16 or float16, and of one type with q: %s" % (name, x.dtype))
         if len(shape) not in (3, 4) or shape[:-2] != lead or shape[-2] < 1:
             raise ValueError("%s must be [tokens, heads, dim] or [batch, tokens, heads, dim], of one batch with q: %s and %s"
@@ -103,7 +104,7 @@ def rotary(q, k, position_ids, inv_freq, interleaved=False, start=0, scale=1.0):
             raise ValueError("%s: %d entries from %d on are not in a head of %d" % (name, part, start, shape[-1]))
     if not math.isfinite(scale):
         raise ValueError("scale must be finite, not %r" % scale)
-    if position_ids.dtype not in (torch.int64, torch.int32):
+    if position_ids.dtype not in _INTS:
         raise TypeError("position_ids must be int64 or int32, not %s" % position_ids.dtype)
     if position_ids.shape != lead:
         if position_ids.dim() == 2 and len(lead) == 1 and position_ids.shape[0] == 1:
