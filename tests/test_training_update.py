@@ -195,3 +195,67 @@ def test_a_scoring_layer_in_eight_bits(dev):
         got, want = stands @ product.double().t(), y.double() @ product.double().t()
         half = (2.0 ** -4 * 1.01 + 2.0 ** -8) * y.double().abs() + 2.0 ** -10 * scale.double().amax(-1, keepdim=True)
         assert ((got - want).abs() <= half @ product.double().abs().t()).all()
+
+
+def _parts(dev, seed):
+    """What one call of each operator takes, and the call."""
+    g = torch.Generator(device=dev).manual_seed(seed)
+    n = lambda *s: torch.randn(*s, generator=g, device=dev)  # noqa: E731
+    x, r, dy, dh, w = n(700, 520).to(BF16), n(700, 520), n(700, 520).to(BF16), n(700, 520), 1 + 0.1 * n(520)
+    q, k, gq, gk = n(300, 6, 64).to(BF16), n(300, 2, 64).to(BF16), n(300, 6, 64).to(BF16), n(300, 2, 64).to(BF16)
+    pos = torch.randint(0, 5000, (300,), generator=g, device=dev)
+    inv, _ = mrl.rotary_frequencies(64, device=dev)
+    params, grads = [n(900, 33), n(5000).to(BF16)], [n(900, 33), n(5000)]
+    state = mrl.adamw_state(params, bits=8)
+
+    def call():
+        ts = [t.detach().requires_grad_() for t in (x, r, w)]
+        y, h = mrl.add_rms_norm(*ts)
+        got = [y.detach(), h.detach(), *torch.autograd.grad([y, h], ts, [dy, dh])]
+        ts = [t.detach().requires_grad_() for t in (q, k)]
+        out = mrl.rotary(*ts, pos, inv)
+        got += [*(t.detach() for t in out), *torch.autograd.grad(out, ts, [gq, gk])]
+        codes, scale = mrl.rms_norm_fp8(x, w)
+        mrl.adamw_(params, grads, **state, lr=1e-3, grad_norm=mrl.global_grad_norm(grads), max_norm=1.0)
+        return [*got, codes.float(), scale, *params, *(t.float() for t in state["exp_avg"] + state["exp_avg_sq"])]
+
+    return call
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once(dev):
+    """Calls that overlap in time, each with a workspace of its own: the bits that they give one after the other."""
+    want = [[[t.clone() for t in call()] for _ in range(6)] for call in (_parts(dev, 1), _parts(dev, 2))]
+    calls, streams = [_parts(dev, 1), _parts(dev, 2)], [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(6):
+        for k in range(2):
+            with torch.cuda.stream(streams[k]):
+                got[k].append([t.clone() for t in calls[k]()])
+    torch.cuda.synchronize()
+    for k in range(2):
+        for a, b in zip(got[k], want[k]):
+            assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+@pytest.mark.gpu
+def test_two_graphs_of_one_pool(dev):
+    """Captured one behind the other into one pool of memory and replayed in turn: the bits of the eager calls."""
+    eager, calls = [_parts(dev, 3), _parts(dev, 4)], [_parts(dev, 3), _parts(dev, 4)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for call in (*eager, *calls):
+            call()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, captured = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], []
+    for k, graph in enumerate(graphs):
+        with torch.cuda.graph(graph, pool=graphs[0].pool() if k else None):
+            captured.append(calls[k]())
+    for _ in range(4):
+        for k in range(2):
+            want = eager[k]()
+            graphs[k].replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(p, q) for p, q in zip(captured[k], want))
