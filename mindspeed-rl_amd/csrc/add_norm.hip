@@ -359,7 +359,8 @@ __global__ __launch_bounds__(1024) void add_norm_fwd_rows_kernel(FwdArgs a, int 
 // The backward in one pass: workgroups stay and take rows in turn, a team a row, and hold the sums over their rows of the lane's
 // columns in registers; the workgroup's sums go to part[group][hidden].
 constexpr int kBwdBlock = 512;              // threads of a workgroup that holds several teams
-constexpr int kBwdGroups = 512;             // most workgroups: two on each of 256 CUs
+// Most workgroups: two on each of 256 CUs (32 768 x 3 584 bf16 156 us, by 768 183, by 1 024 171).
+constexpr int kBwdGroups = 512;
 constexpr int64_t kBwdManyVecs = 4 << 20;   // 64 MiB of rows
 
 template <int DT, int RT, int WDT, int kVecs, int kBlockMost, bool kDh, bool kStream>
@@ -483,8 +484,7 @@ __global__ __launch_bounds__(kBlockMost) void add_norm_bwd_rows_kernel(BwdArgs a
     }
 }
 
-// 16 lanes (not where 32 share a block's scale), then as many wavefronts as `vecs` vectors a lane make, or more vectors where
-// 16 of them are not enough.
+// As many wavefronts as `vecs` vectors a lane make, or more vectors where 16 of them are not enough.
 Team team_of_waves(int64_t nv, int vecs) {
     for (; vecs <= 4; ++vecs) {
         const int64_t lanes = (nv + 64 * vecs - 1) / (64 * vecs) * 64;
@@ -493,22 +493,24 @@ Team team_of_waves(int64_t nv, int vecs) {
     return {0, 0};
 }
 
-// Two vectors of each of x and the residual are on a lane's way, or four of x alone (us, one / two / four: 32 768 x 4 096 bf16
+// Teams of 16 lanes hold up to 32 vectors, without a residual 64 (us, 16 lanes / a wavefront: 65 536 x 256 bf16 25.6 / 31.6, 512 49.0 / 45.3, without a
+// residual 20.4 / 28.1).  Longer rows: two vectors of each of x and the residual are on a lane's way, or four of x alone (us, one / two / four: 32 768 x 4 096 bf16
 // 173 / 171 / 176, to e4m3 by blocks (their codes through the caches) 155 / 158 / 158, without a residual 117 / 84 / 70).
 Team fwd_team_of(int rtype, int64_t hidden, int block, bool residual) {
     const int64_t nv = vectors_of(rtype, hidden);
     if (nv == 0) return {0, 0};
-    if (nv <= 64 && !(block && rtype == MRL_F32)) return team_that_fits(nv, 16, (int)((nv + 15) / 16));
+    if (nv <= (residual ? 32 : 64) && !(block && rtype == MRL_F32)) return team_that_fits(nv, 16, (int)((nv + 15) / 16));
     return team_of_waves(nv, residual ? 2 : 4);
 }
 
-// One vector a lane, the next row requested ahead.  Two (ahead as well) for much data whose rows are 4 or 8 KB: teams of one would be
+// One vector a lane, the next row requested ahead; of rows of 16 vectors by 16 lanes (us, 16 lanes / a wavefront: 65 536 x 128 bf16 18.3 / 28.0, 256
+// by two vectors a lane 42.6 / 32.7).  Two (ahead as well) for much data whose rows are 4 or 8 KB: teams of one would be
 // workgroups of 512 threads then, which take longer (us, one / two: 65 536 x 2 048 bf16 191 / 177, 32 768 x 4 096 191 / 178, 1 536 133 /
 // 142, 32 768 x 3 584 156 / 160, 5 120 228 / 244).  Rows that 1 024 lanes do not hold so: two or, of fp32, four a lane, not ahead.
 Team bwd_team_of(int rtype, int64_t n_rows, int64_t hidden) {
     const int64_t nv = vectors_of(rtype, hidden);
     if (nv == 0) return {0, 0};
-    if (nv <= 32) return team_that_fits(nv, 16, (int)((nv + 15) / 16));
+    if (nv <= 16) return team_that_fits(nv, 16, 1);
     if ((nv == 256 || nv == 512) && n_rows * nv >= kBwdManyVecs) return team_that_fits(nv, nv / 2, 2);
     for (int vecs = 1; vecs <= (rtype == MRL_F32 ? 4 : 2); vecs *= 2) {
         const int64_t lanes = (nv + 64 * vecs - 1) / (64 * vecs) * 64;
@@ -540,6 +542,15 @@ int64_t fwd_groups(const Team& team, int64_t n_rows) {
     return (n_rows + teams - 1) / teams;
 }
 
+// Rows go past the caches where more bytes are read and written than the memory-side cache keeps for what comes next (us, through /
+// past, forward and backward: 67 MB, 65 536 x 128 bf16 11.4 and 18.5 / 13.7 and 19.3; 134 MB, 16 384 x 1 024 25.2 and 31.6 / 23.2 and 29.4; 352 MB,
+// 32 768 x 1 343 72.1 and 71.2 / 69.0 and 67.9; 1 GB, 32 768 x 4 096 183 and 202 / 171 and 177).
+constexpr int64_t kCached = 96 << 20;
+
+bool past_caches(int dtype, int rtype, int64_t entries) {
+    return entries * 2 * (mrl::float_dtype_bytes(dtype) + mrl::float_dtype_bytes(rtype)) > kCached;
+}
+
 // launch(weight's type) for the rows' type or fp32.
 template <int DT, typename F>
 void with_weight(int wide, F launch) {
@@ -562,7 +573,7 @@ void launch_fwd(const FwdArgs& a, hipStream_t stream) {
         hipLaunchKernelGGL((add_norm_fwd_kernel<DT, RT>), grid, block, 0, stream, a);
         return;
     }
-    const bool lines = team.lanes >= 64 && a.hidden * (int64_t)sizeof(typename Elem<DT>::T) % 128 == 0;
+    const bool past = past_caches(DT, RT, a.n_rows * a.hidden);
     const auto launch = [&](auto wdt, auto vecs, auto res, auto fp8, auto nt) {
         hipLaunchKernelGGL((add_norm_fwd_rows_kernel<DT, RT, decltype(wdt)::value, decltype(vecs)::value, decltype(res)::value != 0,
                                                      decltype(fp8)::value != 0, decltype(nt)::value != 0>),
@@ -570,7 +581,7 @@ void launch_fwd(const FwdArgs& a, hipStream_t stream) {
     };
     with_weight<DT>(a.wide_weight, [&](auto wdt) {
         with_vecs(team.vecs, [&](auto vecs) {
-            with_flag(lines, [&](auto nt) {
+            with_flag(past, [&](auto nt) {
                 if (!a.scale) launch(wdt, vecs, Int<1>(), Int<0>(), nt);
                 else if (a.residual) launch(wdt, vecs, Int<1>(), Int<1>(), nt);
                 else if constexpr (DT == RT) launch(wdt, vecs, Int<0>(), Int<1>(), nt);
@@ -591,7 +602,7 @@ void launch_bwd(const BwdArgs& a, hipStream_t stream) {
     };
     if (team.lanes > 0 && a.n_rows > 0 && (a.dx || a.dresidual)) {
         const int groups = bwd_groups(team, a.n_rows), block = bwd_block(team);
-        const bool lines = team.lanes >= 64 && a.hidden * (int64_t)sizeof(typename Elem<DT>::T) % 128 == 0;
+        const bool past = past_caches(DT, RT, a.n_rows * a.hidden);
         BwdArgs b = a;
         if (!a.dweight || groups == 1) b.part = nullptr;
         const size_t lds = a.dweight && block > team.lanes ? (size_t)team.lanes * team.vecs * Elem<RT>::kVec * 4 : 0;
@@ -602,7 +613,7 @@ void launch_bwd(const BwdArgs& a, hipStream_t stream) {
         };
         with_weight<DT>(a.wide_weight, [&](auto wdt) {
             with_flag(a.dh != nullptr, [&](auto dh) {
-                with_flag(lines, [&](auto nt) {
+                with_flag(past, [&](auto nt) {
                     if constexpr (RT == MRL_F32) {
                         if (team.vecs == 4) return launch(wdt, Int<4>(), Int<1024>(), dh, nt);
                     }

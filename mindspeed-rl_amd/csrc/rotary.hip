@@ -260,6 +260,7 @@ void launch(Args a, hipStream_t stream) {
     bool past = 2 * entries * (int64_t)sizeof(typename Elem<DT>::T) > kCached && a.part % (2 * kLine) == 0;
     for (const Side& s : a.side) past = past && s.dim % kLine == 0 && s.start % kLine == 0;
     a.splits = 1;
+    // several tokens a wavefront (us, a token / several: 65 536 tokens of 2 bf16 heads of 64 46.7 / 9.8, of 8 of 128 59.1 / 45.9)
     if (units <= 64) {
         while ((1 << a.lanes_log) < units) ++a.lanes_log;
         const int teams = kBlock >> a.lanes_log;
@@ -269,6 +270,7 @@ void launch(Args a, hipStream_t stream) {
         else hipLaunchKernelGGL((rotary_kernel<DT, kN, kInterleaved, false, 1>), grid, dim3(kBlock), lds, stream, a);
         return;
     }
+    // few tokens by several wavefronts each (us, one / several: 64 tokens of 64 bf16 heads of 128 6.1 / 3.6, 256 of 32 4.5 / 3.8, 1 024 5.8 / 5.6)
     while (a.n_tokens * a.splits < 2048 && units > a.splits * 64) a.splits *= 2;
     const int waves = kBlock / 64;
     const dim3 grid((unsigned)((a.n_tokens * a.splits + waves - 1) / waves));
