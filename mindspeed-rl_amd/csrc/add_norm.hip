@@ -493,9 +493,10 @@ Team team_of_waves(int64_t nv, int vecs) {
     return {0, 0};
 }
 
-// Teams of 16 lanes hold up to 32 vectors, without a residual 64 (us, 16 lanes / a wavefront: 65 536 x 256 bf16 25.6 / 31.6, 512 49.0 / 45.3, without a
-// residual 20.4 / 28.1).  Longer rows: two vectors of each of x and the residual are on a lane's way, or four of x alone (us, one / two / four: 32 768 x 4 096 bf16
-// 173 / 171 / 176, to e4m3 by blocks (their codes through the caches) 155 / 158 / 158, without a residual 117 / 84 / 70).
+// Teams of 16 lanes hold up to 32 vectors, without a residual 64 (us, 16 lanes / a wavefront: 65 536 x 256 bf16 25.6 / 31.6, 512
+// 49.0 / 45.3, to e4m3 without a residual 20.4 / 28.1).  Longer rows: two vectors of each of x and the residual are on a lane's way, or four
+// of x alone (us, one / two / four: 32 768 x 4 096 bf16 173 / 171 / 176, to e4m3 by blocks (their codes through the caches) 155 / 158 /
+// 158, without a residual 117 / 84 / 70).
 Team fwd_team_of(int rtype, int64_t hidden, int block, bool residual) {
     const int64_t nv = vectors_of(rtype, hidden);
     if (nv == 0) return {0, 0};
@@ -503,8 +504,8 @@ Team fwd_team_of(int rtype, int64_t hidden, int block, bool residual) {
     return team_of_waves(nv, residual ? 2 : 4);
 }
 
-// One vector a lane, the next row requested ahead; of rows of 16 vectors by 16 lanes (us, 16 lanes / a wavefront: 65 536 x 128 bf16 18.3 / 28.0, 256
-// by two vectors a lane 42.6 / 32.7).  Two (ahead as well) for much data whose rows are 4 or 8 KB: teams of one would be
+// One vector a lane, the next row requested ahead, by 16 lanes where they hold the row (us, 16 lanes / a wavefront: 65 536 x 128 bf16
+// 18.3 / 28.0, 256 by two vectors a lane 42.6 / 32.7).  Two (ahead as well) for much data whose rows are 4 or 8 KB: teams of one would be
 // workgroups of 512 threads then, which take longer (us, one / two: 65 536 x 2 048 bf16 191 / 177, 32 768 x 4 096 191 / 178, 1 536 133 /
 // 142, 32 768 x 3 584 156 / 160, 5 120 228 / 244).  Rows that 1 024 lanes do not hold so: two or, of fp32, four a lane, not ahead.
 Team bwd_team_of(int rtype, int64_t n_rows, int64_t hidden) {
@@ -543,8 +544,8 @@ int64_t fwd_groups(const Team& team, int64_t n_rows) {
 }
 
 // Rows go past the caches where more bytes are read and written than the memory-side cache keeps for what comes next (us, through /
-// past, forward and backward: 67 MB, 65 536 x 128 bf16 11.4 and 18.5 / 13.7 and 19.3; 134 MB, 16 384 x 1 024 25.2 and 31.6 / 23.2 and 29.4; 352 MB,
-// 32 768 x 1 343 72.1 and 71.2 / 69.0 and 67.9; 1 GB, 32 768 x 4 096 183 and 202 / 171 and 177).
+// past, forward and backward, bf16: 65 536 x 128 (67 MB) 11.4 and 18.5 / 13.7 and 19.3; 16 384 x 1 024 (134 MB) 25.2 and 31.6 / 23.2 and
+// 29.4; 32 768 x 1 343 (352 MB) 72.1 and 71.2 / 69.0 and 67.9; 32 768 x 4 096 (1 GB) 183 and 202 / 171 and 177).
 constexpr int64_t kCached = 96 << 20;
 
 bool past_caches(int dtype, int rtype, int64_t entries) {
