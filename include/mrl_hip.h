@@ -780,9 +780,10 @@ int mrl_grad_clip(const mrl_grad* grads, int64_t n_grads, float max_norm, float*
  * Outputs share no memory with anything else.
  *
  * mrl_norm_fp8_fwd: the same, or (residual and h NULL) the norm of x itself, with y as OCP e4m3 codes q [n_rows, hidden] and
- * scales: scale = max(max |y| / 448, 2^-126) over a row (block 0: scale [n_rows]) or over 128 entries (block 128, hidden
- * whole blocks: scale [n_rows, hidden / 128]), q = y / scale to the nearest, ties to even.  A row (block) with an infinity or NaN has
- * that, or NaN, as its scale. */
+ * scales: scale = max(max |y| * (1/448), 2^-126) over a row (block 0: scale [n_rows]) or over 128 entries (block 128, hidden
+ * whole blocks: scale [n_rows, hidden / 128]), q = y / scale to the nearest, ties to even; y, 1/448, scale and the quotient are fp32 numbers,
+ * each operation rounded once (scales below 2^-93: the quotient within one of its steps).  A row (block) with an infinity or NaN has that, or
+ * NaN, as its scale. */
 int mrl_add_norm_fwd(const void* x, int dtype, int64_t x_stride, const void* residual, int residual_dtype,
                      int64_t residual_stride, int64_t n_rows, int64_t hidden, const void* weight,
                      int weight_dtype, float eps, void* h, void* y, float* rstd, void* stream);

@@ -2,7 +2,7 @@
 //
 //   h = x + residual, rounded to the residual's type;  r = (mean_j h_j^2 + eps)^(-1/2),  n_j = h_j r,  y_j = n_j w_j
 //   d_j = dh_j + r (g_j - n_j mean_i(g_i n_i)),  g_j = dy_j w_j;  dx = dresidual = d, each rounded to its type;  dw_j = sum_rows dy_j n_j
-//   8 bits: s = max(max |y| / 448, 2^-126) over the row or over 128 entries,  q = e4m3(y / s)
+//   8 bits: s = max(max |y| * (1/448), 2^-126) over the row or over 128 entries,  q = e4m3(y / s)
 //
 // What is normalised is h as it is stored: the next layer's residual, this norm and its backward see one value, and the call
 // gives what an addition and a norm behind it give.  Sums are held in fp32.
@@ -47,6 +47,20 @@ __device__ __forceinline__ float scale_of(uint32_t most) {
     const float s = __uint_as_float(most) * (1.f / kMost);
     return s < kLeast ? kLeast : s;         // NaN stays
 }
+
+// Quotients by a scale: y * (1 / s) and a correction by what it leaves of y, which makes it the nearest number to y / s (the
+// reciprocal is, and the rest is exact from |y| = 2^-103 on; below, the last bit may be another).  -0 stays, and numbers under an infinite scale are 0.  us, by the
+// reciprocal alone / so / by the compiler's division: 32 768 x 4 096 bf16 without a residual 67 / 70 / 91, with one 148 / 150 / 150.
+struct Quotient {
+    float s, inv;
+    __device__ __forceinline__ explicit Quotient(float scale) : s(scale), inv(1.f / scale) {
+        if (inv == 0.f) s = 0.f;
+    }
+    __device__ __forceinline__ float of(float y) const {
+        const float q = mrl::mul_rn(y, inv);
+        return __builtin_fmaf(-__builtin_fmaf(q, s, -y), inv, q);
+    }
+};
 
 __device__ __forceinline__ uint8_t code_of(float x) { return (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(x, x, 0, false); }
 
@@ -95,9 +109,10 @@ __global__ __launch_bounds__(kBlock) void add_norm_fwd_kernel(FwdArgs a) {
     if (!a.block) {
         uint32_t most = 0;
         for (int j = threadIdx.x; j < a.hidden; j += kBlock) most = max(most, __float_as_uint(fabsf(value(j))));
-        const float s = scale_of(block_most(most, mlds)), inv = 1.f / s;
+        const float s = scale_of(block_most(most, mlds));
+        const Quotient by(s);
         if (threadIdx.x == 0) a.scale[row] = s;
-        for (int j = threadIdx.x; j < a.hidden; j += kBlock) q[j] = code_of(value(j) * inv);
+        for (int j = threadIdx.x; j < a.hidden; j += kBlock) q[j] = code_of(by.of(value(j)));
         return;
     }
     // a block is two entries of a wavefront's lanes
@@ -119,10 +134,11 @@ __global__ __launch_bounds__(kBlock) void add_norm_fwd_kernel(FwdArgs a) {
         }
 #pragma unroll
         for (int off = 32; off >= 1; off >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, off, 64));
-        const float s = scale_of(most), inv = 1.f / s;
+        const float s = scale_of(most);
+        const Quotient by(s);
         if (lane == 0) a.scale[row * blocks + b] = s;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) q[b * 128 + i * 64 + lane] = code_of(v[i] * inv);
+        for (int i = 0; i < 2; ++i) q[b * 128 + i * 64 + lane] = code_of(by.of(v[i]));
     }
 }
 
@@ -307,7 +323,7 @@ __global__ __launch_bounds__(1024) void add_norm_fwd_rows_kernel(FwdArgs a, int 
         for (int i = 0; i < kVec; ++i) ss += col.own(q, i) ? z[i] * z[i] : 0.f;
     }
     const float r = 1.f / sqrtf(team_sum2(ss, 0.f, lanes, lds).x * (1.f / (float)a.hidden) + a.eps);
-    float inv = 1.f;
+    Quotient by(1.f);
     if (kFp8 && !a.block) {
         uint32_t most = 0;
 #pragma unroll
@@ -319,7 +335,7 @@ __global__ __launch_bounds__(1024) void add_norm_fwd_rows_kernel(FwdArgs a, int 
             for (int i = 0; i < kVec; ++i) most = max(most, __float_as_uint(fabsf(z[i] * r * wf[i])));
         }
         const float s = scale_of(team_most(most, lanes, most_lds));
-        inv = 1.f / s;
+        by = Quotient(s);
         if (live && tl == 0) a.scale[row] = s;
     }
     if (!live) return;
@@ -345,12 +361,12 @@ __global__ __launch_bounds__(1024) void add_norm_fwd_rows_kernel(FwdArgs a, int 
             most = lanes_most(most);
             if (kVec == 4) most = max(most, (uint32_t)__shfl_xor((int)most, 16, 64));
             const float s = scale_of(most);
-            inv = 1.f / s;
+            by = Quotient(s);
             if (q == kVecs - 1 && col.skip) continue;       // lanes behind the row
             if ((tl & (128 / kVec - 1)) == 0) a.scale[at / 128] = s;
         }
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) z[i] *= inv;
+        for (int i = 0; i < kVec; ++i) z[i] = by.of(z[i]);
         store_codes<kStream>((uint8_t*)a.y + at, z);
     }
     if (a.rstd && tl == 0) a.rstd[row] = r;

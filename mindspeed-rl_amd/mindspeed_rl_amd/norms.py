@@ -227,8 +227,8 @@ def add_rms_norm(x, residual, weight, eps=1e-6):
 def rms_norm_fp8(x, weight, eps=1e-6, residual=None, block=None):
     """``(q, scale)``: the RMS norm of ``x`` in 8 bits, for a product that takes OCP e4m3 operands: ``q`` (``torch.float8_e4m3fn``, the shape of
     ``x``) times ``scale`` (fp32) is the norm.  ``block=None``: a scale for each row, ``[..., 1]``; ``block=128``: one for each 128 entries, ``[..., H /
-    128]`` (``H`` a multiple of 128).  ``scale`` is the largest magnitude over 448, at least 2^-126, and ``q`` is rounded to the nearest, ties to
-    even.  With ``residual`` the norm is that of ``h = x + residual`` as in :func:`add_rms_norm`, and ``(q, scale, h)`` is returned.
+    128]`` (``H`` a multiple of 128).  ``scale`` is the largest magnitude times 1/448, at least 2^-126, and ``q`` the fp32 quotient by it rounded to the
+    nearest, ties to even.  With ``residual`` the norm is that of ``h = x + residual`` as in :func:`add_rms_norm`, and ``(q, scale, h)`` is returned.
     A pass without gradients: with inputs that require one it is refused."""
     eps = _added(x, residual, weight, eps)
     if block is not None and block != 128:

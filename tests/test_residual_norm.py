@@ -453,3 +453,50 @@ def test_more_entries_than_31_bits(dev):
     q, s, _ = mrl.rms_norm_fp8(big[0], w, residual=big[1])
     q1, s1, _ = mrl.rms_norm_fp8(x, w, residual=r)
     assert torch.equal(q[-64:].view(torch.uint8), q1.view(torch.uint8)) and torch.equal(s[-64:], s1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hidden", [4, 256, 512, 1024, 4096, 65536])
+@pytest.mark.parametrize("dtype,rtype", [(BF16, None), (F16, F32), (BF16, BF16), (F32, F32), (F32, None)], ids=lambda t: str(t).split(".")[-1])
+def test_codes_are_quotients(dev, dtype, rtype, hidden):
+    """Rows of 1 and -1, whose norm is +- the weight itself, so that y is known to the bit: the scale is max |y| times 1/448, one rounding,
+    and a code the nearest to the fp32 quotient y / scale, ties to even.  Weights lie at and right beside the middle between two codes."""
+    gen = torch.Generator().manual_seed(hidden)
+    for block in (None, 128):
+        if block and hidden % block:
+            continue
+        size = block or hidden
+        most = 1 + torch.rand(hidden // size, 1, generator=gen)
+        s = most * (1 / 448)
+        # 8 to 15 and a half, in the binades below 448
+        middle = (torch.randint(8, 16, (hidden // size, size), generator=gen) + 0.5) * torch.exp2(torch.randint(-12, 5, (hidden // size, size), generator=gen).float())
+        w = (middle * s).clamp(max=most)
+        beside = torch.randint(-1, 2, w.shape, generator=gen)
+        w = torch.where(beside == 0, w, torch.nextafter(w, torch.where(beside > 0, most, 0.0)))
+        w[:, -1:] = most
+        want = (w / s).to(torch.float8_e4m3fn).float().view(-1)
+        ones = torch.randint(0, 2, (5, hidden), generator=gen) * 2.0 - 1
+        x = ones.to(dev, dtype)
+        kw = {} if rtype is None else dict(residual=(2 * x).to(rtype))
+        q, scale, *h = mrl.rms_norm_fp8(-x if kw else x, w.view(-1).to(dev), eps=1e-30, block=block, **kw)
+        assert all(torch.equal(t.float(), x.float()) for t in h)
+        assert torch.equal(scale.cpu(), s.view(1, -1).expand(5, -1))
+        assert torch.equal(q.cpu().float(), want * ones)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hidden", [256, 4096, 65536])
+def test_codes_of_zeros_and_under_an_infinite_scale(dev, hidden):
+    """Numbers over infinity are zeros, infinity over it is NaN; a zero keeps its sign."""
+    w = torch.ones(hidden, device=dev)
+    w[1], w[2] = 0.0, -0.0
+    x = torch.ones(2, hidden, device=dev)
+    for block in (None, 128):
+        q, scale = mrl.rms_norm_fp8(x, w, eps=1e-30, block=block)
+        assert torch.isfinite(scale).all() and (q.view(torch.uint8)[:, 1] == 0).all() and (q.view(torch.uint8)[:, 2] == 0x80).all()
+        bad = w.clone()
+        bad[0] = float("inf")
+        q, scale = mrl.rms_norm_fp8(x, bad, eps=1e-30, block=block)
+        end = block or hidden
+        assert torch.isinf(scale[:, 0]).all() and torch.isnan(q[:, 0].float()).all() and not q[:, 1:end].float().any()
+        assert torch.isfinite(scale[:, 1:]).all() and (q[:, end:].float() == 448).all()
