@@ -222,15 +222,19 @@ __device__ __forceinline__ void step_unit(const Part& p, int64_t at, const Coefs
     Unit<kWT> wu;
     Unit<MRL_F32> mu, vu;
     uint32_t mc, vc;
-    float ms, vs;
-    const int64_t block = kWhole || valid > 0 ? at / 128 : 0;
+    // A lane behind the tensor's end has no block to ask: other lanes write the scales of theirs meanwhile, and what is not finite there
+    // would reach the block that this one shares its reductions with.
+    const bool holds = kWhole || valid > 0;
+    float ms = 0.f, vs = 0.f;
     gu.template load<kWhole>(p.grad, at, valid);
     wu.template load<kWhole>(weights, at, valid);
     if (kSmall) {
         mc = load_codes<kWhole>(p.m, at, valid);
         vc = load_codes<kWhole>(p.v, at, valid);
-        ms = p.m_scale[block];
-        vs = p.v_scale[block];
+        if (holds) {
+            ms = p.m_scale[at / 128];
+            vs = p.v_scale[at / 128];
+        }
     } else {
         mu.template load<kWhole>(p.m, at, valid);
         vu.template load<kWhole>(p.v, at, valid);
@@ -270,9 +274,9 @@ __device__ __forceinline__ void step_unit(const Part& p, int64_t at, const Coefs
         vs = block_scale(root);
         store_codes<kWhole>(p.m, at, valid, codes_of<false>(m, ms, bits));
         store_codes<kWhole>(p.v, at, valid, codes_of<true>(root, vs, bits));
-        if (valid > 0 && (threadIdx.x & 31) == 0) {
-            p.m_scale[block] = ms;
-            p.v_scale[block] = vs;
+        if (holds && (threadIdx.x & 31) == 0) {
+            p.m_scale[at / 128] = ms;
+            p.v_scale[at / 128] = vs;
         }
     } else {
         mu.put(m);

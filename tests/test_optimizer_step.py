@@ -504,3 +504,27 @@ def test_more_entries_than_31_bits(dev):
     for name, x, root in (("exp_avg", m, False), ("exp_avg_sq", v.sqrt(), True)):
         c, s = codes(x, bits, root)
         assert torch.equal(state[name][0][2 ** 31:].double(), c) and torch.equal(state[name + "_scale"][0][2 ** 24:], s)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("worst", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("n", [129, 255, 257, 3 * 1024 + 5, 1024 + 128 + 4])
+def test_a_block_that_is_not_finite_stays_alone(dev, n, worst):
+    """A gradient that is not finite in the first block of a tensor that ends inside its last one, or in the last block itself: after every step all
+    other blocks, the last and not whole one among them, have the bits that they have without it."""
+    for at in (5, n - 1):
+        params, grads, state = make(dev, [(n,), (70,)], BF16, F32, 14, 8)
+        twin, twin_state = clone(params, state)
+        worse = [g.clone() for g in grads]
+        worse[0][at] = worst
+        hit = torch.zeros(-(-n // 128), dtype=torch.bool, device=dev)
+        hit[at // 128] = True
+        rest = ~hit.repeat_interleave(128)[:n]
+        for step in range(3):
+            mrl.adamw_(params, worse if step == 0 else grads, **state, **HYPER)
+            mrl.adamw_(twin, grads, **twin_state, **HYPER)
+            assert torch.isnan(params[0][at]) and not torch.isfinite(state["exp_avg_scale"][0][hit]).any()
+            for mine, other, keep in ((params, twin, rest), *((state[k], twin_state[k], rest) for k in ("master", "exp_avg", "exp_avg_sq")),
+                                      *((state[k], twin_state[k], ~hit) for k in ("exp_avg_scale", "exp_avg_sq_scale"))):
+                assert torch.equal(mine[0][keep].float(), other[0][keep].float()) and torch.equal(mine[1].float(), other[1].float())
+                assert torch.isfinite(other[0].float()).all()
