@@ -805,7 +805,8 @@ int mrl_add_norm_bwd(const void* dy, int64_t dy_stride, const void* dh, int64_t 
 /* mrl_rotary: turns pairs of entries of every head by the angle t = position * inv_freq[i], i = 0 .. part/2 - 1:
  *   (a, b) -> scale * (a cos t - b sin t, b cos t + a sin t);  back != 0: by -t, which is the gradient
  * Of a head the `part` entries from `start` on are turned - pairs are i and i + part/2 of them, or (interleaved) 2i and 2i + 1 -
- * and the others copied.  Tokens are [n_outer, n_inner], fewer than 2^26; x: strides in elements of outer, inner and head, entries of a head
+ * and the others copied.  Tokens are [n_outer, n_inner], fewer than 2^26, and no more than
+ * 2^32 threads hold, 1 to 64 for a token (64 of more than 32 units, which hold up to two vectors of 16 bytes each: at most 2^26 - 4 tokens); x: strides in elements of outer, inner and head, entries of a head
  * dense, only read; out: dense [n_outer, n_inner, heads, dim] of the same type, F32, BF16 or F16.  k is nullable.
  * positions: I32 or I64 of any sign, strides in elements (0: shared); inv_freq: part/2 doubles, in radians.  Angles are formed in 64 bits.
  * part at most MRL_ROTARY_MAX_PART, heads * dim at most MRL_ROTARY_MAX_ROW.  Outputs share no memory with anything else. */

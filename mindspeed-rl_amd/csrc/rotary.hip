@@ -243,8 +243,14 @@ __global__ __launch_bounds__(kBlock) void rotary_kernel(Args a) {
     }
 }
 
+int check_grid(int64_t groups, const Args& a) {
+    MRL_REQUIRE(mrl::launch_fits(groups, kBlock), MRL_ERR_UNSUPPORTED,
+                "mrl_rotary: %d tokens (2^32 threads hold fewer, a wavefront for one of more than 32 units)", a.n_tokens);
+    return MRL_OK;
+}
+
 template <int DT, int kN, bool kInterleaved>
-void launch(Args a, hipStream_t stream) {
+int launch(Args a, hipStream_t stream) {
     constexpr bool kSide = kInterleaved && kN > 1;
     const auto vectors = [](int n) { return (n + kN - 1) / kN; };
     a.turned = kSide ? (vectors(a.part) + 1) / 2 : vectors(a.part / 2);
@@ -264,25 +270,32 @@ void launch(Args a, hipStream_t stream) {
     if (units <= 64) {
         while ((1 << a.lanes_log) < units) ++a.lanes_log;
         const int teams = kBlock >> a.lanes_log;
-        const dim3 grid((unsigned)((a.n_tokens + teams - 1) / teams));
+        const int64_t groups = ((int64_t)a.n_tokens + teams - 1) / teams;
+        const int rc = check_grid(groups, a);
+        if (rc != MRL_OK) return rc;
+        const dim3 grid((unsigned)groups);
         const size_t lds = (size_t)teams * (a.part / 2) * sizeof(float2);
         if (past) hipLaunchKernelGGL((rotary_kernel<DT, kN, kInterleaved, true, 1>), grid, dim3(kBlock), lds, stream, a);
         else hipLaunchKernelGGL((rotary_kernel<DT, kN, kInterleaved, false, 1>), grid, dim3(kBlock), lds, stream, a);
-        return;
+        return MRL_OK;
     }
     // few tokens by several wavefronts each (us, one / several: 64 tokens of 64 bf16 heads of 128 6.1 / 3.6, 256 of 32 4.5 / 3.8, 1 024 5.8 / 5.6)
     while (a.n_tokens * a.splits < 2048 && units > a.splits * 64) a.splits *= 2;
     const int waves = kBlock / 64;
-    const dim3 grid((unsigned)((a.n_tokens * a.splits + waves - 1) / waves));
+    const int64_t groups = ((int64_t)a.n_tokens * a.splits + waves - 1) / waves;
+    const int rc = check_grid(groups, a);
+    if (rc != MRL_OK) return rc;
+    const dim3 grid((unsigned)groups);
     const size_t lds = (size_t)waves * (a.part / 2) * sizeof(float2);
     if (past) hipLaunchKernelGGL((rotary_kernel<DT, kN, kInterleaved, true, kUnits>), grid, dim3(kBlock), lds, stream, a);
     else hipLaunchKernelGGL((rotary_kernel<DT, kN, kInterleaved, false, kUnits>), grid, dim3(kBlock), lds, stream, a);
+    return MRL_OK;
 }
 
 // The widest vectors that no stretch of a head is shorter than: a half of the turned part (interleaved: the part), what lies
 // in front of it and behind.
 template <int DT, int kN>
-void launch_widest(const Args& a, hipStream_t stream) {
+int launch_widest(const Args& a, hipStream_t stream) {
     bool fits = (a.interleaved ? a.part : a.part / 2) >= kN;
     for (const Side& s : a.side) {
         const int behind = s.dim - a.part - s.start;
@@ -291,8 +304,7 @@ void launch_widest(const Args& a, hipStream_t stream) {
     if constexpr (kN > 1) {
         if (!fits) return launch_widest<DT, kN / 2>(a, stream);
     }
-    if (a.interleaved) launch<DT, kN, true>(a, stream);
-    else launch<DT, kN, false>(a, stream);
+    return a.interleaved ? launch<DT, kN, true>(a, stream) : launch<DT, kN, false>(a, stream);
 }
 
 }  // namespace
@@ -340,8 +352,8 @@ extern "C" int mrl_rotary(const mrl_rotary_side* q, const mrl_rotary_side* k, in
     a.scale = scale;
     a.sign = back ? -1.f : 1.f;
     hipStream_t s = mrl::as_stream(stream);
-    if (dtype == MRL_F32) launch_widest<MRL_F32, 4>(a, s);
-    else if (dtype == MRL_BF16) launch_widest<MRL_BF16, 8>(a, s);
-    else launch_widest<MRL_F16, 8>(a, s);
-    return mrl::check_launch(fn);
+    const int rc = dtype == MRL_F32 ? launch_widest<MRL_F32, 4>(a, s)
+                   : dtype == MRL_BF16 ? launch_widest<MRL_BF16, 8>(a, s)
+                                       : launch_widest<MRL_F16, 8>(a, s);
+    return rc != MRL_OK ? rc : mrl::check_launch(fn);
 }

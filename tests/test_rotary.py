@@ -338,3 +338,35 @@ def test_more_entries_than_31_bits(dev):
     positions[-64:] = pos
     y, _ = mrl.rotary(q, None, positions, inv)
     assert torch.equal(y[-64:], mrl.rotary(tail, None, pos, inv)[0]) and not y[:-64].any()
+
+
+def test_entry_point_refuses_launches_that_do_not_fit():
+    """A wavefront a token of more than 32 units, four in a workgroup of 256 threads: from 2^26 - 3 tokens on that is 2^32 threads.  In front of
+    any launch, so the buffers may be anything."""
+    lib = _lib.load()
+    buf = (ctypes.c_char * 64)()
+    p = (ctypes.addressof(buf) + 15) // 16 * 16
+    for heads, dim, part in ((33, 2, 2), (64, 2, 2), (65, 2, 2), (40, 128, 128)):
+        side = RotarySide(p, p, heads, dim, 0, 0, heads * dim, dim)
+        for tokens in (2 ** 26 - 3, 2 ** 26 - 1):
+            for dtype in (_lib.F32, _lib.BF16):
+                for shape in ((1, tokens), (tokens, 1)):
+                    rc = lib.mrl_rotary(ctypes.addressof(side), None, dtype, p, _lib.I64, 0, 1, *shape, p, part, 0, 1.0, 0, None)
+                    assert rc == -2 and b"threads" in lib.mrl_last_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,heads", [(2 ** 26 - 1, 2), (2 ** 26 - 4, 33)])
+def test_as_many_tokens_as_a_launch_holds(dev, tokens, heads):
+    """The last tokens have the bits that they alone have; one more of many heads is refused."""
+    inv, _ = mrl.rotary_frequencies(2, device=dev)
+    q = torch.zeros(tokens, heads, 2, dtype=BF16, device=dev)
+    (tail, _), _, pos = make(dev, 5, (heads, 1), (2, 2), BF16, 6)
+    q[-5:] = tail
+    positions = torch.zeros(tokens, dtype=torch.int32, device=dev)
+    positions[-5:] = pos
+    y, _ = mrl.rotary(q, None, positions, inv)
+    assert torch.equal(y[-5:], mrl.rotary(tail, None, pos, inv)[0]) and not y[:-5].any()
+    if heads > 32:
+        with pytest.raises(_lib.MrlError, match="threads"):
+            mrl.rotary(q[:1].expand(tokens + 1, heads, 2), None, positions[:1].expand(tokens + 1), inv)
