@@ -377,7 +377,7 @@ __global__ __launch_bounds__(1024) void add_norm_fwd_rows_kernel(FwdArgs a, int 
 constexpr int kBwdBlock = 512;              // threads of a workgroup that holds several teams
 // Most workgroups: two on each of 256 CUs (32 768 x 3 584 bf16 156 us, by 768 183, by 1 024 171).
 constexpr int kBwdGroups = 512;
-constexpr int64_t kBwdManyVecs = 4 << 20;   // 64 MiB of rows
+constexpr int64_t kBwdManyVecs = 8 << 20;   // 128 MiB of rows
 
 template <int DT, int RT, int WDT, int kVecs, int kBlockMost, bool kDh, bool kStream>
 __global__ __launch_bounds__(kBlockMost) void add_norm_bwd_rows_kernel(BwdArgs a, int lanes, void* __restrict__ dweight) {
@@ -521,14 +521,19 @@ Team fwd_team_of(int rtype, int64_t hidden, int block, bool residual) {
 }
 
 // One vector a lane, the next row requested ahead, by 16 lanes where they hold the row (us, 16 lanes / a wavefront: 65 536 x 128 bf16
-// 18.3 / 28.0, 256 by two vectors a lane 42.6 / 32.7).  Two (ahead as well) for much data whose rows are 4 or 8 KB: teams of one would be
-// workgroups of 512 threads then, which take longer (us, one / two: 65 536 x 2 048 bf16 191 / 177, 32 768 x 4 096 191 / 178, 1 536 133 /
-// 142, 32 768 x 3 584 156 / 160, 5 120 228 / 244).  Rows that 1 024 lanes do not hold so: two or, of fp32, four a lane, not ahead.
+// 18.3 / 28.0, 256 by two vectors a lane 42.6 / 32.7).  Two (ahead as well) for much data where teams of one fill a workgroup of 512 threads by one
+// or two and the second vector leaves few lanes idle: a sixteenth of 16 bits, none of fp32.  us, one / two, by MiB of rows: bf16, 256 MiB: 1 600 wide 177 / 186,
+// 1 792 181 / 185, 1 920 189 / 185, 2 000 193 / 187, 2 048 190 / 181, 4 000 197 / 185, 4 096 193 / 181, workgroups of other sizes 1 536 175 / 185,
+// 3 584 177 / 181, 5 120 183 / 188, four teams 1 024 189 / 195; fp32: 1 000 192 / 196, 1 024 188 / 184, 2 000 193 / 194, 2 048 188 / 184.  By data: 2 048
+// bf16 64 MiB 52 / 56, 96 76 / 76, 128 96 / 96, 160 122 / 116, 512 412 / 351; 2 000 128 98 / 100, 160 125 / 121.  Rows that 1 024 lanes do not hold so:
+// two or, of fp32, four a lane, not ahead.
 Team bwd_team_of(int rtype, int64_t n_rows, int64_t hidden) {
     const int64_t nv = vectors_of(rtype, hidden);
     if (nv == 0) return {0, 0};
     if (nv <= 16) return team_that_fits(nv, 16, 1);
-    if ((nv == 256 || nv == 512) && n_rows * nv >= kBwdManyVecs) return team_that_fits(nv, nv / 2, 2);
+    const int64_t one = (nv + 63) / 64 * 64;
+    if ((one == kBwdBlock / 2 || one == kBwdBlock) && (one - nv) * 16 <= (rtype == MRL_F32 ? 0 : one) && n_rows * nv >= kBwdManyVecs)
+        return team_that_fits(nv, one / 2, 2);
     for (int vecs = 1; vecs <= (rtype == MRL_F32 ? 4 : 2); vecs *= 2) {
         const int64_t lanes = (nv + 64 * vecs - 1) / (64 * vecs) * 64;
         if (lanes <= 1024) return team_that_fits(nv, lanes, vecs);

@@ -500,3 +500,22 @@ def test_codes_of_zeros_and_under_an_infinite_scale(dev, hidden):
         end = block or hidden
         assert torch.isinf(scale[:, 0]).all() and torch.isnan(q[:, 0].float()).all() and not q[:, 1:end].float().any()
         assert torch.isfinite(scale[:, 1:]).all() and (q[:, end:].float() == 448).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,rtype,rows,hidden", [(BF16, BF16, 32800, 2048), (BF16, BF16, 16500, 4091), (F16, F16, 17000, 3840), (F32, F32, 33001, 1022),
+                                                     (F32, F32, 16400, 2048), (F16, F32, 32790, 1024), (BF16, F32, 16401, 2045)], ids=str)
+def test_much_data_in_teams_of_two_vectors(dev, dtype, rtype, rows, hidden):
+    """128 MiB of rows that two vectors a lane hold, whole and not, with and without a gradient of the sum."""
+    x, r, w, dy, dh = make(dev, (rows, hidden), dtype, rtype, dtype, 15)
+    leaves = [t.requires_grad_() for t in (x, r, w)]
+    for up in (dh, None):
+        y, h = mrl.add_rms_norm(x, r, w, 1e-5)
+        grads = torch.autograd.grad([y] if up is None else [y, h], leaves, [dy] if up is None else [dy, up])
+        with torch.no_grad():
+            want = formula(x, r, w, 1e-5, dy, up)
+            assert torch.equal(h, want["h"])
+            within(y.detach(), want["y"])
+            for name, g in zip(("dx", "dr", "dw"), grads):
+                within(g, want[name])
+        del want, y, h, grads
