@@ -519,3 +519,36 @@ def test_much_data_in_teams_of_two_vectors(dev, dtype, rtype, rows, hidden):
             for name, g in zip(("dx", "dr", "dw"), grads):
                 within(g, want[name])
         del want, y, h, grads
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,rtype,rows,hidden", [(BF16, BF16, 13001, 1024), (BF16, BF16, 101, 128 * 1024), (F16, F32, 8300, 1024), (F32, F32, 50000, 128), (BF16, BF16, 26001, 512)],
+                         ids=str)
+def test_much_data_in_eight_bits(dev, dtype, rtype, rows, hidden):
+    """Past the caches: more than 96 MiB read and written."""
+    x, r, w, _, _ = make(dev, (rows, hidden), dtype, rtype, dtype, 16)
+    for res in (r, None):
+        for block in (None, 128):
+            want = formula(x, res, w, 1e-5)
+            got = mrl.rms_norm_fp8(x, w, 1e-5, residual=res, block=block)
+            check_codes(got[0].float(), got[1], want["wide"], block)
+            assert res is None or torch.equal(got[2], want["h"])
+
+
+@pytest.mark.gpu
+def test_gradients_behind_31_bits(dev):
+    """Rows behind 2^31 entries have the gradients that they alone have; the weight's is off by the order of its sums alone."""
+    rows, n = 600001, 3584
+    few = make(dev, (64, n), BF16, BF16, BF16, 17)
+    x, r, dy, dh = (torch.zeros(rows, n, dtype=BF16, device=dev) for _ in range(4))
+    for b, t in zip((x, r, dy, dh), (few[0], few[1], few[3], few[4])):
+        b[-64:] = t
+    x, r, w = (t.requires_grad_() for t in (x, r, few[2]))
+    y, h = mrl.add_rms_norm(x, r, w)
+    dx, dw = torch.autograd.grad([y, h], [x, w], [dy, dh])
+    fx, fr = few[0].requires_grad_(), few[1].requires_grad_()
+    small = torch.autograd.grad(mrl.add_rms_norm(fx, fr, w), [fx], [few[3], few[4]])
+    assert torch.equal(dx[-64:], small[0]) and not dx[:-64].any()
+    del y, h, dx
+    with torch.no_grad():
+        within(dw, formula(fx, fr, w, 1e-6, few[3], few[4])["dw"])

@@ -370,3 +370,20 @@ def test_as_many_tokens_as_a_launch_holds(dev, tokens, heads):
     if heads > 32:
         with pytest.raises(_lib.MrlError, match="threads"):
             mrl.rotary(q[:1].expand(tokens + 1, heads, 2), None, positions[:1].expand(tokens + 1), inv)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,interleaved,heads,dim,part,start", [(BF16, True, (32, 2), 128, 128, 0), (F16, False, (7, 1), 256, 128, 128), (F32, False, (2, 2), 64, 64, 0),
+                                                                    (F32, True, (9, 2), 96, 64, 32)], ids=str)
+def test_much_data(dev, dtype, interleaved, heads, dim, part, start):
+    """Past the caches: more than 256 MiB read and written, heads of whole lines; many heads and few, both layouts, there and back."""
+    size = torch.finfo(dtype).bits // 8
+    tokens = (256 << 20) // (2 * sum(heads) * dim * size) + 301
+    inv, _ = mrl.rotary_frequencies(part, base=1e4, device=dev)
+    (q, k), grads, pos = make(dev, tokens, heads, (dim, dim), dtype, 7)
+    q.requires_grad_(), k.requires_grad_()
+    out = mrl.rotary(q, k, pos, inv, interleaved=interleaved, start=start, scale=1.25)
+    got = torch.autograd.grad(out, [q, k], grads)
+    for x, y, g, d in zip((q, k), out, grads, got):
+        within(y.detach(), turned(x.detach(), pos, inv, interleaved, start, 1.25))
+        within(d, turned(g, pos, inv, interleaved, start, 1.25, back=True))
