@@ -20,7 +20,7 @@ _CODES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _li
 
 # what every tensor of a list is asked: the host's time is what a short list takes
 _DATA_PTR, _NUMEL, _CONTIGUOUS, _GET_DEVICE = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous, torch.Tensor.get_device
-_DTYPE, _SHAPE, _LAYOUT, _REQUIRES_GRAD = map(operator.attrgetter, ("dtype", "shape", "layout", "requires_grad"))
+_DTYPE, _SHAPE, _LAYOUT, _REQUIRES_GRAD, _IS_LEAF = map(operator.attrgetter, ("dtype", "shape", "layout", "requires_grad", "is_leaf"))
 
 
 _USUAL = {torch.Tensor, torch.nn.Parameter}
@@ -66,6 +66,8 @@ def _check_params(params):
     shapes = [*map(_SHAPE, params)]
     if False in map(_CONTIGUOUS, params):
         raise ValueError("parameters must be contiguous: of the shapes %s not all are" % [tuple(s) for s in shapes])
+    if False in map(_IS_LEAF, params):
+        raise ValueError("a parameter is the result of a graph: give leaves or detached tensors")
     return shapes, dtypes
 
 
@@ -94,7 +96,7 @@ def adamw_(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999), eps
         ``m = b1 m + (1 - b1) g``, ``v = b2 v + (1 - b2) g^2``,
         ``p = p (1 - lr weight_decay) - m / (sqrt(v) / sqrt(1 - b2^t) + eps) * lr / (1 - b1^t)``, ``t`` the number of this step
 
-    ``params``: contiguous fp32, bf16 or fp16 tensors (leaves that require gradients are meant), ``grads``: for each a gradient of the
+    ``params``: contiguous fp32, bf16 or fp16 tensors (leaves that require gradients are meant; what a graph has computed is refused), ``grads``: for each a gradient of the
     same shape and of the parameter's type or fp32, or None, which leaves its parameter alone.  The others are those of :func:`adamw_state`:
     ``adamw_(params, grads, **state, lr=...)``; parameters with another ``lr`` or ``weight_decay`` take a call and a state of their own.
     ``master``: fp32 weights that the step is taken on; the parameter is their rounded value.  ``exp_avg_scale`` and ``exp_avg_sq_scale``

@@ -528,3 +528,17 @@ def test_a_block_that_is_not_finite_stays_alone(dev, n, worst):
                                       *((state[k], twin_state[k], ~hit) for k in ("exp_avg_scale", "exp_avg_sq_scale"))):
                 assert torch.equal(mine[0][keep].float(), other[0][keep].float()) and torch.equal(mine[1].float(), other[1].float())
                 assert torch.isfinite(other[0].float()).all()
+
+
+def test_parameters_that_a_graph_has_computed_are_refused():
+    """A write to one would change what its graph gives; leaves and detached views of them are looked at further."""
+    leaf = torch.zeros(4, 6, requires_grad=True)
+    held = lambda: [torch.zeros(4, 6)]  # noqa: E731
+    for p in (leaf * 1, leaf.view(4, 6), leaf[:]):
+        with pytest.raises(ValueError, match="graph"):
+            mrl.adamw_([p], held(), held(), held(), torch.zeros((), dtype=torch.int64), lr=1e-3)
+        with pytest.raises(ValueError, match="graph"):
+            mrl.adamw_state([p])
+    for p in (leaf, leaf.detach().view(4, 6)):
+        with pytest.raises(RuntimeError, match="GPU only"):
+            mrl.adamw_([p], held(), held(), held(), torch.zeros((), dtype=torch.int64), lr=1e-3)
