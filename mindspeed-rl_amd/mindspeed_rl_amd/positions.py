@@ -125,7 +125,7 @@ def rotary(q, k, position_ids, inv_freq, interleaved=False, start=0, scale=1.0):
     return (outs[0], outs[1] if k is not None else None)
 
 
-def rotary_frequencies(part, base=10000.0, scaling=None, factor=1.0, trained=None, fast=32.0, slow=1.0, device=None):
+def rotary_frequencies(part, base=10000.0, scaling=None, factor=1.0, trained=None, fast=None, slow=1.0, device=None):
     """``(inv_freq, scale)`` for :func:`rotary`: ``base^(-2 i / part)``, ``i < part / 2``, in fp64, for contexts ``factor`` times as long as the
     ``trained`` positions (``scaling``):
 
@@ -134,6 +134,8 @@ def rotary_frequencies(part, base=10000.0, scaling=None, factor=1.0, trained=Non
     * "yarn": those that turn more than ``fast`` times within the ``trained`` positions stay, those that turn less than ``slow`` times are divided by
       ``factor``, in between (by index) a share of both; ``scale`` is ``0.1 ln(factor) + 1``
     * "bands": the same with the share in between by the number of turns, and ``scale`` 1
+
+    ``fast`` is 32 for "yarn" and 4 for "bands" unless it is given, as the models that use them have it.
     """
     part = int(part)
     if part < 2 or part % 2:
@@ -147,6 +149,7 @@ def rotary_frequencies(part, base=10000.0, scaling=None, factor=1.0, trained=Non
     elif scaling == "linear":
         inv_freq = own / factor
     elif scaling in ("yarn", "bands"):
+        fast = (32.0 if scaling == "yarn" else 4.0) if fast is None else fast
         if trained is None or not trained > 0 or not fast > slow > 0:
             raise ValueError("scaling %r needs trained positions and fast > slow > 0: %r, %r, %r" % (scaling, trained, fast, slow))
         if scaling == "yarn":

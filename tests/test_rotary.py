@@ -387,3 +387,16 @@ def test_much_data(dev, dtype, interleaved, heads, dim, part, start):
     for x, y, g, d in zip((q, k), out, grads, got):
         within(y.detach(), turned(x.detach(), pos, inv, interleaved, start, 1.25))
         within(d, turned(g, pos, inv, interleaved, start, 1.25, back=True))
+
+
+def test_frequencies_have_their_schemes_own_borders():
+    """Unless it is given, a pair stays from 32 turns on ("yarn") or from 4 on ("bands")."""
+    for scaling, fast in (("yarn", 32.0), ("bands", 4.0)):
+        kw = dict(base=5e5, scaling=scaling, factor=8.0, trained=8192)
+        inv, scale = mrl.rotary_frequencies(128, **kw)
+        want, wanted_scale = mrl.rotary_frequencies(128, fast=fast, slow=1.0, **kw)
+        assert torch.equal(inv, want) and scale == wanted_scale
+    own, _ = mrl.rotary_frequencies(128, base=5e5)
+    bands, _ = mrl.rotary_frequencies(128, base=5e5, scaling="bands", factor=8.0, trained=8192)
+    turns = 8192 * own / (2 * math.pi)
+    assert torch.equal(bands[turns >= 4], own[turns >= 4]) and ((turns >= 4) & (turns < 32)).any()
