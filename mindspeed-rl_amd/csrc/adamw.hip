@@ -7,10 +7,12 @@
 // one, so that their bits do not depend on how the compiler joins them.  fp32 main weights are where there are any what p is, and the
 // parameter is p rounded.
 //
-// 8 bits: 128 entries of a tensor in a row share an fp32 scale s = max(max |x| / 448, 2^-126), x being m and sqrt(v) (whose
-// range is half of v's in its logarithm), and are held as e4m3 codes of x / s.  Moments change by less than half a step of such a
+// 8 bits: 128 entries of a tensor in a row share an fp32 scale s = max(max |x| * (1/448), 2^-126), x being m and sqrt(v) (whose
+// range is half of v's in its logarithm), and are held as e4m3 codes of x / s (x times 1 / s, two roundings).  Moments change by less than half a step of such a
 // code from one update to the next, and rounding to the nearest would leave them where they are, so a value goes up or down by a
-// dither u in [0, 1), floor(|x / s| / step + u): on average it moves as it should.  u is the hash of the step's number and
+// dither u in [0, 1), floor(|x / s| / step + u): the mean of what is held, m or sqrt(v), moves as it should.  v is the square of what is
+// held, and every update adds the dither's variance to it: with gradients that differ from update to update it is too large by about half of a code's relative step (independent
+// normal ones: 2.5 % at b2 = 0.95, 5 % at 0.999), and sqrt(v) spreads by such a step.  u is the hash of the step's number and
 // the entry's place, the same for both moments; the same call gives the same bits.  A sqrt(v) above zero keeps at least
 // the least code, so that no m is divided by eps alone because its v was lost.
 #include <algorithm>
@@ -82,7 +84,8 @@ __global__ void adamw_prepare_kernel(int64_t* step, double lr, const float* lr_a
     *step = t;
 }
 
-// 16 bits for the even and 16 for the odd entry of a pair: what multiplications and shifts mix of its number and the step's.
+// 16 bits for the even and 16 for the odd entry of a pair: what multiplications and shifts mix of its number and the step's.  Shifts and constants are those of
+// a published 32-bit mixer, which Chris Wellons found by a search for little bias.
 __device__ __forceinline__ uint32_t dither(uint32_t pair, uint32_t key) {
     uint32_t x = pair ^ key;
     x = (x ^ (x >> 16)) * 0x7feb352du;

@@ -7,8 +7,9 @@
 // What is left of it is at most an eighth of a turn off a quarter; sine and cosine of that are their Taylor series in fp32 (terms to x^9 and
 // x^10: what is cut off is below 3e-9).  Entries are turned in fp32 and rounded once.
 //
-// Bound by memory: 32 768 tokens of 32 bf16 heads of 128 (537 MB) 90 us (6.0 TB/s), either layout; heads that end inside lines 4.8 to
-// 5.3 TB/s (72 bf16 59 us).  65 536 tokens of 2 heads of 64: 10 us.  (Here and below: calls that follow each other in a replayed graph.)
+// Bound by memory: 32 768 tokens of 32 bf16 heads of 128 (537 MB) 90 us (6.0 TB/s), either layout; heads that end inside lines 4.6 to
+// 5.5 TB/s (28 and 4 bf16 heads of 72 56 us; the counters show every byte written to memory once, so it is not lines that go there twice), of 66
+// 3.3 (47 us).  65 536 tokens of 2 heads of 64: 10 us.  (Here and below: calls that follow each other in a replayed graph.)
 #include "mrl_internal.h"
 #include "vocab_common.h"
 
@@ -21,7 +22,7 @@ constexpr int kBlock = 256, kBlockLog = 8;
 constexpr int kUnits = 4;
 // Bytes read and written that the memory-side cache holds; more go past the caches, where all stretches are whole lines (us, through /
 // past: 32 768 tokens of 32 bf16 heads of 128 98.8 / 89.6, of 64 fp32 98.0 / 88.1; of 128 with 64 turned 98.0 / 105.9, of 96 75.9 / 89.7; 9 477 of 17
-// fp16 heads of 192, 62 MB, 24.7 / 32.6).
+// fp16 heads of 192, 124 MB, 24.7 / 32.6).
 constexpr int64_t kCached = 256 << 20;
 
 struct Side {                               // queries or keys

@@ -101,7 +101,9 @@ def adamw_(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999), eps
     ``adamw_(params, grads, **state, lr=...)``; parameters with another ``lr`` or ``weight_decay`` take a call and a state of their own.
     ``master``: fp32 weights that the step is taken on; the parameter is their rounded value.  ``exp_avg_scale`` and ``exp_avg_sq_scale``
     belong to moments in 8 bits (``torch.float8_e4m3fn``: of ``m`` and ``sqrt(v)`` over their scales, blocks of 128 entries, rounded
-    up or down by a hash of the step and the place, so that the same call gives the same bits).
+    up or down by a hash of the step and the place, so that the same call gives the same bits; ``v`` is then held a few percent too large, as
+    the square of what is rounded).  One ``step`` counts for all: a parameter whose gradient was None until now has its first moments corrected as if they had
+    been formed from the beginning.
 
     ``grad_norm`` (the fp32 scalar of :func:`global_grad_norm`) and ``max_norm``: gradients are multiplied by ``min(1, max_norm / (grad_norm + 1e-6))``
     first, as :func:`clip_grad_norm_` would have it (but for the factor's last bit, which is that of torch's clipping: ``max_norm`` times the
